@@ -417,6 +417,90 @@ int mpe_gae(int device, int mode, int64_t n_envs, int32_t n_agents, int32_t n_st
             const uint8_t* dones, const float* last_values, const uint8_t* last_dones, double gamma, double lam, float* adv,
             float* ret, mpe_stream_t stream);
 
+/*
+ * Trainer-side operators: what a training loop runs on the rollout that mpe_gae gave advantages to.  None needs a
+ * handle; errors are reported by mpe_last_error(NULL).  All data pointers are device pointers on `device`; the caller
+ * owns every buffer, the workspaces among them, which are 16-byte aligned, hold nothing between calls and must not be
+ * used by two calls that overlap in time.  Element types: MPE_F32, MPE_BF16, MPE_F16.  Data needs its element's
+ * alignment only.  Sizes and strides count elements.  No entry point allocates, synchronises or keeps anything, so all
+ * of them may be captured into a HIP graph.
+ */
+#define MPE_BF16 2
+#define MPE_F16 3
+
+/*
+ * A layer: y = f(x w^T + bias) + residual, one launch.
+ *   x         T[m][k], row stride ldx >= k (an agent's columns of the observation rows of all agents will do)
+ *   w         T[n][k], row stride ldw >= k
+ *   bias      T[n] or NULL
+ *   residual  T[m][n], row stride ldr >= n, or 0: one row for all; NULL: none
+ *   y         T[m][n], row stride ldy >= n; must not overlap an input, except that y may be the residual itself
+ *   pre       T[m][n] contiguous or NULL: x w^T + bias, rounded to T, which the backward pass of every activation other
+ *             than MPE_ACT_NONE reads
+ * Products are summed in float32 or better; one rounding to T at the end.  m may be 0.
+ * mpe_linear_workspace gives the bytes the two passes need (0 may come back: workspace may then be NULL).
+ */
+#define MPE_ACT_NONE 0
+#define MPE_ACT_TANH 1
+#define MPE_ACT_RELU 2
+#define MPE_ACT_GELU 3  /* z Phi(z), Phi by erf */
+#define MPE_ACT_SILU 4
+int mpe_linear_workspace(int dtype, int activation, int64_t m, int64_t n, int64_t k, int64_t* forward_bytes, int64_t* backward_bytes);
+int mpe_linear_forward(int device, int dtype, int activation, int64_t m, int64_t n, int64_t k, const void* x, int64_t ldx, const void* w,
+                       int64_t ldw, const void* bias, const void* residual, int64_t ldr, void* y, int64_t ldy, void* pre, void* workspace,
+                       int64_t workspace_bytes, mpe_stream_t stream);
+/*
+ * Its gradients from dy = d(objective)/dy, T[m][n] with row stride lddy (>= n, or 0: one row for all):
+ *   dz = dy f'(pre),  dx = dz w  T[m][k] (row stride lddx),  dw = dz^T x  T[n][k],  db = column sums of dz  T[n]
+ * The residual's gradient is dy itself.  dx, dw, db: NULL for what is not wanted.  `pre` is what the forward wrote
+ * (for MPE_ACT_RELU any array with the same signs will do, e.g. y where there was no residual); NULL with MPE_ACT_NONE.
+ * The outputs must not overlap each other or an input.  Sums do not change their order from run to run.
+ */
+int mpe_linear_backward(int device, int dtype, int activation, int64_t m, int64_t n, int64_t k, const void* dy, int64_t lddy, const void* x,
+                        int64_t ldx, const void* w, int64_t ldw, const void* pre, void* dx, int64_t lddx, void* dw, void* db, void* workspace,
+                        int64_t workspace_bytes, mpe_stream_t stream);
+
+/*
+ * The clipped policy loss over `rows` decisions among `v` words (moves), with value loss and entropy bonus.
+ *   logits      T[rows][v], row stride ld >= v
+ *   actions     int32 or int64 [rows] (action_bytes 4 or 8)
+ *   old_logp    float[rows]     log-probability of the action when the rollout was collected
+ *   adv         float[rows]     advantages (mpe_gae)
+ *   mask        uint8[rows][v], row stride ldm >= v, or NULL: 0 forbids the word
+ *   weights     float[rows] or NULL (all 1)
+ *   values, old_values, returns  float[rows], all three or none
+ * Per row, over the allowed words: lp = log softmax(logits)[action], q = exp(lp - old_logp), H the entropy,
+ *   s = min(q adv, clamp(q, 1 - clip, 1 + clip) adv),
+ *   u = max((V - R)^2, (V0 + clamp(V - V0, -value_clip, value_clip) - R)^2) / 2   (value_clip < 0: (V - R)^2 / 2)
+ *   loss  = sum w (-s + value_coef u - entropy_coef H) / sum w
+ *   stats = [sum w (-s), sum w u, sum w H, sum w (lp - old_logp)^2 / 2, sum w [|q - 1| > clip]] / sum w, sum w   (6 floats)
+ * A row is left out, its gradients 0, if its weight is 0 or its action is not in [0, v), is forbidden, or has the logit
+ * -infinity (so also where no word is left); what else the row holds is then not used.  With no row left, loss and stats are 0.  rows may be 0.
+ * The backward pass reads the same inputs, the forward's stats and one device float grad_loss = d(objective)/d(loss) and
+ * writes dlogits T[rows][v] (row stride ldd) and, with values, dvalues float[rows] (NULL: not wanted).
+ */
+#define MPE_PPO_WORKSPACE_BYTES 98304
+int mpe_ppo_loss_forward(int device, int dtype, int64_t rows, int64_t v, const void* logits, int64_t ld, const void* actions, int action_bytes,
+                         const float* old_logp, const float* adv, const uint8_t* mask, int64_t ldm, const float* weights, const float* values,
+                         const float* old_values, const float* returns, double clip, double value_clip, double value_coef,
+                         double entropy_coef, float* loss, float* stats, void* workspace, int64_t workspace_bytes, mpe_stream_t stream);
+int mpe_ppo_loss_backward(int device, int dtype, int64_t rows, int64_t v, const void* logits, int64_t ld, const void* actions, int action_bytes,
+                          const float* old_logp, const float* adv, const uint8_t* mask, int64_t ldm, const float* weights, const float* values,
+                          const float* old_values, const float* returns, double clip, double value_clip, double value_coef,
+                          double entropy_coef, const float* stats, const float* grad_loss, void* dlogits, int64_t ldd, float* dvalues,
+                          mpe_stream_t stream);
+
+/*
+ * Global norm over n tensors, and clipping to it: norm = sqrt(sum of squares of every element), dst = src * f with
+ * f = max_norm / norm where norm > max_norm, else 1 (NaN if the norm is).  src, dst, counts (elements, 0 allowed) and
+ * dtypes are HOST arrays of length n, read before the call returns; the tensors are dense.  dst NULL: the norm alone;
+ * dst[i] == src[i]: in place.  Any other overlap among the tensors is an error of the caller's.  norm: one device float,
+ * or NULL.  The squares are summed in float64, in an order that does not change from run to run.
+ */
+#define MPE_CLIP_WORKSPACE_BYTES 16384
+int mpe_clip_grad_norm(int device, int32_t n, const void* const* src, void* const* dst, const int64_t* counts, const int32_t* dtypes,
+                       double max_norm, float* norm, void* workspace, int64_t workspace_bytes, mpe_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

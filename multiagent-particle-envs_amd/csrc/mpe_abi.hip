@@ -8,6 +8,7 @@
 #include <new>
 
 #include "mpe_launch.hpp"
+#include "mpe_learn.hpp"
 
 using namespace mpe;
 
@@ -621,6 +622,212 @@ int mpe_gae(int device, int mode, int64_t n_envs, int32_t n_agents, int32_t n_st
     e = launch_gae(mode, n_envs, n_agents, n_steps, rewards, values, dones, last_values, last_dones, gamma, lam, adv, ret, (hipStream_t)stream);
     if (e != hipSuccess) return hip_fail(nullptr, e, "mpe_gae");
     return MPE_OK;
+}
+
+// ---- trainer-side operators ----
+
+// Sizes and strides up to 2^40 elements: every offset the kernels form then fits 63 bits.
+static const int64_t SIZE_MAX_ELEMS = (int64_t)1 << 40;
+
+static int check_learn(const char* who, int dtype, int64_t rows, int64_t a, int64_t b) {
+    if (!learn_dtype(dtype)) return fail(nullptr, MPE_ERR_INVALID, "%s: dtype must be MPE_F32, MPE_BF16 or MPE_F16", who);
+    if (rows < 0 || a < 1 || b < 1) return fail(nullptr, MPE_ERR_INVALID, "%s: sizes must be positive (rows may be 0)", who);
+    if (rows > SIZE_MAX_ELEMS || a > 0x7fffffff || b > 0x7fffffff || (rows && (a > SIZE_MAX_ELEMS / rows || b > SIZE_MAX_ELEMS / rows)) || a > SIZE_MAX_ELEMS / b)
+        return fail(nullptr, MPE_ERR_INVALID, "%s: at most 2^40 elements a matrix and 2^31-1 columns", who);
+    return MPE_OK;
+}
+
+static bool misaligned(const void* p, int64_t bytes) { return ((uintptr_t)p & (uintptr_t)(bytes - 1)) != 0; }
+
+static int check_workspace(const char* who, const void* ws, int64_t have, int64_t need) {
+    if (need > 0 && (!ws || have < need || misaligned(ws, 16)))
+        return fail(nullptr, MPE_ERR_INVALID, "%s: needs a 16-byte aligned workspace of %lld bytes", who, (long long)need);
+    return MPE_OK;
+}
+
+// [a, a + na) and [b, b + nb) share a byte
+static bool overlap(const void* a, int64_t na, const void* b, int64_t nb) {
+    return a && b && na > 0 && nb > 0 && (uintptr_t)a < (uintptr_t)b + (uintptr_t)nb && (uintptr_t)b < (uintptr_t)a + (uintptr_t)na;
+}
+
+// bytes from the first to behind the last element of a [rows][cols] matrix
+static int64_t extent(int64_t rows, int64_t cols, int64_t ld, int64_t size) { return rows > 0 ? ((rows - 1) * ld + cols) * size : 0; }
+
+static bool bad_stride(int64_t rows, int64_t ld, int64_t cols, bool broadcast) {
+    if (broadcast && ld == 0) return false;
+    return ld < cols || (rows > 0 && ld > SIZE_MAX_ELEMS / rows);
+}
+
+int mpe_linear_workspace(int dtype, int activation, int64_t m, int64_t n, int64_t k, int64_t* forward_bytes, int64_t* backward_bytes) {
+    const int rc = check_learn("mpe_linear_workspace", dtype, m, n, k);
+    if (rc != MPE_OK) return rc;
+    if (activation < MPE_ACT_NONE || activation > MPE_ACT_SILU) return fail(nullptr, MPE_ERR_INVALID, "mpe_linear_workspace: unknown activation %d", activation);
+    if (forward_bytes) *forward_bytes = linear_forward_workspace(dtype, m, n, k);
+    if (backward_bytes) *backward_bytes = linear_backward_workspace(dtype, activation, m, n, k);
+    return MPE_OK;
+}
+
+int mpe_linear_forward(int device, int dtype, int activation, int64_t m, int64_t n, int64_t k, const void* x, int64_t ldx, const void* w,
+                       int64_t ldw, const void* bias, const void* residual, int64_t ldr, void* y, int64_t ldy, void* pre, void* workspace,
+                       int64_t workspace_bytes, mpe_stream_t stream) {
+    int rc = check_learn("mpe_linear_forward", dtype, m, n, k);
+    if (rc != MPE_OK) return rc;
+    if (activation < MPE_ACT_NONE || activation > MPE_ACT_SILU) return fail(nullptr, MPE_ERR_INVALID, "mpe_linear_forward: unknown activation %d", activation);
+    if (m == 0) return MPE_OK;
+    if (!x || !w || !y) return fail(nullptr, MPE_ERR_INVALID, "mpe_linear_forward: x, w and y must not be NULL");
+    if (bad_stride(m, ldx, k, false) || bad_stride(n, ldw, k, false) || bad_stride(m, ldy, n, false) || (residual && bad_stride(m, ldr, n, true)))
+        return fail(nullptr, MPE_ERR_INVALID, "mpe_linear_forward: a row stride is smaller than its row");
+    const int64_t s = dtype_bytes(dtype), ny = extent(m, n, ldy, s), np = m * n * s;
+    if (misaligned(x, s) || misaligned(w, s) || misaligned(y, s) || misaligned(bias, s) || misaligned(residual, s) || misaligned(pre, s))
+        return fail(nullptr, MPE_ERR_INVALID, "mpe_linear_forward: a buffer is not aligned to its element");
+    if (overlap(y, ny, x, extent(m, k, ldx, s)) || overlap(y, ny, w, extent(n, k, ldw, s)) || overlap(y, ny, bias, n * s) || overlap(y, ny, pre, np) ||
+        overlap(pre, np, x, extent(m, k, ldx, s)) || overlap(pre, np, w, extent(n, k, ldw, s)) || overlap(pre, np, bias, n * s) ||
+        overlap(pre, np, residual, extent(m, n, ldr, s)) || (overlap(y, ny, residual, extent(m, n, ldr, s)) && (y != residual || ldy != ldr)))
+        return fail(nullptr, MPE_ERR_INVALID, "mpe_linear_forward: y and pre must not overlap another buffer (y may be the residual itself)");
+    rc = check_workspace("mpe_linear_forward", workspace, workspace_bytes, linear_forward_workspace(dtype, m, n, k));
+    if (rc != MPE_OK) return rc;
+    DeviceScope scope(device);
+    if (scope.status != hipSuccess) return hip_fail(nullptr, scope.status, "hipSetDevice");
+    LinearArgs a = {};
+    a.dtype = dtype; a.act = activation; a.m = m; a.n = n; a.k = k;
+    a.x = x; a.ldx = ldx; a.w = w; a.ldw = ldw; a.bias = bias; a.residual = residual; a.ldr = ldr; a.y = y; a.ldy = ldy; a.pre = pre; a.ws = workspace;
+    const hipError_t e = launch_linear_forward(a, (hipStream_t)stream);
+    return e == hipSuccess ? MPE_OK : hip_fail(nullptr, e, "mpe_linear_forward");
+}
+
+int mpe_linear_backward(int device, int dtype, int activation, int64_t m, int64_t n, int64_t k, const void* dy, int64_t lddy, const void* x,
+                        int64_t ldx, const void* w, int64_t ldw, const void* pre, void* dx, int64_t lddx, void* dw, void* db, void* workspace,
+                        int64_t workspace_bytes, mpe_stream_t stream) {
+    int rc = check_learn("mpe_linear_backward", dtype, m, n, k);
+    if (rc != MPE_OK) return rc;
+    if (activation < MPE_ACT_NONE || activation > MPE_ACT_SILU) return fail(nullptr, MPE_ERR_INVALID, "mpe_linear_backward: unknown activation %d", activation);
+    if (!dx && !dw && !db) return MPE_OK;
+    if (m > 0 && (!dy || !x || !w || (activation != MPE_ACT_NONE && !pre)))
+        return fail(nullptr, MPE_ERR_INVALID, "mpe_linear_backward: dy, x, w and, with an activation, pre must not be NULL");
+    if (bad_stride(m, lddy, n, true) || bad_stride(m, ldx, k, false) || bad_stride(n, ldw, k, false) || (dx && bad_stride(m, lddx, k, false)))
+        return fail(nullptr, MPE_ERR_INVALID, "mpe_linear_backward: a row stride is smaller than its row");
+    const int64_t s = dtype_bytes(dtype);
+    const void* in[4] = {dy, x, w, activation != MPE_ACT_NONE ? pre : nullptr};
+    const int64_t in_bytes[4] = {extent(m, n, lddy, s), extent(m, k, ldx, s), extent(n, k, ldw, s), m * n * s};
+    void* out[3] = {dx, dw, db};
+    const int64_t out_bytes[3] = {extent(m, k, lddx, s), n * k * s, n * s};
+    for (int i = 0; i < 4; ++i)
+        if (misaligned(in[i], s)) return fail(nullptr, MPE_ERR_INVALID, "mpe_linear_backward: a buffer is not aligned to its element");
+    for (int o = 0; o < 3; ++o) {
+        if (misaligned(out[o], s)) return fail(nullptr, MPE_ERR_INVALID, "mpe_linear_backward: a buffer is not aligned to its element");
+        bool bad = false;
+        for (int i = 0; i < 4; ++i) bad = bad || overlap(out[o], out_bytes[o], in[i], in_bytes[i]);
+        for (int q = 0; q < o; ++q) bad = bad || overlap(out[o], out_bytes[o], out[q], out_bytes[q]);
+        if (bad) return fail(nullptr, MPE_ERR_INVALID, "mpe_linear_backward: dx, dw and db must not overlap another buffer");
+    }
+    rc = check_workspace("mpe_linear_backward", workspace, workspace_bytes, linear_backward_workspace(dtype, activation, m, n, k));
+    if (rc != MPE_OK) return rc;
+    DeviceScope scope(device);
+    if (scope.status != hipSuccess) return hip_fail(nullptr, scope.status, "hipSetDevice");
+    LinearArgs a = {};
+    a.dtype = dtype; a.act = activation; a.m = m; a.n = n; a.k = k;
+    a.dy = dy; a.lddy = lddy; a.x = x; a.ldx = ldx; a.w = w; a.ldw = ldw; a.pre = const_cast<void*>(in[3]);
+    a.dx = dx; a.lddx = lddx; a.dw = dw; a.db = db; a.ws = workspace;
+    const hipError_t e = launch_linear_backward(a, (hipStream_t)stream);
+    return e == hipSuccess ? MPE_OK : hip_fail(nullptr, e, "mpe_linear_backward");
+}
+
+static int check_ppo(const char* who, const PpoArgs& a) {
+    const int rc = check_learn(who, a.dtype, a.rows, a.v, 1);
+    if (rc != MPE_OK) return rc;
+    if (a.action_bytes != 4 && a.action_bytes != 8) return fail(nullptr, MPE_ERR_INVALID, "%s: actions are int32 or int64", who);
+    if (!(a.clip >= 0.0f) || !(a.value_clip == a.value_clip)) return fail(nullptr, MPE_ERR_INVALID, "%s: clip must not be negative", who);
+    if ((a.values != nullptr) != (a.old_values != nullptr) || (a.values != nullptr) != (a.returns != nullptr))
+        return fail(nullptr, MPE_ERR_INVALID, "%s: values, old_values and returns go together", who);
+    if (a.rows == 0) return MPE_OK;
+    if (!a.logits || !a.actions || !a.old_logp || !a.adv) return fail(nullptr, MPE_ERR_INVALID, "%s: logits, actions, old_logp and adv must not be NULL", who);
+    if (bad_stride(a.rows, a.ld, a.v, false) || (a.mask && bad_stride(a.rows, a.ldm, a.v, false)))
+        return fail(nullptr, MPE_ERR_INVALID, "%s: a row stride is smaller than its row", who);
+    if (misaligned(a.logits, dtype_bytes(a.dtype)) || misaligned(a.actions, a.action_bytes) || misaligned(a.old_logp, 4) || misaligned(a.adv, 4) ||
+        misaligned(a.weights, 4) || misaligned(a.values, 4) || misaligned(a.old_values, 4) || misaligned(a.returns, 4))
+        return fail(nullptr, MPE_ERR_INVALID, "%s: a buffer is not aligned to its element", who);
+    return MPE_OK;
+}
+
+static PpoArgs ppo_args(int dtype, int64_t rows, int64_t v, const void* logits, int64_t ld, const void* actions, int action_bytes, const float* old_logp,
+                        const float* adv, const uint8_t* mask, int64_t ldm, const float* weights, const float* values, const float* old_values,
+                        const float* returns, double clip, double value_clip, double value_coef, double entropy_coef) {
+    PpoArgs a = {};
+    a.dtype = dtype; a.rows = rows; a.v = v; a.logits = logits; a.ld = ld; a.actions = actions; a.action_bytes = action_bytes;
+    a.old_logp = old_logp; a.adv = adv; a.mask = mask; a.ldm = ldm; a.weights = weights; a.values = values; a.old_values = old_values; a.returns = returns;
+    a.clip = (float)clip; a.value_clip = (float)value_clip; a.value_coef = (float)value_coef; a.entropy_coef = (float)entropy_coef;
+    return a;
+}
+
+int mpe_ppo_loss_forward(int device, int dtype, int64_t rows, int64_t v, const void* logits, int64_t ld, const void* actions, int action_bytes,
+                         const float* old_logp, const float* adv, const uint8_t* mask, int64_t ldm, const float* weights, const float* values,
+                         const float* old_values, const float* returns, double clip, double value_clip, double value_coef, double entropy_coef,
+                         float* loss, float* stats, void* workspace, int64_t workspace_bytes, mpe_stream_t stream) {
+    PpoArgs a = ppo_args(dtype, rows, v, logits, ld, actions, action_bytes, old_logp, adv, mask, ldm, weights, values, old_values, returns, clip,
+                         value_clip, value_coef, entropy_coef);
+    int rc = check_ppo("mpe_ppo_loss_forward", a);
+    if (rc != MPE_OK) return rc;
+    if (!loss || !stats || misaligned(loss, 4) || misaligned(stats, 4)) return fail(nullptr, MPE_ERR_INVALID, "mpe_ppo_loss_forward: loss and stats must be aligned and not NULL");
+    rc = check_workspace("mpe_ppo_loss_forward", workspace, workspace_bytes, MPE_PPO_WORKSPACE_BYTES);
+    if (rc != MPE_OK) return rc;
+    a.loss = loss; a.stats = stats; a.ws = (double*)workspace;
+    DeviceScope scope(device);
+    if (scope.status != hipSuccess) return hip_fail(nullptr, scope.status, "hipSetDevice");
+    const hipError_t e = launch_ppo_forward(a, (hipStream_t)stream);
+    return e == hipSuccess ? MPE_OK : hip_fail(nullptr, e, "mpe_ppo_loss_forward");
+}
+
+int mpe_ppo_loss_backward(int device, int dtype, int64_t rows, int64_t v, const void* logits, int64_t ld, const void* actions, int action_bytes,
+                          const float* old_logp, const float* adv, const uint8_t* mask, int64_t ldm, const float* weights, const float* values,
+                          const float* old_values, const float* returns, double clip, double value_clip, double value_coef, double entropy_coef,
+                          const float* stats, const float* grad_loss, void* dlogits, int64_t ldd, float* dvalues, mpe_stream_t stream) {
+    PpoArgs a = ppo_args(dtype, rows, v, logits, ld, actions, action_bytes, old_logp, adv, mask, ldm, weights, values, old_values, returns, clip,
+                         value_clip, value_coef, entropy_coef);
+    const int rc = check_ppo("mpe_ppo_loss_backward", a);
+    if (rc != MPE_OK) return rc;
+    if (rows == 0) return MPE_OK;
+    if (!stats || !grad_loss || !dlogits) return fail(nullptr, MPE_ERR_INVALID, "mpe_ppo_loss_backward: stats, grad_loss and dlogits must not be NULL");
+    if (dvalues && !values) return fail(nullptr, MPE_ERR_INVALID, "mpe_ppo_loss_backward: dvalues without values");
+    const int64_t s = dtype_bytes(dtype), nd = extent(rows, v, ldd, s);
+    if (bad_stride(rows, ldd, v, false)) return fail(nullptr, MPE_ERR_INVALID, "mpe_ppo_loss_backward: a row stride is smaller than its row");
+    if (misaligned(dlogits, s) || misaligned(dvalues, 4) || misaligned(stats, 4) || misaligned(grad_loss, 4))
+        return fail(nullptr, MPE_ERR_INVALID, "mpe_ppo_loss_backward: a buffer is not aligned to its element");
+    const void* in[10] = {logits, actions, old_logp, adv, mask, weights, values, old_values, returns, stats};
+    const int64_t in_bytes[10] = {extent(rows, v, ld, s), rows * action_bytes, rows * 4, rows * 4, extent(rows, v, ldm, 1), rows * 4, rows * 4, rows * 4, rows * 4, 24};
+    for (int i = 0; i < 10; ++i)
+        if (overlap(dlogits, nd, in[i], in_bytes[i]) || overlap(dvalues, rows * 4, in[i], in_bytes[i]))
+            return fail(nullptr, MPE_ERR_INVALID, "mpe_ppo_loss_backward: dlogits and dvalues must not overlap another buffer");
+    if (overlap(dlogits, nd, dvalues, rows * 4) || overlap(dlogits, nd, grad_loss, 4) || overlap(dvalues, rows * 4, grad_loss, 4))
+        return fail(nullptr, MPE_ERR_INVALID, "mpe_ppo_loss_backward: dlogits and dvalues must not overlap another buffer");
+    a.stats = const_cast<float*>(stats); a.grad = grad_loss; a.dlogits = dlogits; a.ldd = ldd; a.dvalues = dvalues;
+    DeviceScope scope(device);
+    if (scope.status != hipSuccess) return hip_fail(nullptr, scope.status, "hipSetDevice");
+    const hipError_t e = launch_ppo_backward(a, (hipStream_t)stream);
+    return e == hipSuccess ? MPE_OK : hip_fail(nullptr, e, "mpe_ppo_loss_backward");
+}
+
+int mpe_clip_grad_norm(int device, int32_t n, const void* const* src, void* const* dst, const int64_t* counts, const int32_t* dtypes, double max_norm,
+                       float* norm, void* workspace, int64_t workspace_bytes, mpe_stream_t stream) {
+    if (n < 0 || (n > 0 && (!src || !counts || !dtypes))) return fail(nullptr, MPE_ERR_INVALID, "mpe_clip_grad_norm: src, counts and dtypes must not be NULL");
+    if (!dst && !norm) return fail(nullptr, MPE_ERR_INVALID, "mpe_clip_grad_norm: neither dst nor norm is wanted");
+    if (dst && !(max_norm >= 0.0)) return fail(nullptr, MPE_ERR_INVALID, "mpe_clip_grad_norm: max_norm must not be negative");
+    if (misaligned(norm, 4)) return fail(nullptr, MPE_ERR_INVALID, "mpe_clip_grad_norm: norm is not aligned to its element");
+    for (int32_t i = 0; i < n; ++i) {
+        if (!learn_dtype(dtypes[i])) return fail(nullptr, MPE_ERR_INVALID, "mpe_clip_grad_norm: tensor %d: dtype must be MPE_F32, MPE_BF16 or MPE_F16", i);
+        if (counts[i] < 0 || counts[i] > SIZE_MAX_ELEMS) return fail(nullptr, MPE_ERR_INVALID, "mpe_clip_grad_norm: tensor %d: bad count", i);
+        if (counts[i] == 0) continue;
+        const int64_t s = dtype_bytes(dtypes[i]);
+        if (!src[i] || (dst && !dst[i]) || misaligned(src[i], s) || (dst && misaligned(dst[i], s)))
+            return fail(nullptr, MPE_ERR_INVALID, "mpe_clip_grad_norm: tensor %d: NULL or misaligned", i);
+        if (dst && dst[i] != src[i] && overlap(dst[i], counts[i] * s, src[i], counts[i] * s))
+            return fail(nullptr, MPE_ERR_INVALID, "mpe_clip_grad_norm: tensor %d: source and destination overlap", i);
+    }
+    const int rc = check_workspace("mpe_clip_grad_norm", workspace, workspace_bytes, MPE_CLIP_WORKSPACE_BYTES);
+    if (rc != MPE_OK) return rc;
+    DeviceScope scope(device);
+    if (scope.status != hipSuccess) return hip_fail(nullptr, scope.status, "hipSetDevice");
+    const hipError_t e = launch_clip(n, src, dst, counts, dtypes, max_norm, norm, (double*)workspace, (hipStream_t)stream);
+    return e == hipSuccess ? MPE_OK : hip_fail(nullptr, e, "mpe_clip_grad_norm");
 }
 
 }  // extern "C"

@@ -7,3 +7,4 @@ from .world import Action, Agent, AgentState, Entity, EntityState, Landmark, Wal
 from .scenario import BaseScenario, HipScenario  # noqa: F401
 from .env import MultiAgentEnv, make_env  # noqa: F401
 from .train import BatchedVecEnv, gae  # noqa: F401
+from .learn import clip_grad_norm, clip_grad_norm_, grad_norm, linear, ppo_loss  # noqa: F401

@@ -11,7 +11,9 @@ _HERE = os.path.dirname(os.path.abspath(__file__))
 # MPE_HIP_LIB selects another build of the same library (kernel A/B experiments)
 LIB_PATH = os.environ.get("MPE_HIP_LIB") or os.path.join(_HERE, "libmpe_hip.so")
 
-MPE_F32, MPE_F64 = 0, 1
+MPE_F32, MPE_F64, MPE_BF16, MPE_F16 = 0, 1, 2, 3
+ACT_NONE, ACT_TANH, ACT_RELU, ACT_GELU, ACT_SILU = 0, 1, 2, 3, 4
+CLIP_WORKSPACE_BYTES, PPO_WORKSPACE_BYTES = 16384, 98304
 SCN_NONE, SCN_SPREAD, SCN_TAG, SCN_WORLD_COMM, SCN_SIMPLE, SCN_ADVERSARY, SCN_PUSH = 0, 1, 2, 3, 4, 5, 6
 SCN_SPEAKER_LISTENER, SCN_REFERENCE, SCN_CRYPTO, SCN_PREDATOR_PREY, SCN_CONSENSUS = 7, 8, 9, 10, 11
 SCN_COLLECTOR = 12
@@ -89,6 +91,23 @@ EXPORTS = {
     # (spec, n_envs, dtype, device, u, c, pos, vel, comm, stream): no handle, no allocation
     "mpe_world_step_static": (C.c_int, [C.POINTER(MpeSpec), C.c_int64, C.c_int, C.c_int] + [C.c_void_p] * 5 + [C.c_void_p]),
     # (device, mode, n_envs, n_agents, n_steps, rewards, values, dones, last_values, last_dones, gamma, lam, adv, ret, stream)
+    # (dtype, activation, m, n, k, forward_bytes*, backward_bytes*)
+    "mpe_linear_workspace": (C.c_int, [C.c_int, C.c_int] + [C.c_int64] * 3 + [C.POINTER(C.c_int64)] * 2),
+    # (device, dtype, activation, m, n, k, x, ldx, w, ldw, bias, residual, ldr, y, ldy, pre, workspace, workspace_bytes, stream)
+    "mpe_linear_forward": (C.c_int, [C.c_int] * 3 + [C.c_int64] * 3 + [C.c_void_p, C.c_int64] * 2 + [C.c_void_p] + [C.c_void_p, C.c_int64] * 2
+                           + [C.c_void_p, C.c_void_p, C.c_int64, C.c_void_p]),
+    # (device, dtype, activation, m, n, k, dy, lddy, x, ldx, w, ldw, pre, dx, lddx, dw, db, workspace, workspace_bytes, stream)
+    "mpe_linear_backward": (C.c_int, [C.c_int] * 3 + [C.c_int64] * 3 + [C.c_void_p, C.c_int64] * 3 + [C.c_void_p, C.c_void_p, C.c_int64]
+                            + [C.c_void_p] * 3 + [C.c_int64, C.c_void_p]),
+    # (device, dtype, rows, v, logits, ld, actions, action_bytes, old_logp, adv, mask, ldm, weights, values, old_values, returns, clip,
+    #  value_clip, value_coef, entropy_coef, loss, stats, workspace, workspace_bytes, stream)
+    "mpe_ppo_loss_forward": (C.c_int, [C.c_int, C.c_int, C.c_int64, C.c_int64, C.c_void_p, C.c_int64, C.c_void_p, C.c_int] + [C.c_void_p] * 3
+                             + [C.c_int64] + [C.c_void_p] * 4 + [C.c_double] * 4 + [C.c_void_p] * 3 + [C.c_int64, C.c_void_p]),
+    # (... the same, stats, grad_loss, dlogits, ldd, dvalues, stream)
+    "mpe_ppo_loss_backward": (C.c_int, [C.c_int, C.c_int, C.c_int64, C.c_int64, C.c_void_p, C.c_int64, C.c_void_p, C.c_int] + [C.c_void_p] * 3
+                              + [C.c_int64] + [C.c_void_p] * 4 + [C.c_double] * 4 + [C.c_void_p] * 3 + [C.c_int64, C.c_void_p, C.c_void_p]),
+    # (device, n, src**, dst**, counts*, dtypes*, max_norm, norm, workspace, workspace_bytes, stream): the four arrays in host memory
+    "mpe_clip_grad_norm": (C.c_int, [C.c_int, C.c_int32] + [C.c_void_p] * 4 + [C.c_double, C.c_void_p, C.c_void_p, C.c_int64, C.c_void_p]),
     "mpe_gae": (C.c_int, [C.c_int, C.c_int, C.c_int64, C.c_int32, C.c_int32] + [C.c_void_p] * 5 + [C.c_double, C.c_double] + [C.c_void_p] * 3),
 }
 
