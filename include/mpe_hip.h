@@ -435,9 +435,11 @@ int mpe_gae(int device, int mode, int64_t n_envs, int32_t n_agents, int32_t n_st
  *   bias      T[n] or NULL
  *   residual  T[m][n], row stride ldr >= n, or 0: one row for all; NULL: none
  *   y         T[m][n], row stride ldy >= n; must not overlap an input, except that y may be the residual itself
- *   pre       T[m][n] contiguous or NULL: x w^T + bias, rounded to T, which the backward pass of every activation other
- *             than MPE_ACT_NONE reads
- * Products are summed in float32 or better; one rounding to T at the end.  m may be 0.
+ *   pre       float[m][n] contiguous or NULL: x w^T + bias, which the backward pass of every activation other than
+ *             MPE_ACT_NONE reads (float32 whatever T is: rounded to 16 bits it would cost the gradients more than any
+ *             other step; MPE_ACT_RELU, of which only the sign matters, keeps T[m][n])
+ * Products are summed in float32; one rounding to T at the end.  m may be 0; n, k and the row strides of x, w and dy
+ * reach at most 2^22.
  * mpe_linear_workspace gives the bytes the two passes need (0 may come back: workspace may then be NULL).
  */
 #define MPE_ACT_NONE 0
@@ -445,6 +447,7 @@ int mpe_gae(int device, int mode, int64_t n_envs, int32_t n_agents, int32_t n_st
 #define MPE_ACT_RELU 2
 #define MPE_ACT_GELU 3  /* z Phi(z), Phi by erf */
 #define MPE_ACT_SILU 4
+#define MPE_ACT_TANH_OUT 5
 int mpe_linear_workspace(int dtype, int activation, int64_t m, int64_t n, int64_t k, int64_t* forward_bytes, int64_t* backward_bytes);
 int mpe_linear_forward(int device, int dtype, int activation, int64_t m, int64_t n, int64_t k, const void* x, int64_t ldx, const void* w,
                        int64_t ldw, const void* bias, const void* residual, int64_t ldr, void* y, int64_t ldy, void* pre, void* workspace,
@@ -453,7 +456,9 @@ int mpe_linear_forward(int device, int dtype, int activation, int64_t m, int64_t
  * Its gradients from dy = d(objective)/dy, T[m][n] with row stride lddy (>= n, or 0: one row for all):
  *   dz = dy f'(pre),  dx = dz w  T[m][k] (row stride lddx),  dw = dz^T x  T[n][k],  db = column sums of dz  T[n]
  * The residual's gradient is dy itself.  dx, dw, db: NULL for what is not wanted.  `pre` is what the forward wrote
- * (for MPE_ACT_RELU any array with the same signs will do, e.g. y where there was no residual); NULL with MPE_ACT_NONE.
+ * (for MPE_ACT_RELU any T[m][n] with the same signs will do, e.g. y where there was no residual; with
+ * MPE_ACT_TANH_OUT, which only this pass knows, it is float32 tanh(x w^T + bias)); NULL with MPE_ACT_NONE.
+ * dz is rounded to T where the products are 16-bit.
  * The outputs must not overlap each other or an input.  Sums do not change their order from run to run.
  */
 int mpe_linear_backward(int device, int dtype, int activation, int64_t m, int64_t n, int64_t k, const void* dy, int64_t lddy, const void* x,

@@ -629,6 +629,9 @@ int mpe_gae(int device, int mode, int64_t n_envs, int32_t n_agents, int32_t n_st
 // Sizes and strides up to 2^40 elements: every offset the kernels form then fits 63 bits.
 static const int64_t SIZE_MAX_ELEMS = (int64_t)1 << 40;
 
+// The products form offsets within a tile of 128 rows in 32 bits.
+static const int64_t ROW_MAX = (int64_t)1 << 22;
+
 static int check_learn(const char* who, int dtype, int64_t rows, int64_t a, int64_t b) {
     if (!learn_dtype(dtype)) return fail(nullptr, MPE_ERR_INVALID, "%s: dtype must be MPE_F32, MPE_BF16 or MPE_F16", who);
     if (rows < 0 || a < 1 || b < 1) return fail(nullptr, MPE_ERR_INVALID, "%s: sizes must be positive (rows may be 0)", who);
@@ -653,6 +656,9 @@ static bool overlap(const void* a, int64_t na, const void* b, int64_t nb) {
 // bytes from the first to behind the last element of a [rows][cols] matrix
 static int64_t extent(int64_t rows, int64_t cols, int64_t ld, int64_t size) { return rows > 0 ? ((rows - 1) * ld + cols) * size : 0; }
 
+// what the forward pass saves: float32 pre-activations; of relu only the sign is read and the element type will do
+static int64_t pre_bytes(int dtype, int activation) { return activation == MPE_ACT_RELU ? dtype_bytes(dtype) : 4; }
+
 static bool bad_stride(int64_t rows, int64_t ld, int64_t cols, bool broadcast) {
     if (broadcast && ld == 0) return false;
     return ld < cols || (rows > 0 && ld > SIZE_MAX_ELEMS / rows);
@@ -661,7 +667,7 @@ static bool bad_stride(int64_t rows, int64_t ld, int64_t cols, bool broadcast) {
 int mpe_linear_workspace(int dtype, int activation, int64_t m, int64_t n, int64_t k, int64_t* forward_bytes, int64_t* backward_bytes) {
     const int rc = check_learn("mpe_linear_workspace", dtype, m, n, k);
     if (rc != MPE_OK) return rc;
-    if (activation < MPE_ACT_NONE || activation > MPE_ACT_SILU) return fail(nullptr, MPE_ERR_INVALID, "mpe_linear_workspace: unknown activation %d", activation);
+    if (activation < MPE_ACT_NONE || activation > MPE_ACT_TANH_OUT) return fail(nullptr, MPE_ERR_INVALID, "mpe_linear_workspace: unknown activation %d", activation);
     if (forward_bytes) *forward_bytes = linear_forward_workspace(dtype, m, n, k);
     if (backward_bytes) *backward_bytes = linear_backward_workspace(dtype, activation, m, n, k);
     return MPE_OK;
@@ -675,10 +681,11 @@ int mpe_linear_forward(int device, int dtype, int activation, int64_t m, int64_t
     if (activation < MPE_ACT_NONE || activation > MPE_ACT_SILU) return fail(nullptr, MPE_ERR_INVALID, "mpe_linear_forward: unknown activation %d", activation);
     if (m == 0) return MPE_OK;
     if (!x || !w || !y) return fail(nullptr, MPE_ERR_INVALID, "mpe_linear_forward: x, w and y must not be NULL");
+    if (k > ROW_MAX || n > ROW_MAX || ldx > ROW_MAX || ldw > ROW_MAX) return fail(nullptr, MPE_ERR_INVALID, "mpe_linear_forward: n, k and the row strides of x and w reach at most %lld", (long long)ROW_MAX);
     if (bad_stride(m, ldx, k, false) || bad_stride(n, ldw, k, false) || bad_stride(m, ldy, n, false) || (residual && bad_stride(m, ldr, n, true)))
         return fail(nullptr, MPE_ERR_INVALID, "mpe_linear_forward: a row stride is smaller than its row");
-    const int64_t s = dtype_bytes(dtype), ny = extent(m, n, ldy, s), np = m * n * s;
-    if (misaligned(x, s) || misaligned(w, s) || misaligned(y, s) || misaligned(bias, s) || misaligned(residual, s) || misaligned(pre, s))
+    const int64_t s = dtype_bytes(dtype), ny = extent(m, n, ldy, s), sp = pre_bytes(dtype, activation), np = m * n * sp;
+    if (misaligned(x, s) || misaligned(w, s) || misaligned(y, s) || misaligned(bias, s) || misaligned(residual, s) || misaligned(pre, sp))
         return fail(nullptr, MPE_ERR_INVALID, "mpe_linear_forward: a buffer is not aligned to its element");
     if (overlap(y, ny, x, extent(m, k, ldx, s)) || overlap(y, ny, w, extent(n, k, ldw, s)) || overlap(y, ny, bias, n * s) || overlap(y, ny, pre, np) ||
         overlap(pre, np, x, extent(m, k, ldx, s)) || overlap(pre, np, w, extent(n, k, ldw, s)) || overlap(pre, np, bias, n * s) ||
@@ -700,19 +707,21 @@ int mpe_linear_backward(int device, int dtype, int activation, int64_t m, int64_
                         int64_t workspace_bytes, mpe_stream_t stream) {
     int rc = check_learn("mpe_linear_backward", dtype, m, n, k);
     if (rc != MPE_OK) return rc;
-    if (activation < MPE_ACT_NONE || activation > MPE_ACT_SILU) return fail(nullptr, MPE_ERR_INVALID, "mpe_linear_backward: unknown activation %d", activation);
+    if (activation < MPE_ACT_NONE || activation > MPE_ACT_TANH_OUT) return fail(nullptr, MPE_ERR_INVALID, "mpe_linear_backward: unknown activation %d", activation);
     if (!dx && !dw && !db) return MPE_OK;
     if (m > 0 && (!dy || !x || !w || (activation != MPE_ACT_NONE && !pre)))
         return fail(nullptr, MPE_ERR_INVALID, "mpe_linear_backward: dy, x, w and, with an activation, pre must not be NULL");
+    if (k > ROW_MAX || n > ROW_MAX || ldx > ROW_MAX || ldw > ROW_MAX || lddy > ROW_MAX)
+        return fail(nullptr, MPE_ERR_INVALID, "mpe_linear_backward: n, k and the row strides of x, w and dy reach at most %lld", (long long)ROW_MAX);
     if (bad_stride(m, lddy, n, true) || bad_stride(m, ldx, k, false) || bad_stride(n, ldw, k, false) || (dx && bad_stride(m, lddx, k, false)))
         return fail(nullptr, MPE_ERR_INVALID, "mpe_linear_backward: a row stride is smaller than its row");
-    const int64_t s = dtype_bytes(dtype);
+    const int64_t s = dtype_bytes(dtype), sp = pre_bytes(dtype, activation);
     const void* in[4] = {dy, x, w, activation != MPE_ACT_NONE ? pre : nullptr};
-    const int64_t in_bytes[4] = {extent(m, n, lddy, s), extent(m, k, ldx, s), extent(n, k, ldw, s), m * n * s};
+    const int64_t in_bytes[4] = {extent(m, n, lddy, s), extent(m, k, ldx, s), extent(n, k, ldw, s), m * n * sp};
     void* out[3] = {dx, dw, db};
     const int64_t out_bytes[3] = {extent(m, k, lddx, s), n * k * s, n * s};
     for (int i = 0; i < 4; ++i)
-        if (misaligned(in[i], s)) return fail(nullptr, MPE_ERR_INVALID, "mpe_linear_backward: a buffer is not aligned to its element");
+        if (misaligned(in[i], i == 3 ? sp : s)) return fail(nullptr, MPE_ERR_INVALID, "mpe_linear_backward: a buffer is not aligned to its element");
     for (int o = 0; o < 3; ++o) {
         if (misaligned(out[o], s)) return fail(nullptr, MPE_ERR_INVALID, "mpe_linear_backward: a buffer is not aligned to its element");
         bool bad = false;

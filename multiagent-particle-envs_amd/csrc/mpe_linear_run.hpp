@@ -1,0 +1,158 @@
+// The launches of a layer's two passes for one element type (mpe_linear_<type>.hip instantiate it).
+#pragma once
+#include "mpe_linear_impl.hpp"
+
+namespace mpe {
+
+// ---- dz = dy f'(pre) as an array of its own ----
+template <typename T>
+__global__ __launch_bounds__(256) void slope_pass(long long m, long long n, const T* __restrict__ dy, long long lddy, const void* __restrict__ pre,
+                                                  int act, T* __restrict__ dz) {
+    for (long long at = (long long)blockIdx.x * 256 + threadIdx.x; at < m * n; at += (long long)gridDim.x * 256) {
+        const long long j = at / n, i = at - j * n;
+        const float z = act == MPE_ACT_RELU ? (float)((const T*)pre)[at] : ((const float*)pre)[at];
+        dz[at] = (T)((float)dy[j * lddy + i] * act_slope(act, z));
+    }
+}
+
+// ---- sums of the splits: out[c] = sum_s partial[s][c], in the order of s within a group of rows, then of the groups ----
+template <typename T, int COLS>
+__global__ __launch_bounds__(256) void add_splits(const float* __restrict__ partial, int splits, long long n, T* __restrict__ out) {
+    constexpr int G = 256 / COLS;
+    __shared__ float part[G][COLS];
+    const int c = threadIdx.x % COLS, g = threadIdx.x / COLS;
+    const long long at = (long long)blockIdx.x * COLS + c;
+    float s = 0.0f;
+    if (at < n)
+        for (int k = g; k < splits; k += G) s += partial[(long long)k * n + at];
+    part[g][c] = s;
+    __syncthreads();
+    if (g == 0 && at < n) {
+        for (int k = 1; k < G; ++k) s += part[k][c];
+        out[at] = (T)s;
+    }
+}
+
+template <typename T>
+inline hipError_t launch_add_splits(const float* partial, int splits, long long n, T* out, hipStream_t st) {
+    if (n >= 65536) hipLaunchKernelGGL((add_splits<T, 64>), dim3((unsigned)((n + 63) / 64)), dim3(256), 0, st, partial, splits, n, out);
+    else hipLaunchKernelGGL((add_splits<T, 16>), dim3((unsigned)((n + 15) / 16)), dim3(256), 0, st, partial, splits, n, out);
+    return hipGetLastError();
+}
+
+inline long long tiles_of(long long n, int b) { return (n + b - 1) / b; }
+
+template <typename T, int EPI, int PL, int QL, bool DZ, int BI, int BJ, int WI, int WJ>
+inline hipError_t launch_product(ProductArgs<T> a, int splits, hipStream_t st) {
+    const long long ti = tiles_of(a.ni, BI), tiles = ti * tiles_of(a.nj, BJ);
+    if (tiles * splits > 0x7fffffffLL) return hipErrorInvalidValue;
+    a.ti = (int)ti;
+    a.tiles = (unsigned)tiles;
+    hipLaunchKernelGGL((product<T, EPI, PL, QL, DZ, BI, BJ, WI, WJ>), dim3((unsigned)(tiles * splits)), dim3(256), 0, st, a);
+    return hipGetLastError();
+}
+
+// Tiles of the products that write rows of m: by the output's width.
+template <typename T, int EPI, int PL, int QL, bool DZ>
+inline hipError_t launch_rows(const ProductArgs<T>& a, hipStream_t st) {
+    if (a.ni <= 16) return launch_product<T, EPI, PL, QL, DZ, 16, 128, 1, 4>(a, 1, st);
+    if (tiles_of(a.ni, 128) * tiles_of(a.nj, 128) < 256) return launch_product<T, EPI, PL, QL, DZ, 64, 64, 2, 2>(a, 1, st);
+    if (a.ni <= 64) return launch_product<T, EPI, PL, QL, DZ, 64, 128, 2, 2>(a, 1, st);
+    return launch_product<T, EPI, PL, QL, DZ, 128, 128, 2, 2>(a, 1, st);
+}
+
+// Weight gradients: the sum over m is long and the output small, so it is split over workgroups that leave float32 partial
+// sums.  One rule for the launch and the workspace.
+struct WeightPlan {
+    int bi, bj, splits;
+    long long r_split;
+};
+inline WeightPlan weight_plan(int bk, long long m, long long n, long long k) {
+    WeightPlan p;
+    p.bi = k <= 16 ? 16 : n <= 16 || k <= 64 || n <= 64 ? 64 : 128;
+    p.bj = p.bi == 128 ? 128 : p.bi == 64 && n <= 16 ? 16 : 64;
+    const long long tiles = tiles_of(k, p.bi) * tiles_of(n, p.bj);
+    long long s = 1024 / tiles;
+    const long long most = tiles_of(m, 4 * bk);      // at least four steps each
+    if (s > most) s = most;
+    if (s < 1) s = 1;
+    p.r_split = tiles_of(tiles_of(m, s), bk) * bk;
+    p.splits = (int)tiles_of(m, p.r_split);
+    return p;
+}
+
+// dz becomes an array of its own where it would otherwise be recomputed for more than one tile of k, twice
+inline bool own_dz(int act, long long k) { return act != MPE_ACT_NONE && k > 128; }
+
+inline long long round_up(long long n) { return (n + 255) / 256 * 256; }
+
+template <typename T>
+struct LinearRun {
+    static long long backward_workspace(int act, long long m, long long n, long long k) {
+        if (m == 0) return 0;
+        const WeightPlan p = weight_plan(Piece<T>::BK, m, n, k);
+        return (own_dz(act, k) ? round_up(m * n * (long long)sizeof(T)) : 0) + round_up(p.splits * n * k * 4) + round_up(p.splits * n * 4);
+    }
+
+    static hipError_t forward(const LinearArgs& a, hipStream_t st) {
+        ProductArgs<T> g = {};
+        g.p = {(const T*)a.w, a.ldw, nullptr, 0, 0};
+        g.q = {(const T*)a.x, a.ldx, nullptr, 0, 0};
+        g.ni = a.n; g.nj = a.m; g.nr = a.k;
+        g.out = (T*)a.y; g.ldo = a.ldy;
+        g.bias = (const T*)a.bias; g.residual = (const T*)a.residual; g.ldr = a.ldr; g.pre = a.pre; g.act = a.act;
+        return launch_rows<T, EPI_FORWARD, R_INNER, R_INNER, false>(g, st);
+    }
+
+    template <bool DZ>
+    static hipError_t weights(const ProductArgs<T>& g, const WeightPlan& p, hipStream_t st) {
+        if (p.bi == 128) return launch_product<T, EPI_PARTIAL, O_INNER, O_INNER, DZ, 128, 128, 2, 2>(g, p.splits, st);
+        if (p.bi == 16) return launch_product<T, EPI_PARTIAL, O_INNER, O_INNER, DZ, 16, 64, 1, 4>(g, p.splits, st);
+        if (p.bj == 16) return launch_product<T, EPI_PARTIAL, O_INNER, O_INNER, DZ, 64, 16, 4, 1>(g, p.splits, st);
+        return launch_product<T, EPI_PARTIAL, O_INNER, O_INNER, DZ, 64, 64, 2, 2>(g, p.splits, st);
+    }
+
+    static hipError_t backward(const LinearArgs& a, hipStream_t st) {
+        hipError_t e = hipSuccess;
+        if (a.m == 0) {         // no rows: the gradients are empty sums
+            if (a.dw) e = launch_add_splits<T>(nullptr, 0, a.n * a.k, (T*)a.dw, st);
+            if (e == hipSuccess && a.db) e = launch_add_splits<T>(nullptr, 0, a.n, (T*)a.db, st);
+            return e;
+        }
+        char* ws = (char*)a.ws;
+        Operand<T> dz = {(const T*)a.dy, a.lddy, a.act != MPE_ACT_NONE ? a.pre : nullptr, a.n, a.act};
+        const bool own = own_dz(a.act, a.k);
+        if (own) {
+            const long long want = (a.m * a.n + 255) / 256;
+            hipLaunchKernelGGL((slope_pass<T>), dim3((unsigned)(want < 8192 ? want : 8192)), dim3(256), 0, st, a.m, a.n, (const T*)a.dy, a.lddy, (const void*)a.pre, a.act, (T*)ws);
+            e = hipGetLastError();
+            if (e != hipSuccess) return e;
+            dz = {(const T*)ws, a.n, nullptr, 0, MPE_ACT_NONE};
+            ws += round_up(a.m * a.n * (long long)sizeof(T));
+        }
+        if (a.dx) {
+            ProductArgs<T> g = {};
+            g.p = {(const T*)a.w, a.ldw, nullptr, 0, 0};
+            g.q = dz;
+            g.ni = a.k; g.nj = a.m; g.nr = a.n;
+            g.out = (T*)a.dx; g.ldo = a.lddx;
+            e = dz.pre ? launch_rows<T, EPI_STORE, O_INNER, R_INNER, true>(g, st) : launch_rows<T, EPI_STORE, O_INNER, R_INNER, false>(g, st);
+            if (e != hipSuccess) return e;
+        }
+        if (a.dw || a.db) {
+            const WeightPlan p = weight_plan(Piece<T>::BK, a.m, a.n, a.k);
+            ProductArgs<T> g = {};
+            g.p = {(const T*)a.x, a.ldx, nullptr, 0, 0};
+            g.q = dz;
+            g.ni = a.k; g.nj = a.n; g.nr = a.m; g.r_split = p.r_split;
+            g.partial = (float*)ws;
+            g.partial_sum = a.db ? (float*)(ws + round_up(p.splits * a.n * a.k * 4)) : nullptr;
+            e = dz.pre ? weights<true>(g, p, st) : weights<false>(g, p, st);
+            if (e == hipSuccess && a.dw) e = launch_add_splits<T>(g.partial, p.splits, a.n * a.k, (T*)a.dw, st);
+            if (e == hipSuccess && a.db) e = launch_add_splits<T>(g.partial_sum, p.splits, a.n, (T*)a.db, st);
+        }
+        return e;
+    }
+};
+
+}  // namespace mpe

@@ -20,6 +20,9 @@ ACTIVATIONS = {None: _lib.ACT_NONE, "none": _lib.ACT_NONE, "tanh": _lib.ACT_TANH
                "silu": _lib.ACT_SILU}
 
 
+_ROW_MAX = 1 << 22      # the longest row stride the kernels take
+
+
 def _stream(device):
     return torch.cuda.current_stream(device).cuda_stream
 
@@ -45,7 +48,7 @@ def _dtype(t, what):
 def _rows(t, cols):
     """``t`` as a matrix of ``cols`` columns whose rows are contiguous (any row stride >= cols), copied only if it has to be."""
     m = t if t.dim() == 2 else t.reshape(-1, cols)
-    if cols > 1 and m.stride(1) != 1 or (m.shape[0] > 1 and m.stride(0) < cols):
+    if cols > 1 and m.stride(1) != 1 or (m.shape[0] > 1 and not cols <= m.stride(0) <= _ROW_MAX):
         m = m.contiguous()
     return m
 
@@ -90,7 +93,7 @@ def _linear_forward(x, weight, bias, residual, act, code, keep_pre):
     m = x2.shape[0]
     dev = x.device
     y = torch.empty(x.shape[:-1] + (n,), dtype=x.dtype, device=dev)
-    pre = torch.empty(m, n, dtype=x.dtype, device=dev) if keep_pre else None
+    pre = torch.empty(m, n, dtype=x.dtype if act == _lib.ACT_RELU else torch.float32, device=dev) if keep_pre else None
     r2, ldr = (None, 0) if residual is None else _rows_or_one(residual, n)
     b1 = None if bias is None else bias.contiguous()
     ws_bytes = _workspace(code, act, m, n, k)[0]
@@ -103,9 +106,12 @@ def _linear_forward(x, weight, bias, residual, act, code, keep_pre):
 class _Linear(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias, residual, act, code):
-        # relu's slope is told by the output's sign where nothing was added to it
-        own_pre = act != _lib.ACT_NONE and not (act == _lib.ACT_RELU and residual is None)
+        # where nothing was added to it, the output itself tells relu's slope, and in float32 tanh's
+        from_y = residual is None and (act == _lib.ACT_RELU or (act == _lib.ACT_TANH and code == _lib.MPE_F32))
+        own_pre = act != _lib.ACT_NONE and not from_y
         y, pre = _linear_forward(x, weight, bias, residual, act, code, own_pre)
+        if from_y and act == _lib.ACT_TANH:
+            act = _lib.ACT_TANH_OUT
         ctx.act, ctx.code, ctx.has_bias = act, code, bias is not None
         ctx.save_for_backward(x, weight, pre if own_pre else y if act != _lib.ACT_NONE else None)
         return y
@@ -140,7 +146,7 @@ def linear(x, weight, bias=None, activation=None, residual=None):
     ``residual`` of the result's shape ``[..., n]`` (an expanded tensor will do); all of one type (float32, bfloat16,
     float16) on one GPU.  ``activation``: None / "none", "tanh", "relu", "gelu" (by erf) or "silu".  Sums are in float32 or
     better, with one rounding to the type at the end; float32 products are as exact as float32 multiplications.  For the
-    backward pass the pre-activations are kept in the tensors' type."""
+    backward pass the pre-activations are kept in float32 (nothing is kept for none, relu and float32 tanh without residual)."""
     try:
         act = ACTIVATIONS[activation]
     except (KeyError, TypeError):
