@@ -484,7 +484,7 @@ int mpe_linear_backward(int device, int dtype, int activation, int64_t m, int64_
  * The backward pass reads the same inputs, the forward's stats and one device float grad_loss = d(objective)/d(loss) and
  * writes dlogits T[rows][v] (row stride ldd) and, with values, dvalues float[rows] (NULL: not wanted).
  */
-#define MPE_PPO_WORKSPACE_BYTES 98304
+#define MPE_PPO_WORKSPACE_BYTES 61440
 int mpe_ppo_loss_forward(int device, int dtype, int64_t rows, int64_t v, const void* logits, int64_t ld, const void* actions, int action_bytes,
                          const float* old_logp, const float* adv, const uint8_t* mask, int64_t ldm, const float* weights, const float* values,
                          const float* old_values, const float* returns, double clip, double value_clip, double value_coef,

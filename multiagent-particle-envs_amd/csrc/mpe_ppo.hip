@@ -16,14 +16,15 @@ namespace mpe {
 namespace {
 
 constexpr int NSTAT = 6;        // policy, value, entropy, kl, clipped, weight
-constexpr int BLOCKS = MPE_PPO_WORKSPACE_BYTES / (8 * NSTAT);
-
-// Maximum that keeps NaN: a NaN logit has to reach the loss, whatever stands beside it.
-__device__ inline float larger(float a, float b) { return a > b || a != a ? a : b; }
+// Grids.  Forward: five workgroups a CU, which all find room at once (the rollout of 4.9 M rows: 67 us at 1024 workgroups,
+// 64 at 1280, 72 at 1792, when the last ones have to wait for a place).  Backward: enough that none is left over at the
+// end (86 us at 4096 workgroups of 256 rows, 84 at 8192, 88 at 16384; whole rows: 50 us from 2048 to 16384, 55 at 1280).
+constexpr int FORWARD_GRID = 1280, BACKWARD_GRID = 8192;
+static_assert(FORWARD_GRID * 8 * NSTAT <= MPE_PPO_WORKSPACE_BYTES, "a partial sum for every workgroup");
 
 struct Row {
     bool live;
-    float w, old_lp, adv;
+    float w, old_lp, adv, v, v0, ret;
     long long a;
 };
 
@@ -33,15 +34,19 @@ __device__ inline Row read_row(const PpoArgs& p, long long r) {
     x.a = p.action_bytes == 8 ? ((const long long*)p.actions)[r] : (long long)((const int32_t*)p.actions)[r];
     x.w = p.weights ? p.weights[r] : 1.0f;
     x.live = x.w != 0.0f && x.a >= 0 && x.a < p.v;
-    x.old_lp = x.live ? p.old_logp[r] : 0.0f;
-    x.adv = x.live ? p.adv[r] : 0.0f;
+    // read whether the row counts or not: no load waits for another
+    x.old_lp = p.old_logp[r];
+    x.adv = p.adv[r];
+    x.v = p.values ? p.values[r] : 0.0f;
+    x.v0 = p.values ? p.old_values[r] : 0.0f;
+    x.ret = p.values ? p.returns[r] : 0.0f;
     return x;
 }
 
 // The value half of a row in float64: which square is the larger decides the gradient's branch, and differences of
 // float32 numbers are exact there.
-__device__ inline void value_terms(const PpoArgs& p, long long r, double& loss, double& slope) {
-    const double v = p.values[r], v0 = p.old_values[r], ret = p.returns[r];
+__device__ inline void value_terms(const PpoArgs& p, const Row& x, double& loss, double& slope) {
+    const double v = x.v, v0 = x.v0, ret = x.ret;
     const double d = v - ret;
     loss = 0.5 * d * d;
     slope = d;
@@ -58,19 +63,26 @@ __device__ inline void value_terms(const PpoArgs& p, long long r, double& loss, 
 // exp by the hardware's 2^x: off by the rounding of d log2(e), |d| 2^-24, and one step
 __device__ inline float fast_exp(float d) { return __builtin_amdgcn_exp2f(d * 1.44269504088896341f); }
 
-// A row's softmax over the allowed words as running maximum, sum and sum of e^(l - m) (l - m).
+__device__ inline float fast_log(float x) { return __builtin_amdgcn_logf(x) * 0.69314718055994531f; }
+
+// e^d d without 0 * inf where d is -inf or the type's lowest value (a NaN is left to the sum of e^d)
+__device__ inline float weighted(float e, float d) { return e * fmaxf(d, -200.0f); }
+
+// A row's softmax over the allowed words as maximum, sum of e^(l - m) and sum of e^(l - m) (l - m).  Maxima pass over NaN;
+// the sums do not, so that a NaN logit reaches the loss whatever stands beside it.
 struct Soft {
     float m, s, t;
 };
 
 __device__ inline Soft merge(Soft a, Soft b) {
-    const float m = larger(a.m, b.m);
-    // a side that holds nothing (-inf) adds nothing, whatever m is
-    const float da = a.m - m, db = b.m - m, ea = a.m == -INFINITY ? 0.0f : fast_exp(da), eb = b.m == -INFINITY ? 0.0f : fast_exp(db);
+    const float m = fmaxf(a.m, b.m);
+    // a side that holds nothing (-inf) has the factor 0, which a NaN sum survives
+    const float da = a.m == -INFINITY ? -INFINITY : a.m - m, db = b.m == -INFINITY ? -INFINITY : b.m - m;
+    const float ea = fast_exp(da), eb = fast_exp(db);
     Soft c;
     c.m = m;
     c.s = a.s * ea + b.s * eb;
-    c.t = (ea == 0.0f ? 0.0f : ea * (a.t + a.s * da)) + (eb == 0.0f ? 0.0f : eb * (b.t + b.s * db));
+    c.t = ea * a.t + a.s * weighted(ea, da) + eb * b.t + b.s * weighted(eb, db);
     return c;
 }
 
@@ -81,15 +93,15 @@ struct Terms {
 };
 
 template <bool BACK>
-__device__ inline Terms row_terms(const PpoArgs& p, long long r, const Row& x, const Soft& q, float at, float share_all, double* sum) {
+__device__ inline Terms row_terms(const PpoArgs& p, const Row& x, const Soft& q, float at, float share_all, double* sum) {
     Terms y;
-    y.logs = logf(q.s);
+    y.logs = fast_log(q.s);
     y.ent = y.logs - q.t / q.s;
-    const float diff = at - q.m - y.logs - x.old_lp, ratio = expf(diff);
+    const float diff = at - q.m - y.logs - x.old_lp, ratio = fast_exp(diff);
     const float held = fminf(fmaxf(ratio, 1.0f - p.clip), 1.0f + p.clip);
     const float free_term = ratio * x.adv, held_term = held * x.adv;
     double vloss = 0.0, vslope = 0.0;
-    if (p.values) value_terms(p, r, vloss, vslope);
+    if (p.values) value_terms(p, x, vloss, vslope);
     if (BACK) {
         const float share = share_all * x.w;
         y.g = free_term <= held_term ? -free_term * share : 0.0f;
@@ -112,7 +124,7 @@ __device__ inline Terms row_terms(const PpoArgs& p, long long r, const Row& x, c
 // gradient of one allowed logit
 __device__ inline float logit_grad(const Terms& y, const Soft& q, float l, bool is_action) {
     const float lk = l - q.m - y.logs, pk = fast_exp(lk);
-    return (is_action ? y.g : 0.0f) - y.g * pk + (pk == 0.0f ? 0.0f : y.ce * pk * (lk + y.ent));
+    return (is_action ? y.g : 0.0f) + pk * (y.ce * y.ent - y.g) + y.ce * weighted(pk, lk);
 }
 
 __device__ inline float share_of(const PpoArgs& p) {
@@ -153,34 +165,62 @@ __device__ inline void leave_sums(const PpoArgs& p, const double* sum, double (*
 // gradients leave the same way.
 constexpr int FEW = 32;
 
-template <typename T, bool BACK>
+template <typename T, bool BACK, int VR>        // VR: at least v
 __global__ __launch_bounds__(256) void ppo_few(const PpoArgs p) {
     extern __shared__ float tile[];
     __shared__ double scratch[4][NSTAT];
     const int v = (int)p.v, stride = v | 1, tid = threadIdx.x;
-    const int dr = 256 / v, dc = 256 % v;
+    const int dr = 256 / v, dc = 256 % v, row0 = tid / v, col0 = tid % v;
     double sum[NSTAT] = {0, 0, 0, 0, 0, 0};
     const float share_all = BACK ? share_of(p) : 0.0f;
-    for (long long r0 = (long long)blockIdx.x * 256; r0 < p.rows; r0 += (long long)gridDim.x * 256) {
+
+    // the next tile's loads are in flight while this one is worked on
+    T raw[VR];
+    unsigned ok = 0;
+    Row next;
+    auto load = [&](long long r0) {
         const int rows = (int)min(256LL, p.rows - r0), n = rows * v;
-        __syncthreads();
-        {
-            int row = tid / v, col = tid % v;
-            const T* base = (const T*)p.logits + r0 * p.ld;
-            for (int i = tid; i < n; i += 256) {
-                const long long at = (long long)row * p.ld + col;
-                const bool ok = !p.mask || p.mask[(r0 + row) * p.ldm + col];
-                tile[row * stride + col] = ok ? (float)base[at] : -INFINITY;      // a forbidden word is one of weight zero
+        next = read_row(p, r0 + min(tid, rows - 1));
+        const T* base = (const T*)p.logits + r0 * p.ld;
+        const uint8_t* mask = p.mask ? p.mask + r0 * p.ldm : nullptr;
+        int row = row0, col = col0;
+        ok = 0;
+#pragma unroll
+        for (int u = 0; u < VR; ++u)
+            if (u < v) {
+                if (tid + u * 256 < n) {
+                    raw[u] = base[(long long)row * p.ld + col];
+                    ok |= (!mask || mask[(long long)row * p.ldm + col] ? 1u : 0u) << u;
+                }
                 row += dr;
                 col += dc;
                 if (col >= v) { col -= v; ++row; }
             }
+    };
+
+    const long long step = (long long)gridDim.x * 256;
+    long long r0 = (long long)blockIdx.x * 256;
+    if (r0 < p.rows) load(r0);
+    for (; r0 < p.rows; r0 += step) {
+        const int rows = (int)min(256LL, p.rows - r0), n = rows * v;
+        Row x = next;
+        __syncthreads();
+        {
+            int row = row0, col = col0;
+#pragma unroll
+            for (int u = 0; u < VR; ++u)
+                if (u < v) {
+                    if (tid + u * 256 < n) tile[row * stride + col] = ok >> u & 1 ? (float)raw[u] : -INFINITY;     // a forbidden word is one of weight zero
+                    row += dr;
+                    col += dc;
+                    if (col >= v) { col -= v; ++row; }
+                }
         }
         __syncthreads();
+        if (r0 + step < p.rows) load(r0 + step);
         float* l = tile + tid * stride;
         if (tid < rows) {
             const long long r = r0 + tid;
-            Row x = read_row(p, r);
             float at = 0.0f;
             if (x.live) {
                 at = l[x.a];
@@ -188,13 +228,13 @@ __global__ __launch_bounds__(256) void ppo_few(const PpoArgs p) {
             }
             if (x.live) {
                 Soft q = {-INFINITY, 0.0f, 0.0f};
-                for (int k = 0; k < v; ++k) q.m = larger(q.m, l[k]);
+                for (int k = 0; k < v; ++k) q.m = fmaxf(q.m, l[k]);
                 for (int k = 0; k < v; ++k) {
                     const float d = l[k] - q.m, e = fast_exp(d);
                     q.s += e;
-                    q.t += e == 0.0f ? 0.0f : e * d;      // -inf and the type's lowest value: nothing, not 0 * inf
+                    q.t += weighted(e, d);
                 }
-                const Terms y = row_terms<BACK>(p, r, x, q, at, share_all, sum);
+                const Terms y = row_terms<BACK>(p, x, q, at, share_all, sum);
                 if (BACK) {
                     for (int k = 0; k < v; ++k) l[k] = logit_grad(y, q, l[k], k == x.a);
                     if (p.dvalues) p.dvalues[r] = (float)(y.vslope * y.share);
@@ -206,7 +246,7 @@ __global__ __launch_bounds__(256) void ppo_few(const PpoArgs p) {
         }
         if (BACK) {
             __syncthreads();
-            int row = tid / v, col = tid % v;
+            int row = row0, col = col0;
             T* base = (T*)p.dlogits + r0 * p.ldd;
             for (int i = tid; i < n; i += 256) {
                 base[(long long)row * p.ldd + col] = (T)tile[row * stride + col];
@@ -230,48 +270,36 @@ __global__ __launch_bounds__(256) void ppo_many(const PpoArgs p) {
     double sum[NSTAT] = {0, 0, 0, 0, 0, 0};
     const float share_all = BACK ? share_of(p) : 0.0f;
 
-    // vector i of the row: words [k, k + E) as float32, a forbidden word and one behind the end as -inf
-    auto fetch = [&](long long r, long long k, float* f) {
+    // words [k, k + E) of the row, a forbidden one and one behind the end as -inf
+    auto fetch = [&](long long r, long long k, T* f) {
         const T* l = (const T*)p.logits + r * p.ld + k;
         if (k + E <= p.v) {
-            T raw[E];
-            __builtin_memcpy(raw, l, sizeof(raw));
-#pragma unroll
-            for (int e = 0; e < E; ++e) f[e] = (float)raw[e];
+            __builtin_memcpy(f, l, E * sizeof(T));
             if (p.mask) {
                 uint8_t ok[E];
                 __builtin_memcpy(ok, p.mask + r * p.ldm + k, E);
 #pragma unroll
-                for (int e = 0; e < E; ++e) f[e] = ok[e] ? f[e] : -INFINITY;
+                for (int e = 0; e < E; ++e) f[e] = ok[e] ? f[e] : (T)-INFINITY;
             }
         } else {
 #pragma unroll
-            for (int e = 0; e < E; ++e) f[e] = k + e < p.v && (!p.mask || p.mask[r * p.ldm + k + e]) ? (float)l[e] : -INFINITY;
+            for (int e = 0; e < E; ++e) f[e] = k + e < p.v && (!p.mask || p.mask[r * p.ldm + k + e]) ? l[e] : (T)-INFINITY;
         }
     };
-    auto take = [&](Soft& q, const float* f) {      // adds E words
-        float m = q.m;
-#pragma unroll
-        for (int e = 0; e < E; ++e) m = larger(m, f[e]);
-        if (m == -INFINITY) return;
-        if (m != q.m && q.m != -INFINITY) {
-            const float d = q.m - m, c = fast_exp(d);
-            q.t = c == 0.0f ? 0.0f : c * (q.t + q.s * d);
-            q.s *= c;
-        }
-        q.m = m;
+    auto take = [&](Soft& q, const T* f, float m) {      // adds E words relative to m; where m is -inf there are only -inf and NaN
+        const float m0 = m == -INFINITY ? 0.0f : m;
 #pragma unroll
         for (int e = 0; e < E; ++e) {
-            const float d = f[e] - m, x = fast_exp(d);
+            const float d = (float)f[e] - m0, x = fast_exp(d);
             q.s += x;
-            q.t += x == 0.0f ? 0.0f : x * d;
+            q.t += weighted(x, d);
         }
     };
-    auto give = [&](long long r, long long k, const float* f, const Row& x, const Terms& y, const Soft& q) {
+    auto give = [&](long long r, long long k, const T* f, const Row& x, const Terms& y, const Soft& q) {
         T* d = (T*)p.dlogits + r * p.ldd + k;
         T out[E];
 #pragma unroll
-        for (int e = 0; e < E; ++e) out[e] = (T)(x.live ? logit_grad(y, q, f[e], k + e == x.a) : 0.0f);
+        for (int e = 0; e < E; ++e) out[e] = (T)(x.live ? logit_grad(y, q, (float)f[e], k + e == x.a) : 0.0f);
         if (k + E <= p.v) __builtin_memcpy(d, out, sizeof(out));
         else {
 #pragma unroll
@@ -292,7 +320,7 @@ __global__ __launch_bounds__(256) void ppo_many(const PpoArgs p) {
             at = !p.mask || p.mask[r * p.ldm + x.a] ? (float)((const T*)p.logits)[r * p.ld + x.a] : -INFINITY;
             x.live = at != -INFINITY;
         }
-        float f[NV ? NV : 1][E];
+        T f[NV ? NV : 1][E];
         Soft q = {-INFINITY, 0.0f, 0.0f};
         if (x.live) {
             if (NV) {
@@ -302,21 +330,23 @@ __global__ __launch_bounds__(256) void ppo_many(const PpoArgs p) {
                     if (k < p.v) fetch(r, k, f[i]);
                     else
 #pragma unroll
-                        for (int e = 0; e < E; ++e) f[i][e] = -INFINITY;
+                        for (int e = 0; e < E; ++e) f[i][e] = (T)-INFINITY;
                 }
                 // one maximum for all that a thread holds
 #pragma unroll
                 for (int i = 0; i < NV; ++i)
 #pragma unroll
-                    for (int e = 0; e < E; ++e) q.m = larger(q.m, f[i][e]);
-                if (q.m != -INFINITY) {
+                    for (int e = 0; e < E; ++e) q.m = fmaxf(q.m, (float)f[i][e]);
 #pragma unroll
-                    for (int i = 0; i < NV; ++i) take(q, f[i]);
-                }
+                for (int i = 0; i < NV; ++i) take(q, f[i], q.m);
             } else {
                 for (long long k = (long long)lane * E; k < p.v; k += LANES * E) {
                     fetch(r, k, f[0]);
-                    take(q, f[0]);
+                    Soft w = {-INFINITY, 0.0f, 0.0f};
+#pragma unroll
+                    for (int e = 0; e < E; ++e) w.m = fmaxf(w.m, (float)f[0][e]);
+                    take(w, f[0], w.m);
+                    q = merge(q, w);
                 }
             }
         }
@@ -335,7 +365,7 @@ __global__ __launch_bounds__(256) void ppo_many(const PpoArgs p) {
         Terms y = {};
         if (x.live) {
             double mine[NSTAT] = {0, 0, 0, 0, 0, 0};
-            y = row_terms<BACK>(p, r, x, q, at, share_all, mine);
+            y = row_terms<BACK>(p, x, q, at, share_all, mine);
             if (!BACK && lane == 0)
                 for (int i = 0; i < NSTAT; ++i) sum[i] += mine[i];
         }
@@ -378,8 +408,9 @@ __global__ __launch_bounds__(1024) void ppo_finish(const double* __restrict__ pa
 }
 
 template <typename T, bool BACK>
-hipError_t launch_rows(const PpoArgs& a, int most, int* grid_out, hipStream_t st) {
+hipError_t launch_rows(const PpoArgs& a, int* grid_out, hipStream_t st) {
     const auto grid_for = [&](long long per_block) {
+        const int most = BACK ? BACKWARD_GRID : FORWARD_GRID;
         long long g = (a.rows + per_block - 1) / per_block;
         g = g < 1 ? 1 : g > most ? most : g;
         if (grid_out) *grid_out = (int)g;
@@ -388,7 +419,8 @@ hipError_t launch_rows(const PpoArgs& a, int most, int* grid_out, hipStream_t st
     constexpr int E = 16 / (int)sizeof(T);
     if (a.v <= FEW) {
         const size_t bytes = 256 * (size_t)(a.v | 1) * 4;
-        hipLaunchKernelGGL((ppo_few<T, BACK>), grid_for(256), dim3(256), bytes, st, a);
+        if (a.v <= 8) hipLaunchKernelGGL((ppo_few<T, BACK, 8>), grid_for(256), dim3(256), bytes, st, a);
+        else hipLaunchKernelGGL((ppo_few<T, BACK, FEW>), grid_for(256), dim3(256), bytes, st, a);
     } else if (a.v <= 64 * E) {
         hipLaunchKernelGGL((ppo_many<T, BACK, 1, 1>), grid_for(4), dim3(256), 0, st, a);
     } else if (a.v <= 4 * 64 * E) {
@@ -405,7 +437,7 @@ hipError_t launch_rows(const PpoArgs& a, int most, int* grid_out, hipStream_t st
 
 hipError_t launch_ppo_forward(const PpoArgs& a, hipStream_t st) {
     int grid = 0;
-    hipError_t e = with_dtype(a.dtype, [&](auto z) { return launch_rows<decltype(z), false>(a, BLOCKS, &grid, st); });
+    hipError_t e = with_dtype(a.dtype, [&](auto z) { return launch_rows<decltype(z), false>(a, &grid, st); });
     if (e != hipSuccess || grid == 1) return e;
     hipLaunchKernelGGL(ppo_finish, dim3(1), dim3(1024), 0, st, a.ws, grid, a.value_coef, a.entropy_coef, a.loss, a.stats);
     return hipGetLastError();
@@ -413,7 +445,7 @@ hipError_t launch_ppo_forward(const PpoArgs& a, hipStream_t st) {
 
 hipError_t launch_ppo_backward(const PpoArgs& a, hipStream_t st) {
     if (a.rows == 0) return hipSuccess;
-    return with_dtype(a.dtype, [&](auto z) { return launch_rows<decltype(z), true>(a, 16384, nullptr, st); });
+    return with_dtype(a.dtype, [&](auto z) { return launch_rows<decltype(z), true>(a, nullptr, st); });
 }
 
 }  // namespace mpe

@@ -13,7 +13,7 @@ LIB_PATH = os.environ.get("MPE_HIP_LIB") or os.path.join(_HERE, "libmpe_hip.so")
 
 MPE_F32, MPE_F64, MPE_BF16, MPE_F16 = 0, 1, 2, 3
 ACT_NONE, ACT_TANH, ACT_RELU, ACT_GELU, ACT_SILU, ACT_TANH_OUT = 0, 1, 2, 3, 4, 5
-CLIP_WORKSPACE_BYTES, PPO_WORKSPACE_BYTES = 16384, 98304
+CLIP_WORKSPACE_BYTES, PPO_WORKSPACE_BYTES = 16384, 61440
 SCN_NONE, SCN_SPREAD, SCN_TAG, SCN_WORLD_COMM, SCN_SIMPLE, SCN_ADVERSARY, SCN_PUSH = 0, 1, 2, 3, 4, 5, 6
 SCN_SPEAKER_LISTENER, SCN_REFERENCE, SCN_CRYPTO, SCN_PREDATOR_PREY, SCN_CONSENSUS = 7, 8, 9, 10, 11
 SCN_COLLECTOR = 12

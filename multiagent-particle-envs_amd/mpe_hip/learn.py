@@ -9,6 +9,7 @@ device and return without synchronising.  All may be captured into a graph; a ba
 autograd's own rule that no eager graph of the same leaves is alive.  Second derivatives are not available.
 """
 import ctypes as C
+from array import array
 
 import torch
 from torch.autograd.function import once_differentiable
@@ -23,8 +24,13 @@ ACTIVATIONS = {None: _lib.ACT_NONE, "none": _lib.ACT_NONE, "tanh": _lib.ACT_TANH
 _ROW_MAX = 1 << 22      # the longest row stride the kernels take
 
 
-def _stream(device):
-    return torch.cuda.current_stream(device).cuda_stream
+def _raw_stream():
+    """index of a device -> handle of its current stream; torch's own getter costs a microsecond more by making an object."""
+    fn = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+    return fn if fn is not None else lambda index: torch.cuda.current_stream(index).cuda_stream
+
+
+_stream = _raw_stream()
 
 
 def _ptr(t):
@@ -37,33 +43,31 @@ def _check(code):
 
 
 def _dtype(t, what):
-    if t.device.type != "cuda":
+    if not t.is_cuda:
         raise ValueError("%s needs GPU tensors; there is no CPU path" % what)
-    try:
-        return _DTYPES[t.dtype]
-    except KeyError:
-        raise ValueError("%s takes float32, bfloat16 or float16, not %s" % (what, t.dtype)) from None
+    code = _DTYPES.get(t.dtype)
+    if code is None:
+        raise ValueError("%s takes float32, bfloat16 or float16, not %s" % (what, t.dtype))
+    return code
 
 
 def _rows(t, cols):
-    """``t`` as a matrix of ``cols`` columns whose rows are contiguous (any row stride >= cols), copied only if it has to be."""
+    """``(matrix, row stride)``: ``t`` as rows of ``cols`` contiguous elements (any row stride >= cols), copied only if it has to be."""
+    if t.is_contiguous():
+        return t, cols
     m = t if t.dim() == 2 else t.reshape(-1, cols)
-    if cols > 1 and m.stride(1) != 1 or (m.shape[0] > 1 and not cols <= m.stride(0) <= _ROW_MAX):
-        m = m.contiguous()
-    return m
-
-
-def _ld(m):
-    """Row stride of what _rows returned; a single row's stride says nothing."""
-    return m.stride(0) if m.shape[0] > 1 else m.shape[1]
+    rows, (ld, inner) = m.shape[0], m.stride()
+    if (cols > 1 and inner != 1) or (rows > 1 and not cols <= ld <= _ROW_MAX):
+        return m.contiguous(), cols
+    return m, ld if rows > 1 else cols      # a single row's stride says nothing
 
 
 def _rows_or_one(t, cols):
     """As _rows, but one row repeated by ``expand`` stays one row (stride 0)."""
-    if t.dim() >= 2 and t.numel() > 0 and (cols == 1 or t.stride(-1) == 1) and all(s == 0 or n == 1 for s, n in zip(t.stride()[:-1], t.shape[:-1])):
-        return t.as_strided((t.numel() // cols, cols), (0, 1)), 0
-    m = _rows(t, cols)
-    return m, _ld(m)
+    if not t.is_contiguous() and t.dim() >= 2 and t.numel() > 0 and (cols == 1 or t.stride(-1) == 1) \
+            and all(s == 0 or n == 1 for s, n in zip(t.stride()[:-1], t.shape[:-1])):
+        return t, 0
+    return _rows(t, cols)
 
 
 # ---- linear -------------------------------------------------------------------------------------------------------------
@@ -89,17 +93,19 @@ def _space(nbytes, device):
 
 def _linear_forward(x, weight, bias, residual, act, code, keep_pre):
     n, k = weight.shape
-    x2, w2 = _rows(x, k), _rows(weight, k)
-    m = x2.shape[0]
+    x2, ldx = _rows(x, k)
+    w2, ldw = _rows(weight, k)
+    m = x.numel() // k
     dev = x.device
     y = torch.empty(x.shape[:-1] + (n,), dtype=x.dtype, device=dev)
     pre = torch.empty(m, n, dtype=x.dtype if act == _lib.ACT_RELU else torch.float32, device=dev) if keep_pre else None
     r2, ldr = (None, 0) if residual is None else _rows_or_one(residual, n)
-    b1 = None if bias is None else bias.contiguous()
+    if bias is not None and not bias.is_contiguous():
+        bias = bias.contiguous()
     ws_bytes = _workspace(code, act, m, n, k)[0]
     ws = _space(ws_bytes, dev)
-    _check(_lib.load().mpe_linear_forward(dev.index, code, act, m, n, k, x2.data_ptr(), _ld(x2), w2.data_ptr(), _ld(w2), _ptr(b1), _ptr(r2), ldr,
-                                          y.data_ptr(), n, _ptr(pre), _ptr(ws), ws_bytes, _stream(dev)))
+    _check(_lib.load().mpe_linear_forward(dev.index, code, act, m, n, k, x2.data_ptr(), ldx, w2.data_ptr(), ldw, _ptr(bias), _ptr(r2), ldr,
+                                          y.data_ptr(), n, _ptr(pre), _ptr(ws), ws_bytes, _stream(dev.index)))
     return y, pre
 
 
@@ -125,8 +131,9 @@ class _Linear(torch.autograd.Function):
         dx = dw = db = None
         if need_x or need_w or need_b:
             n, k = weight.shape
-            x2, w2 = _rows(x, k), _rows(weight, k)
-            m = x2.shape[0]
+            x2, ldx = _rows(x, k)
+            w2, ldw = _rows(weight, k)
+            m = x.numel() // k
             dev = x.device
             dy2, lddy = _rows_or_one(dy, n)
             dx = torch.empty(x.shape, dtype=x.dtype, device=dev) if need_x else None
@@ -134,8 +141,8 @@ class _Linear(torch.autograd.Function):
             db = torch.empty(n, dtype=x.dtype, device=dev) if need_b else None
             ws_bytes = _workspace(ctx.code, ctx.act, m, n, k)[1]
             ws = _space(ws_bytes, dev)
-            _check(_lib.load().mpe_linear_backward(dev.index, ctx.code, ctx.act, m, n, k, _ptr(dy2), lddy, x2.data_ptr(), _ld(x2), w2.data_ptr(),
-                                                   _ld(w2), _ptr(pre), _ptr(dx), k, _ptr(dw), _ptr(db), _ptr(ws), ws_bytes, _stream(dev)))
+            _check(_lib.load().mpe_linear_backward(dev.index, ctx.code, ctx.act, m, n, k, dy2.data_ptr(), lddy, x2.data_ptr(), ldx, w2.data_ptr(),
+                                                   ldw, _ptr(pre), _ptr(dx), k, _ptr(dw), _ptr(db), _ptr(ws), ws_bytes, _stream(dev.index)))
         return dx, dw, db, dy if need_r else None, None, None
 
 
@@ -152,18 +159,21 @@ def linear(x, weight, bias=None, activation=None, residual=None):
     except (KeyError, TypeError):
         raise ValueError("linear: activation must be one of none, tanh, relu, gelu, silu; got %r" % (activation,)) from None
     code = _dtype(x, "linear")
-    if x.dim() < 1 or weight.dim() != 2 or x.shape[-1] != weight.shape[1] or weight.shape[0] < 1 or weight.shape[1] < 1:
-        raise ValueError("linear: x [..., k] and weight [n, k], n and k at least 1; got %s and %s" % (tuple(x.shape), tuple(weight.shape)))
-    n = weight.shape[0]
+    shape, wshape = x.shape, weight.shape
+    if len(shape) < 1 or len(wshape) != 2 or shape[-1] != wshape[1] or wshape[0] < 1 or wshape[1] < 1:
+        raise ValueError("linear: x [..., k] and weight [n, k], n and k at least 1; got %s and %s" % (tuple(shape), tuple(wshape)))
+    n, dt, dev = wshape[0], x.dtype, x.device
     if bias is not None and tuple(bias.shape) != (n,):
         raise ValueError("linear: bias must have shape (%d,), got %s" % (n, tuple(bias.shape)))
-    if residual is not None and residual.shape != x.shape[:-1] + (n,):
-        raise ValueError("linear: residual must have the result's shape %s, got %s" % (tuple(x.shape[:-1]) + (n,), tuple(residual.shape)))
+    if residual is not None and residual.shape != shape[:-1] + (n,):
+        raise ValueError("linear: residual must have the result's shape %s, got %s" % (tuple(shape[:-1]) + (n,), tuple(residual.shape)))
+    needs = x.requires_grad or weight.requires_grad
     for t in (weight, bias, residual):
-        if t is not None and (t.dtype != x.dtype or t.device != x.device):
-            raise ValueError("linear: all tensors must share x's type and device (%s, %s)" % (x.dtype, x.device))
-    if torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad or (bias is not None and bias.requires_grad)
-                                    or (residual is not None and residual.requires_grad)):
+        if t is not None:
+            if t.dtype != dt or t.device != dev:
+                raise ValueError("linear: all tensors must share x's type and device (%s, %s)" % (dt, dev))
+            needs = needs or t.requires_grad
+    if needs and torch.is_grad_enabled():
         return _Linear.apply(x, weight, bias, residual, act, code)
     return _linear_forward(x, weight, bias, residual, act, code, False)[0]
 
@@ -172,20 +182,20 @@ def linear(x, weight, bias=None, activation=None, residual=None):
 
 class _PpoLoss(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, logits, values, shared, coefs, code):
-        actions, old_logp, adv, old_values, returns, mask, weights = shared
+    def forward(ctx, logits, values, actions, old_logp, adv, old_values, returns, mask, weights, coefs, code):
         v = logits.shape[-1]
-        l2 = _rows(logits, v)
+        l2, ld = _rows(logits, v)
         dev = logits.device
         loss, stats = torch.empty((), dtype=torch.float32, device=dev), torch.empty(6, dtype=torch.float32, device=dev)
-        ws = _space(_lib.PPO_WORKSPACE_BYTES, dev)
-        val = None if values is None else values.contiguous()
-        args = (dev.index, code, l2.shape[0], v, l2.data_ptr(), _ld(l2), actions.data_ptr(), actions.element_size(), old_logp.data_ptr(), adv.data_ptr(),
-                _ptr(mask), 0 if mask is None else _ld(mask), _ptr(weights), _ptr(val), _ptr(old_values), _ptr(returns)) + coefs
-        _check(_lib.load().mpe_ppo_loss_forward(*args, loss.data_ptr(), stats.data_ptr(), ws.data_ptr(), _lib.PPO_WORKSPACE_BYTES, _stream(dev)))
-        ctx.args, ctx.values_shape = args, None if values is None else values.shape
-        ctx.save_for_backward(logits, values, stats, *shared)
-        ctx.kept = (l2, val)        # what args point to, where it is a copy
+        ws = torch.empty(_lib.PPO_WORKSPACE_BYTES, dtype=torch.uint8, device=dev)
+        val = values if values is None or values.is_contiguous() else values.contiguous()
+        m2, ldm = (None, 0) if mask is None else _rows(mask, v)
+        args = (dev.index, code, logits.numel() // v, v, l2.data_ptr(), ld, actions.data_ptr(), actions.element_size(), old_logp.data_ptr(), adv.data_ptr(),
+                _ptr(m2), ldm, _ptr(weights), _ptr(val), _ptr(old_values), _ptr(returns)) + coefs
+        _check(_lib.load().mpe_ppo_loss_forward(*args, loss.data_ptr(), stats.data_ptr(), ws.data_ptr(), _lib.PPO_WORKSPACE_BYTES, _stream(dev.index)))
+        ctx.args = args
+        ctx.save_for_backward(logits, values, stats, actions, old_logp, adv, old_values, returns, mask, weights)
+        ctx.kept = (l2, val, m2)        # what args point to, where it is a copy
         ctx.mark_non_differentiable(stats)
         return loss, stats
 
@@ -194,14 +204,28 @@ class _PpoLoss(torch.autograd.Function):
     def backward(ctx, grad, _):
         logits, values, stats = ctx.saved_tensors[:3]       # raises where an input was written since
         need_l, need_v = ctx.needs_input_grad[0], ctx.needs_input_grad[1] and values is not None
-        if not (need_l or need_v):
-            return None, None, None, None, None
-        dev = logits.device
-        dlogits = torch.empty(logits.shape, dtype=logits.dtype, device=dev)
-        dvalues = torch.empty(ctx.values_shape, dtype=torch.float32, device=dev) if need_v else None
-        grad = grad.to(torch.float32)
-        _check(_lib.load().mpe_ppo_loss_backward(*ctx.args, stats.data_ptr(), grad.data_ptr(), dlogits.data_ptr(), logits.shape[-1], _ptr(dvalues), _stream(dev)))
-        return dlogits if need_l else None, dvalues, None, None, None
+        dlogits = dvalues = None
+        if need_l or need_v:
+            dev = logits.device
+            dlogits = torch.empty(logits.shape, dtype=logits.dtype, device=dev)
+            if need_v:
+                dvalues = torch.empty(values.shape, dtype=torch.float32, device=dev)
+            if grad.dtype != torch.float32:
+                grad = grad.to(torch.float32)
+            _check(_lib.load().mpe_ppo_loss_backward(*ctx.args, stats.data_ptr(), grad.data_ptr(), dlogits.data_ptr(), logits.shape[-1], _ptr(dvalues),
+                                                     _stream(dev.index)))
+        return (dlogits if need_l else None, dvalues) + (None,) * 9
+
+
+def _side(name, t, dtype, shape, dev):
+    """A tensor that goes with the logits, checked and contiguous."""
+    if t is None:
+        return None
+    if t.dtype != dtype:
+        raise ValueError("ppo_loss: %s must be %s, not %s" % (name, str(dtype).replace("torch.", ""), t.dtype))
+    if t.shape != shape or t.device != dev:
+        raise ValueError("ppo_loss: %s must have shape %s on %s, got %s on %s" % (name, tuple(shape), dev, tuple(t.shape), t.device))
+    return t if t.is_contiguous() else t.contiguous()
 
 
 def ppo_loss(logits, actions, old_logp, advantages, values=None, old_values=None, returns=None, action_mask=None, weights=None, clip=0.2,
@@ -220,34 +244,30 @@ def ppo_loss(logits, actions, old_logp, advantages, values=None, old_values=None
     has the logit -infinity (so also where no move is left).  Returns ``(loss, stats)``: a float32 scalar and the float32 means
     ``[-s, u, H, (logp - old_logp)^2 / 2, share of clipped decisions]``."""
     code = _dtype(logits, "ppo_loss")
-    if logits.dim() < 1 or logits.shape[-1] < 1:
-        raise ValueError("ppo_loss: logits must be [..., v] with v at least 1, got %s" % (tuple(logits.shape),))
-    lead, dev = logits.shape[:-1], logits.device
+    shape, dev = logits.shape, logits.device
+    if len(shape) < 1 or shape[-1] < 1:
+        raise ValueError("ppo_loss: logits must be [..., v] with v at least 1, got %s" % (tuple(shape),))
+    lead, f32 = shape[:-1], torch.float32
     if (values is None) != (old_values is None) or (values is None) != (returns is None):
         raise ValueError("ppo_loss: values, old_values and returns go together")
     if actions.dtype not in (torch.int32, torch.int64):
         raise ValueError("ppo_loss: actions must be int32 or int64, not %s" % actions.dtype)
-    for name, t, want in (("old_logp", old_logp, torch.float32), ("advantages", advantages, torch.float32), ("values", values, torch.float32),
-                          ("old_values", old_values, torch.float32), ("returns", returns, torch.float32)):
-        if t is not None and t.dtype != want:
-            raise ValueError("ppo_loss: %s must be float32, not %s" % (name, t.dtype))
     if weights is not None and weights.dtype == torch.bool:
         weights = weights.float()
-    if weights is not None and weights.dtype != torch.float32:
-        raise ValueError("ppo_loss: weights must be float32 or bool, not %s" % weights.dtype)
-    if action_mask is not None and action_mask.dtype not in (torch.bool, torch.uint8):
-        raise ValueError("ppo_loss: action_mask must be bool or uint8, not %s" % action_mask.dtype)
-    for name, t, shape in (("actions", actions, lead), ("old_logp", old_logp, lead), ("advantages", advantages, lead), ("values", values, lead),
-                           ("old_values", old_values, lead), ("returns", returns, lead), ("weights", weights, lead), ("action_mask", action_mask, logits.shape)):
-        if t is not None and (t.shape != shape or t.device != dev):
-            raise ValueError("ppo_loss: %s must have shape %s on %s, got %s on %s" % (name, tuple(shape), dev, tuple(t.shape), t.device))
+    if action_mask is not None:
+        if action_mask.dtype not in (torch.bool, torch.uint8):
+            raise ValueError("ppo_loss: action_mask must be bool or uint8, not %s" % action_mask.dtype)
+        if action_mask.shape != shape or action_mask.device != dev:
+            raise ValueError("ppo_loss: action_mask must have shape %s on %s, got %s on %s" % (tuple(shape), dev, tuple(action_mask.shape), action_mask.device))
+    if values is not None and (values.dtype != f32 or values.shape != lead or values.device != dev):
+        raise ValueError("ppo_loss: values must be float32 of shape %s on %s, got %s %s on %s" % (tuple(lead), dev, values.dtype, tuple(values.shape), values.device))
     clip, value_clip = float(clip), -1.0 if value_clip is None else float(value_clip)
     if not clip >= 0 or not (value_clip >= 0 or value_clip == -1.0):
         raise ValueError("ppo_loss: clip and value_clip must not be negative")
-    flat = lambda t: None if t is None else t.detach().contiguous()
-    shared = (flat(actions), flat(old_logp), flat(advantages), flat(old_values), flat(returns),
-              None if action_mask is None else _rows(action_mask, logits.shape[-1]), flat(weights))
-    loss, stats = _PpoLoss.apply(logits, values, shared, (clip, value_clip, float(value_coef), float(entropy_coef)), code)
+    loss, stats = _PpoLoss.apply(logits, values, _side("actions", actions, actions.dtype, lead, dev), _side("old_logp", old_logp, f32, lead, dev),
+                                 _side("advantages", advantages, f32, lead, dev), _side("old_values", old_values, f32, lead, dev),
+                                 _side("returns", returns, f32, lead, dev), action_mask, _side("weights", weights, f32, lead, dev),
+                                 (clip, value_clip, float(value_coef), float(entropy_coef)), code)
     return loss, stats[:5]
 
 
@@ -266,32 +286,36 @@ def _dense(t):
 
 
 def _clip(tensors, max_norm, outs):
-    n = len(tensors)
     dev = tensors[0].device
-    src, cnt, typ = (C.c_void_p * n)(), (C.c_int64 * n)(), (C.c_int32 * n)()
+    types = [t.dtype for t in tensors]
     for i, t in enumerate(tensors):
-        if t.device != dev or t.dtype not in _DTYPES or dev.type != "cuda":
+        if t.device != dev or not t.is_cuda or types[i] not in _DTYPES:
             raise ValueError("clip_grad_norm: tensor %d must be float32, bfloat16 or float16 on the GPU of tensor 0 (%s), got %s on %s"
-                             % (i, dev, t.dtype, t.device))
-        if t.layout != torch.strided or not _dense(t):
+                             % (i, dev, types[i], t.device))
+        if t.layout != torch.strided or not (t.is_contiguous() or _dense(t)):
             raise ValueError("clip_grad_norm: tensor %d is sparse or has gaps or repeated elements" % i)
-        src[i], cnt[i], typ[i] = t.data_ptr(), t.numel(), _DTYPES[t.dtype]
+    src = array("Q", [t.data_ptr() for t in tensors])
+    counts = array("q", [t.numel() for t in tensors])
+    codes = array("i", [_DTYPES[d] for d in types])
     dst = None
-    if outs is not None:
-        if outs is tensors:
-            dst = src
-        else:
-            dst = (C.c_void_p * n)()
-            for i, (t, o) in enumerate(zip(tensors, outs)):
-                if o.dtype != t.dtype or o.device != dev or o.shape != t.shape or (o.stride() != t.stride() and not (t.is_contiguous() and o.is_contiguous())):
-                    raise ValueError("clip_grad_norm: out %d must have the shape, strides, type and device of its tensor" % i)
-                dst[i] = o.data_ptr()
-        spans = sorted((p, p + c * t.element_size()) for p, c, t in zip(dst, cnt, tensors) if c)
-        if any(a[1] > b[0] for a, b in zip(spans, spans[1:])):
-            raise ValueError("clip_grad_norm: a tensor is given twice, or two share memory")
+    if outs is tensors:
+        dst = src
+    elif outs is not None:
+        for i, (t, o) in enumerate(zip(tensors, outs)):
+            if o.dtype != types[i] or o.device != dev or o.shape != t.shape or not (o.is_contiguous() and t.is_contiguous() or o.stride() == t.stride()):
+                raise ValueError("clip_grad_norm: out %d must have the shape, strides, type and device of its tensor" % i)
+        dst = array("Q", [o.data_ptr() for o in outs])
+    if dst is not None:
+        end = 0
+        for p, bytes_ in sorted([(p, c * (4 if d == 0 else 2)) for p, c, d in zip(dst, counts, codes) if c]):
+            if p < end:
+                raise ValueError("clip_grad_norm: a tensor is given twice, or two share memory")
+            end = p + bytes_
     norm = torch.empty((), dtype=torch.float32, device=dev)
-    ws = _space(_lib.CLIP_WORKSPACE_BYTES, dev)
-    _check(_lib.load().mpe_clip_grad_norm(dev.index, n, src, dst, cnt, typ, max_norm, norm.data_ptr(), ws.data_ptr(), _lib.CLIP_WORKSPACE_BYTES, _stream(dev)))
+    ws = torch.empty(_lib.CLIP_WORKSPACE_BYTES, dtype=torch.uint8, device=dev)
+    _check(_lib.load().mpe_clip_grad_norm(dev.index, len(tensors), src.buffer_info()[0], dst.buffer_info()[0] if dst is not None else None,
+                                          counts.buffer_info()[0], codes.buffer_info()[0], max_norm, norm.data_ptr(), ws.data_ptr(),
+                                          _lib.CLIP_WORKSPACE_BYTES, _stream(dev.index)))
     if outs is not None:
         torch.autograd.graph.increment_version(outs)
     return norm
@@ -308,7 +332,7 @@ def _tensors(tensors):
     tensors = [tensors] if torch.is_tensor(tensors) else list(tensors)
     if not tensors:
         raise ValueError("clip_grad_norm: no tensors")
-    return [t.detach() for t in tensors]
+    return tensors
 
 
 def grad_norm(tensors):
@@ -332,7 +356,7 @@ def clip_grad_norm_(parameters, max_norm):
     returns their norm before clipping."""
     parameters = [parameters] if torch.is_tensor(parameters) else list(parameters)
     max_norm = _max_norm(max_norm)
-    grads = [p.grad.detach() for p in parameters if p.grad is not None]
+    grads = [p.grad for p in parameters if p.grad is not None]
     if not grads:
         raise ValueError("clip_grad_norm_: no parameter has a gradient")
     return _clip(grads, max_norm, grads)
