@@ -23,12 +23,51 @@ namespace mpe {
 
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 
+// exp by the hardware's 2^x: off by the rounding of x log2(e), |x| 2^-24, and one step
+__device__ inline float fast_exp(float x) { return __builtin_amdgcn_exp2f(x * 1.44269504088896341f); }
+
+// 1 / (1 + e^-z); e^-z overflows to infinity and gives 0
+__device__ inline float sigmoid(float z) { return __builtin_amdgcn_rcpf(1.0f + fast_exp(-z)); }
+
+// tanh: its series below 0.3 (the next term is 6e-10 of it), elsewhere 1 - 2 / (1 + e^2|z|), which loses bits only where
+// they are far behind the point.
+__device__ inline float tanh_of(float z) {
+    const float q = z * z;
+    float s = fmaf(q, -0.00886323552990219657f, 0.0218694885361552028f);
+    s = fmaf(q, s, -0.0539682539682539683f);
+    s = fmaf(q, s, 0.133333333333333333f);
+    s = fmaf(q, s, -0.333333333333333333f);
+    const float big = copysignf(fmaf(-2.0f, __builtin_amdgcn_rcpf(1.0f + fast_exp(2.0f * fabsf(z))), 1.0f), z);
+    return fabsf(z) < 0.3f ? fmaf(z * q, s, z) : big;
+}
+
+// Phi(z) and e^(-z^2/2).  erfc(x) e^(x^2) = t Q(t) with t = 1 / (1 + 0.33 x) and Q a polynomial fitted to it over x >= 0
+// (relative error 9.4e-8), so that the far tail keeps its relative precision.
+struct Normal {
+    float phi, e;
+};
+__device__ inline Normal normal_of(float z) {
+    Normal n;
+    n.e = fast_exp(-0.5f * z * z);
+    const float t = __builtin_amdgcn_rcpf(fmaf(fabsf(z), 0.33f * 0.70710678118654752f, 1.0f));
+    float q = fmaf(t, -0.1353444f, 0.46023187f);
+    q = fmaf(t, q, -0.351141f);
+    q = fmaf(t, q, 0.40849227f);
+    q = fmaf(t, q, 0.047224592f);
+    q = fmaf(t, q, 0.20122273f);
+    q = fmaf(t, q, 0.18295613f);
+    q = fmaf(t, q, 0.1863578f);
+    const float h = 0.5f * (t * q) * n.e;
+    n.phi = z < 0.0f ? h : 1.0f - h;
+    return n;
+}
+
 __device__ inline float act_value(int act, float z) {
     switch (act) {
-        case MPE_ACT_TANH: return tanhf(z);
+        case MPE_ACT_TANH: return tanh_of(z);
         case MPE_ACT_RELU: return z > 0.0f || z != z ? z : 0.0f;
-        case MPE_ACT_GELU: return 0.5f * z * erfcf(-0.70710678118654752f * z);
-        case MPE_ACT_SILU: return z / (1.0f + expf(-z));
+        case MPE_ACT_GELU: return z * normal_of(z).phi;
+        case MPE_ACT_SILU: return z * sigmoid(z);
         default: return z;
     }
 }
@@ -36,10 +75,10 @@ __device__ inline float act_value(int act, float z) {
 __device__ inline float act_slope(int act, float z) {
     switch (act) {
         case MPE_ACT_TANH_OUT: return 1.0f - z * z;
-        case MPE_ACT_TANH: { const float t = tanhf(z); return 1.0f - t * t; }
+        case MPE_ACT_TANH: { const float t = tanh_of(z); return 1.0f - t * t; }
         case MPE_ACT_RELU: return z > 0.0f ? 1.0f : z != z ? z : 0.0f;
-        case MPE_ACT_GELU: return 0.5f * erfcf(-0.70710678118654752f * z) + z * 0.39894228040143268f * expf(-0.5f * z * z);
-        case MPE_ACT_SILU: { const float s = 1.0f / (1.0f + expf(-z)); return s * (1.0f + z * (1.0f - s)); }
+        case MPE_ACT_GELU: { const Normal n = normal_of(z); return fmaf(z * 0.39894228040143268f, n.e, n.phi); }
+        case MPE_ACT_SILU: { const float s = sigmoid(z); return s * (1.0f + z * (1.0f - s)); }
         default: return 1.0f;
     }
 }
@@ -69,8 +108,9 @@ template <typename T>
 struct Operand {
     const T* data;
     long long ld;               // may be 0 with DZ: one row for all
+    long long extent;           // elements from the first to behind the last, at least 8
     const void* pre;            // [rows][ld_pre], float (relu: T), or null: slope 1
-    long long ld_pre;
+    long long ld_pre, extent_pre;
     int act;
 };
 
@@ -79,12 +119,35 @@ __device__ inline float pre_at(const Operand<T>& o, long long at) {
     return o.act == MPE_ACT_RELU ? (float)((const T*)o.pre)[at] : ((const float*)o.pre)[at];
 }
 
+// Where a tile's vectors of W elements lie: a uniform base, and offsets from it that fit 32 bits (the host sees to it that
+// a tile's rows lie within 4 GB).  A vector that would reach beyond the matrix is moved back to end with it.
+struct Window {
+    long long base;
+    unsigned skip, last;
+    __device__ inline Window(long long extent, long long first, int w) {
+        base = min(first, extent - w);
+        skip = (unsigned)(first - base);
+        last = (unsigned)min(extent - w - base, (long long)0x7fffffff);
+    }
+    __device__ inline unsigned at(unsigned off) const { return min(skip + off, last); }
+    __device__ inline int moved(unsigned off) const { return (int)(skip + off - at(off)); }     // by how many elements
+};
+
+// v[e] = v[e + by] for 0 <= by < N; what comes in at the end is of no interest
+template <int N, typename V>
+__device__ inline void shift_down(V& v, int by) {
+#pragma unroll
+    for (int s = N / 2; s > 0; s /= 2)
+        if (by & s)
+#pragma unroll
+            for (int e = 0; e + s < N; ++e) v[e] = v[e + s];
+}
+
 // Loads a BO x BK tile of an operand into registers and writes it to LDS in pieces.  A thread's unit is one 16-byte chunk:
 // eight consecutive r of one o.  R_INNER reads a unit as one run; O_INNER reads U neighbouring o at eight r and turns them
-// by naming registers differently.  Addresses are a uniform base plus 32-bit offsets that stay the same from step to step
-// (the host sees to it that a tile's rows lie within 4 GB).  A step that lies inside the matrix takes wide loads; the
-// last step of the sum and, with O_INNER, the last tile of o read element by element from clamped places and put 0
-// where nothing is.
+// by naming registers differently.  Loads ask nothing: they take whatever lies in the vector's place (Window keeps it
+// inside the matrix).  Only in a step that reaches the end of the sum or of the matrix does fix() put the elements into
+// their places and zeros where the sum has ended; rows and columns of the output that do not exist may hold anything.
 template <typename T, int BO, int LAYOUT, bool DZ>
 struct Loader {
     typedef Piece<T> P;
@@ -94,85 +157,72 @@ struct Loader {
     static constexpr int U = UNITS >= 256 ? UNITS / 256 : 1;
     static constexpr bool SOME = UNITS < 256;       // only the first UNITS threads have one
     static constexpr int PLANE = BO * BK * 2;       // bytes of one piece's tile
+    static constexpr int NV = LAYOUT == R_INNER ? U : 8, W = LAYOUT == R_INNER ? 8 : U;      // vectors and their width
 
-    T v[U][8];
-    float z[DZ ? U : 1][8];
+    typedef T vec __attribute__((ext_vector_type(W)));      // two 16-bit elements a register
+    typedef float zvec __attribute__((ext_vector_type(W)));
+    vec v[NV];
+    zvec z[DZ ? NV : 1];
 
     static __device__ inline int row_of(int u) { return LAYOUT == R_INNER ? (threadIdx.x + u * 256) / CH : ((int)threadIdx.x % (BO / U)) * U + u; }
     static __device__ inline int chunk_of(int u) { return LAYOUT == R_INNER ? (threadIdx.x + u * 256) % CH : (int)threadIdx.x / (BO / U); }
+    // offset of vector i within the tile
+    static __device__ inline unsigned offset(int i, unsigned ld, int left_o) {
+        return LAYOUT == R_INNER ? (unsigned)min(row_of(i), left_o - 1) * ld + chunk_of(i) * 8 : (unsigned)(chunk_of(0) * 8 + i) * ld + row_of(0);
+    }
+    static __device__ inline long long first(long long o0, long long r0, long long ld) { return LAYOUT == R_INNER ? o0 * ld + r0 : r0 * ld + o0; }
 
-    // N consecutive values of the saved array from element `at` of the uniform base
-    template <int N>
-    static __device__ inline void load_pre(const Operand<T>& op, long long base, unsigned at, float* out) {
-        if (op.act == MPE_ACT_RELU) {
-            T t[N];
-            __builtin_memcpy(t, (const char*)((const T*)op.pre + base) + at * (unsigned)sizeof(T), sizeof(t));
+    __device__ inline void load(const Operand<T>& op, long long o0, long long no, long long r0) {
+        if (SOME && (int)threadIdx.x >= UNITS) return;
+        const int left_o = (int)min(no - o0, (long long)BO);
+        const Window w(op.extent, first(o0, r0, op.ld), W);
+        const char* base = (const char*)(op.data + w.base);
 #pragma unroll
-            for (int e = 0; e < N; ++e) out[e] = (float)t[e];
-        } else {
-            __builtin_memcpy(out, (const char*)((const float*)op.pre + base) + at * 4u, N * 4);
+        for (int i = 0; i < NV; ++i) __builtin_memcpy(&v[i], base + w.at(offset(i, (unsigned)op.ld, left_o)) * (unsigned)sizeof(T), W * sizeof(T));
+        if (DZ && op.pre) {
+            const Window wp(op.extent_pre, first(o0, r0, op.ld_pre), W);
+            if (op.act == MPE_ACT_RELU) {
+                const char* bp = (const char*)((const T*)op.pre + wp.base);
+#pragma unroll
+                for (int i = 0; i < NV; ++i) {
+                    vec t;
+                    __builtin_memcpy(&t, bp + wp.at(offset(i, (unsigned)op.ld_pre, left_o)) * (unsigned)sizeof(T), W * sizeof(T));
+#pragma unroll
+                    for (int e = 0; e < W; ++e) z[i][e] = (float)t[e];
+                }
+            } else {
+                const char* bp = (const char*)((const float*)op.pre + wp.base);
+#pragma unroll
+                for (int i = 0; i < NV; ++i) __builtin_memcpy(&z[i], bp + wp.at(offset(i, (unsigned)op.ld_pre, left_o)) * 4u, W * 4);
+            }
         }
     }
 
-    // rows [o0, no) and the sum's [r0, r1) exist; what lies outside reads as 0
-    __device__ inline void load(const Operand<T>& op, long long o0, long long no, long long r0, long long r1) {
+    // true for all if this step needs fix()
+    static __device__ inline bool reaches_end(const Operand<T>& op, long long o0, long long r0, long long r1) {
+        const long long span = LAYOUT == R_INNER ? (long long)(BO - 1) * op.ld + BK : (long long)(BK - 1) * op.ld + BO;
+        const long long span_pre = LAYOUT == R_INNER ? (long long)(BO - 1) * op.ld_pre + BK : (long long)(BK - 1) * op.ld_pre + BO;
+        return r0 + BK > r1 || first(o0, r0, op.ld) + span > op.extent || (DZ && op.pre && first(o0, r0, op.ld_pre) + span_pre > op.extent_pre);
+    }
+
+    __device__ inline void fix(const Operand<T>& op, long long o0, long long no, long long r0, long long r1) {
         if (SOME && (int)threadIdx.x >= UNITS) return;
-        const unsigned ld = (unsigned)op.ld, ldp = (unsigned)op.ld_pre;
-        const int left_o = (int)min(no - o0, (long long)BO), left_r = (int)min(r1 - r0, (long long)BK);     // uniform
-        const bool with_pre = DZ && op.pre;
-        if (LAYOUT == R_INNER) {
-            const T* base = op.data + o0 * op.ld + r0;
-            const long long base_pre = o0 * op.ld_pre + r0;
-            if (left_r == BK) {
+        const int left_o = (int)min(no - o0, (long long)BO), left_r = (int)min(r1 - r0, (long long)BK);
+        const Window w(op.extent, first(o0, r0, op.ld), W);
+        const Window wp(DZ && op.pre ? op.extent_pre : (long long)W, DZ && op.pre ? first(o0, r0, op.ld_pre) : 0, W);
 #pragma unroll
-                for (int u = 0; u < U; ++u) {
-                    const unsigned o = min(row_of(u), left_o - 1), r = chunk_of(u) * 8;     // a row that is not there: the last one again, never stored
-                    __builtin_memcpy(v[u], (const char*)base + (o * ld + r) * (unsigned)sizeof(T), 8 * sizeof(T));
-                    if (with_pre) load_pre<8>(op, base_pre, o * ldp + r, z[u]);
-                }
-            } else {
-#pragma unroll
-                for (int u = 0; u < U; ++u) {
-                    const unsigned o = min(row_of(u), left_o - 1);
-#pragma unroll
-                    for (int e = 0; e < 8; ++e) {
-                        const int r = chunk_of(u) * 8 + e, rc = min(r, left_r - 1);
-                        const T x = *(const T*)((const char*)base + (o * ld + rc) * (unsigned)sizeof(T));
-                        v[u][e] = r < left_r ? x : (T)0.0f;
-                        if (with_pre) load_pre<1>(op, base_pre, o * ldp + rc, &z[u][e]);
-                    }
-                }
+        for (int i = 0; i < NV; ++i) {
+            const int by = w.moved(offset(i, (unsigned)op.ld, left_o));
+            if (by > 0 && by < W) shift_down<W>(v[i], by);
+            if (DZ && op.pre) {
+                const int byp = wp.moved(offset(i, (unsigned)op.ld_pre, left_o));
+                if (byp > 0 && byp < W) shift_down<W>(z[i], byp);
             }
-        } else {
-            const T* base = op.data + r0 * op.ld + o0;
-            const long long base_pre = r0 * op.ld_pre + o0;
-            const unsigned o = row_of(0), r = chunk_of(0) * 8;
-            if (left_r == BK && left_o == BO) {
 #pragma unroll
-                for (int e = 0; e < 8; ++e) {
-                    T t[U];
-                    __builtin_memcpy(t, (const char*)(base + e * op.ld) + (r * ld + o) * (unsigned)sizeof(T), sizeof(t));
-#pragma unroll
-                    for (int u = 0; u < U; ++u) v[u][e] = t[u];
-                    if (with_pre) {
-                        float f[U];
-                        load_pre<U>(op, base_pre + e * op.ld_pre, r * ldp + o, f);
-#pragma unroll
-                        for (int u = 0; u < U; ++u) z[u][e] = f[u];
-                    }
-                }
-            } else {
-#pragma unroll
-                for (int e = 0; e < 8; ++e) {
-                    const unsigned rc = min((int)r + e, left_r - 1);
-#pragma unroll
-                    for (int u = 0; u < U; ++u) {
-                        const unsigned oc = min((int)o + u, left_o - 1);
-                        const T x = *(const T*)((const char*)base + (rc * ld + oc) * (unsigned)sizeof(T));
-                        v[u][e] = (int)r + e < left_r && (int)o + u < left_o ? x : (T)0.0f;
-                        if (with_pre) load_pre<1>(op, base_pre, rc * ldp + oc, &z[u][e]);
-                    }
-                }
+            for (int e = 0; e < W; ++e) {
+                const bool in = (LAYOUT == R_INNER ? chunk_of(i) * 8 + e : chunk_of(0) * 8 + i) < left_r;
+                v[i][e] = in ? v[i][e] : (T)0.0f;
+                if (DZ) z[i][e] = in ? z[i][e] : 0.0f;
             }
         }
     }
@@ -187,35 +237,38 @@ struct Loader {
         if (SOME && (int)threadIdx.x >= UNITS) return;
 #pragma unroll
         for (int u = 0; u < U; ++u) {
+            char* to = lds + place(row_of(u), chunk_of(u));
+            pt8 h;
+            if (P::N == 1 && !DZ && !sums) {
+#pragma unroll
+                for (int e = 0; e < 8; ++e) h[e] = LAYOUT == R_INNER ? (PT)v[u][e] : (PT)v[e][u];
+                *(pt8*)to = h;
+                continue;
+            }
             float f[8];
 #pragma unroll
-            for (int e = 0; e < 8; ++e) f[e] = (float)v[u][e];
+            for (int e = 0; e < 8; ++e) f[e] = LAYOUT == R_INNER ? (float)v[u][e] : (float)v[e][u];
             if (DZ && op.pre) {
 #pragma unroll
-                for (int e = 0; e < 8; ++e) f[e] *= act_slope(op.act, z[u][e]);
+                for (int e = 0; e < 8; ++e) f[e] *= act_slope(op.act, LAYOUT == R_INNER ? z[u][e] : z[e][u]);
             }
             if (sums) {
 #pragma unroll
                 for (int e = 0; e < 8; ++e) sums[u] += f[e];
             }
-            char* to = lds + place(row_of(u), chunk_of(u));
-            pt8 h;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) h[e] = (PT)f[e];
+            *(pt8*)to = h;
             if (P::N == 3) {
                 pt8 m, l;
 #pragma unroll
                 for (int e = 0; e < 8; ++e) {
-                    h[e] = (PT)f[e];
                     const float rest = f[e] - (float)h[e];
                     m[e] = (PT)rest;
                     l[e] = (PT)(rest - (float)m[e]);
                 }
-                *(pt8*)to = h;
                 *(pt8*)(to + PLANE) = m;
                 *(pt8*)(to + 2 * PLANE) = l;
-            } else {
-#pragma unroll
-                for (int e = 0; e < 8; ++e) h[e] = DZ ? (PT)f[e] : (PT)v[u][e];
-                *(pt8*)to = h;
             }
         }
     }
@@ -306,6 +359,30 @@ __device__ inline void finish(const ProductArgs<T>& a, unsigned split, long long
     put<T, N>(a.out + j * a.ldo + i, o, mask);
 }
 
+// Operands of fewer than eight elements, for which there is no vector to load: a thread an element of the output, whose sum
+// then has fewer than eight terms (of an expanded dy: as many as there are rows).
+template <typename T, int EPI, int PL, int QL, bool DZ>
+__global__ __launch_bounds__(256) void product_few(const ProductArgs<T> a, int splits) {
+    const long long n = a.ni * a.nj * splits;
+    for (long long at = (long long)blockIdx.x * 256 + threadIdx.x; at < n; at += (long long)gridDim.x * 256) {
+        const long long i = at % a.ni, j = at / a.ni % a.nj;
+        const unsigned split = (unsigned)(at / (a.ni * a.nj));
+        const long long r0 = split * a.r_split, r1 = EPI == EPI_PARTIAL ? min(r0 + a.r_split, a.nr) : a.nr;
+        const float bias[1] = {EPI == EPI_FORWARD && a.bias ? (float)a.bias[i] : 0.0f};
+        const float f[1] = {plain_sum<T, PL, QL, DZ>(a.p, a.q, i, j, r0, r1)};
+        finish<T, EPI, 1>(a, split, i, j, 1u, bias, f);
+        if (EPI == EPI_PARTIAL && a.partial_sum && i == 0) {
+            float s = 0.0f;
+            for (long long r = r0; r < r1; ++r) {
+                float b = (float)a.q.data[r * a.q.ld + j];
+                if (DZ && a.q.pre) b *= act_slope(a.q.act, pre_at(a.q, r * a.q.ld_pre + j));
+                s += b;
+            }
+            a.partial_sum[split * a.nj + j] = s;
+        }
+    }
+}
+
 // Workgroups are dealt to the eight XCDs in turn; this gives every XCD a run of neighbouring tiles, which share operands in
 // its L2.
 __device__ inline unsigned xcd_run(unsigned b, unsigned n) {
@@ -314,7 +391,7 @@ __device__ inline unsigned xcd_run(unsigned b, unsigned n) {
 }
 
 template <typename T, int EPI, int PL, int QL, bool DZ, int BI, int BJ, int WI, int WJ>
-__global__ __launch_bounds__(256) void product(const ProductArgs<T> a) {
+__global__ __launch_bounds__(256, BI * BJ > 8192 ? 2 : 3) void product(const ProductArgs<T> a) {
     typedef Piece<T> P;
     typedef typename P::type PT;
     typedef PT pt8 __attribute__((ext_vector_type(8)));
@@ -343,15 +420,17 @@ __global__ __launch_bounds__(256) void product(const ProductArgs<T> a) {
 
     LP gp;
     LQ gq;
-    gp.load(a.p, i0, a.ni, r0, r1);
-    gq.load(a.q, j0, a.nj, r0, r1);
+    gp.load(a.p, i0, a.ni, r0);
+    gq.load(a.q, j0, a.nj, r0);
     for (long long r = r0; r < r1; r += BK) {
+        if (LP::reaches_end(a.p, i0, r, r1)) gp.fix(a.p, i0, a.ni, r, r1);
+        if (LQ::reaches_end(a.q, j0, r, r1)) gq.fix(a.q, j0, a.nj, r, r1);
         gp.store(a.p, lp, nullptr);
         gq.store(a.q, lq, want_sums ? sums : nullptr);
         __syncthreads();
         if (r + BK < r1) {
-            gp.load(a.p, i0, a.ni, r + BK, r1);
-            gq.load(a.q, j0, a.nj, r + BK, r1);
+            gp.load(a.p, i0, a.ni, r + BK);
+            gq.load(a.q, j0, a.nj, r + BK);
         }
 #pragma unroll
         for (int kk = 0; kk < BK / 32; ++kk) {

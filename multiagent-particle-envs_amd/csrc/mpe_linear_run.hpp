@@ -46,6 +46,11 @@ template <typename T, int EPI, int PL, int QL, bool DZ, int BI, int BJ, int WI, 
 inline hipError_t launch_product(ProductArgs<T> a, int splits, hipStream_t st) {
     const long long ti = tiles_of(a.ni, BI), tiles = ti * tiles_of(a.nj, BJ);
     if (tiles * splits > 0x7fffffffLL) return hipErrorInvalidValue;
+    if (a.p.extent < 8 || a.q.extent < 8 || (a.q.pre && a.q.extent_pre < 8)) {
+        const long long want = (a.ni * a.nj * splits + 255) / 256;
+        hipLaunchKernelGGL((product_few<T, EPI, PL, QL, DZ>), dim3((unsigned)(want < 8192 ? want : 8192)), dim3(256), 0, st, a, splits);
+        return hipGetLastError();
+    }
     a.ti = (int)ti;
     a.tiles = (unsigned)tiles;
     hipLaunchKernelGGL((product<T, EPI, PL, QL, DZ, BI, BJ, WI, WJ>), dim3((unsigned)(tiles * splits)), dim3(256), 0, st, a);
@@ -96,8 +101,8 @@ struct LinearRun {
 
     static hipError_t forward(const LinearArgs& a, hipStream_t st) {
         ProductArgs<T> g = {};
-        g.p = {(const T*)a.w, a.ldw, nullptr, 0, 0};
-        g.q = {(const T*)a.x, a.ldx, nullptr, 0, 0};
+        g.p = {(const T*)a.w, a.ldw, (a.n - 1) * a.ldw + a.k, nullptr, 0, 0, 0};
+        g.q = {(const T*)a.x, a.ldx, (a.m - 1) * a.ldx + a.k, nullptr, 0, 0, 0};
         g.ni = a.n; g.nj = a.m; g.nr = a.k;
         g.out = (T*)a.y; g.ldo = a.ldy;
         g.bias = (const T*)a.bias; g.residual = (const T*)a.residual; g.ldr = a.ldr; g.pre = a.pre; g.act = a.act;
@@ -120,19 +125,19 @@ struct LinearRun {
             return e;
         }
         char* ws = (char*)a.ws;
-        Operand<T> dz = {(const T*)a.dy, a.lddy, a.act != MPE_ACT_NONE ? a.pre : nullptr, a.n, a.act};
+        Operand<T> dz = {(const T*)a.dy, a.lddy, (a.m - 1) * a.lddy + a.n, a.act != MPE_ACT_NONE ? a.pre : nullptr, a.n, a.m * a.n, a.act};
         const bool own = own_dz(a.act, a.k);
         if (own) {
             const long long want = (a.m * a.n + 255) / 256;
             hipLaunchKernelGGL((slope_pass<T>), dim3((unsigned)(want < 8192 ? want : 8192)), dim3(256), 0, st, a.m, a.n, (const T*)a.dy, a.lddy, (const void*)a.pre, a.act, (T*)ws);
             e = hipGetLastError();
             if (e != hipSuccess) return e;
-            dz = {(const T*)ws, a.n, nullptr, 0, MPE_ACT_NONE};
+            dz = {(const T*)ws, a.n, a.m * a.n, nullptr, 0, 0, MPE_ACT_NONE};
             ws += round_up(a.m * a.n * (long long)sizeof(T));
         }
         if (a.dx) {
             ProductArgs<T> g = {};
-            g.p = {(const T*)a.w, a.ldw, nullptr, 0, 0};
+            g.p = {(const T*)a.w, a.ldw, (a.n - 1) * a.ldw + a.k, nullptr, 0, 0, 0};
             g.q = dz;
             g.ni = a.k; g.nj = a.m; g.nr = a.n;
             g.out = (T*)a.dx; g.ldo = a.lddx;
@@ -142,7 +147,7 @@ struct LinearRun {
         if (a.dw || a.db) {
             const WeightPlan p = weight_plan(Piece<T>::BK, a.m, a.n, a.k);
             ProductArgs<T> g = {};
-            g.p = {(const T*)a.x, a.ldx, nullptr, 0, 0};
+            g.p = {(const T*)a.x, a.ldx, (a.m - 1) * a.ldx + a.k, nullptr, 0, 0, 0};
             g.q = dz;
             g.ni = a.k; g.nj = a.n; g.nr = a.m; g.r_split = p.r_split;
             g.partial = (float*)ws;

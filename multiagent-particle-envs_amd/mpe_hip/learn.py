@@ -63,8 +63,8 @@ def _rows(t, cols):
 
 
 def _rows_or_one(t, cols):
-    """As _rows, but one row repeated by ``expand`` stays one row (stride 0)."""
-    if not t.is_contiguous() and t.dim() >= 2 and t.numel() > 0 and (cols == 1 or t.stride(-1) == 1) \
+    """As _rows, but one row of a vector's length or more that is repeated by ``expand`` stays one row (stride 0)."""
+    if cols >= 8 and not t.is_contiguous() and t.dim() >= 2 and t.numel() > 0 and t.stride(-1) == 1 \
             and all(s == 0 or n == 1 for s, n in zip(t.stride()[:-1], t.shape[:-1])):
         return t, 0
     return _rows(t, cols)

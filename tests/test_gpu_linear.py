@@ -146,6 +146,42 @@ def test_backward(m, k, n, dt):
 
 
 @pytest.mark.parametrize("dt", DTYPES)
+def test_the_smallest_matrices(dt):
+    """Operands shorter than a vector, and matrices that end inside one, in every combination."""
+    for m in (1, 2, 3, 7, 9):
+        for k in (1, 2, 3, 5, 7, 8, 9, 15):
+            for n in (1, 2, 3, 4, 6, 7, 9):
+                x, w, b, r, dy = make(m, k, n, dt, residual=(m + k + n) % 2 == 0)
+                check_forward(x, w, b, r, "tanh")
+                check_backward(x, w, b, r, dy, "tanh")
+    for k, ld in ((1, 3), (3, 4), (5, 7)):
+        x, w, b, r, dy = make(70, k, 3, dt, ld=ld)
+        check_forward(x, w, b, r, "silu")
+        check_backward(x, w, b, r, dy, "silu")
+
+
+@pytest.mark.parametrize("dt", DTYPES)
+@pytest.mark.parametrize("n", [1, 5, 12, 130])
+def test_matrices_that_end_where_memory_ends(dt, n):
+    """The last row's last vector: inputs that are the last elements of their buffers, with NaN all around them, give the same
+    as inputs that stand alone."""
+    import mpe_hip
+    for m, k in ((65, 33), (129, 14), (40, 258), (300, 7)):
+        x, w, b, r, dy = make(m, k, n, dt, residual=True)
+        def framed(t):
+            flat = torch.full((t.numel() + 64,), math.nan, device=DEV).to(dt)
+            v = flat[33:33 + t.numel()].view(t.shape)
+            v.copy_(t)
+            return v
+        for act in ("gelu", "relu", "none"):
+            a = [t.detach().clone().requires_grad_(True) for t in (x, w, b, r)]
+            f = [framed(t).requires_grad_(True) for t in (x, w, b, r)]
+            one, two = (mpe_hip.linear(q[0], q[1], q[2], activation=act, residual=q[3]) for q in (a, f))
+            assert torch.equal(one, two)
+            assert all(torch.equal(p, q) for p, q in zip(torch.autograd.grad(one, a, dy), torch.autograd.grad(two, f, framed(dy))))
+
+
+@pytest.mark.parametrize("dt", DTYPES)
 def test_long_reduction_over_rows(dt):
     """The weight gradient of a whole rollout step: many rows, few columns."""
     x, w, b, r, dy = make(70001, 14, 9, dt)
