@@ -75,6 +75,15 @@ struct LinearArgs {
     void* db;               // may be null
     void* ws;
 };
+// one element type's passes
+struct LinearOps {
+    long long (*backward_workspace)(int act, long long m, long long n, long long k);
+    hipError_t (*forward)(const LinearArgs& a, hipStream_t st);
+    hipError_t (*backward)(const LinearArgs& a, hipStream_t st);
+};
+const LinearOps& linear_f32();
+const LinearOps& linear_bf16();
+const LinearOps& linear_f16();
 long long linear_forward_workspace(int dtype, long long m, long long n, long long k);
 long long linear_backward_workspace(int dtype, int act, long long m, long long n, long long k);
 hipError_t launch_linear_forward(const LinearArgs& a, hipStream_t st);

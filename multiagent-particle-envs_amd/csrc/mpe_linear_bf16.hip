@@ -3,6 +3,9 @@
 
 namespace mpe {
 
-template struct LinearRun<bf16>;
+const LinearOps& linear_bf16() {
+    static const LinearOps ops = {LinearRun<bf16>::backward_workspace, LinearRun<bf16>::forward, LinearRun<bf16>::backward};
+    return ops;
+}
 
 }  // namespace mpe

@@ -3,6 +3,9 @@
 
 namespace mpe {
 
-template struct LinearRun<f16>;
+const LinearOps& linear_f16() {
+    static const LinearOps ops = {LinearRun<f16>::backward_workspace, LinearRun<f16>::forward, LinearRun<f16>::backward};
+    return ops;
+}
 
 }  // namespace mpe

@@ -3,6 +3,9 @@
 
 namespace mpe {
 
-template struct LinearRun<float>;
+const LinearOps& linear_f32() {
+    static const LinearOps ops = {LinearRun<float>::backward_workspace, LinearRun<float>::forward, LinearRun<float>::backward};
+    return ops;
+}
 
 }  // namespace mpe

@@ -302,7 +302,9 @@ struct ProductArgs {
     long long ldr;
     void* pre;
     int act;
-    float *partial, *partial_sum;   // EPI_PARTIAL: [split][nj][ni], and [split][nj] or null
+    float* partial;             // EPI_PARTIAL: [split], of [nj][ni] products and, with_sums, [nj] sums of Q over r
+    long long partial_ld;       // floats a split
+    int with_sums;
 };
 
 // Finishes N consecutive elements of row j: those whose bit is set in mask.
@@ -322,7 +324,7 @@ __device__ inline void finish(const ProductArgs<T>& a, unsigned split, long long
 #pragma unroll
     for (int e = 0; e < N; ++e) f[e] = sum[e];
     if (EPI == EPI_PARTIAL) {
-        put<float, N>(a.partial + ((long long)split * a.nj + j) * a.ni + i, f, mask);
+        put<float, N>(a.partial + split * a.partial_ld + j * a.ni + i, f, mask);
         return;
     }
     T o[N];
@@ -371,14 +373,14 @@ __global__ __launch_bounds__(256) void product_few(const ProductArgs<T> a, int s
         const float bias[1] = {EPI == EPI_FORWARD && a.bias ? (float)a.bias[i] : 0.0f};
         const float f[1] = {plain_sum<T, PL, QL, DZ>(a.p, a.q, i, j, r0, r1)};
         finish<T, EPI, 1>(a, split, i, j, 1u, bias, f);
-        if (EPI == EPI_PARTIAL && a.partial_sum && i == 0) {
+        if (EPI == EPI_PARTIAL && a.with_sums && i == 0) {
             float s = 0.0f;
             for (long long r = r0; r < r1; ++r) {
                 float b = (float)a.q.data[r * a.q.ld + j];
                 if (DZ && a.q.pre) b *= act_slope(a.q.act, pre_at(a.q, r * a.q.ld_pre + j));
                 s += b;
             }
-            a.partial_sum[split * a.nj + j] = s;
+            a.partial[split * a.partial_ld + a.nj * a.ni + j] = s;
         }
     }
 }
@@ -398,7 +400,10 @@ __global__ __launch_bounds__(256, BI * BJ > 8192 ? 2 : 3) void product(const Pro
     typedef Loader<T, BI, PL, false> LP;
     typedef Loader<T, BJ, QL, DZ> LQ;
     constexpr int NP = P::N, BK = P::BK, FI = BI / WI / 16, FJ = BJ / WJ / 16;
-    __shared__ __attribute__((aligned(16))) char lds[NP * (LP::PLANE + LQ::PLANE)];
+    // the results pass through LDS too, ROWS rows at a time, so that they leave as whole rows from a loop of little code
+    constexpr int HALVES = BI * BJ > 8192 ? 2 : 1, ROWS = BJ / HALVES, PITCH = BI + 4;
+    constexpr int TILES = NP * (LP::PLANE + LQ::PLANE), RESULTS = ROWS * PITCH * 4;
+    __shared__ __attribute__((aligned(16))) char lds[TILES > RESULTS ? TILES : RESULTS];
     char* const lp = lds;
     char* const lq = lds + NP * LP::PLANE;
 
@@ -416,7 +421,7 @@ __global__ __launch_bounds__(256, BI * BJ > 8192 ? 2 : 3) void product(const Pro
     float sums[LQ::U];
 #pragma unroll
     for (int u = 0; u < LQ::U; ++u) sums[u] = 0.0f;
-    const bool want_sums = EPI == EPI_PARTIAL && a.partial_sum && i0 == 0;
+    const bool want_sums = EPI == EPI_PARTIAL && a.with_sums && i0 == 0;
 
     LP gp;
     LQ gq;
@@ -476,63 +481,42 @@ __global__ __launch_bounds__(256, BI * BJ > 8192 ? 2 : 3) void product(const Pro
             if ((int)threadIdx.x < BJ && j0 + threadIdx.x < a.nj) {
                 float tot = 0.0f;
                 for (int c = 0; c < LQ::CH; ++c) tot += s[c * BJ + threadIdx.x];
-                a.partial_sum[split * a.nj + j0 + threadIdx.x] = tot;
+                a.partial[split * a.partial_ld + a.nj * a.ni + j0 + threadIdx.x] = tot;
             }
         }
     }
 
-    // Results that are not finite are left out here, noted in LDS and summed again below.
-    constexpr bool AGAIN = NP == 3;
-    unsigned* const again = (unsigned*)lds;
-    static_assert(!AGAIN || BI * BJ / 8 <= (int)sizeof(lds), "a bit for every element");
-    bool bad = false;
-    if (AGAIN) {
+    const int it = threadIdx.x % (BI / 4) * 4;      // a thread's four columns, the same in every row it takes
+    const long long i = i0 + it;
+    const int have = (int)max(0LL, min(4LL, a.ni - i));
+    const unsigned mask = (1u << have) - 1;
+    float bias[4];
 #pragma unroll
-        for (int y = 0; y < FJ; ++y)
+    for (int e = 0; e < 4; ++e) bias[e] = EPI == EPI_FORWARD && a.bias && e < have ? (float)a.bias[i + e] : 0.0f;
+    float* const res = (float*)lds;
 #pragma unroll
-            for (int x = 0; x < FI; ++x)
-#pragma unroll
-                for (int e = 0; e < 4; ++e) bad = bad || !(fabsf(acc[x][y][e]) < INFINITY);
-        bad = __syncthreads_or(bad);
-        if (bad) {
-            for (int w = threadIdx.x; w < BI * BJ / 32; w += 256) again[w] = 0;
-            __syncthreads();
-        }
-    }
-#pragma unroll
-    for (int x = 0; x < FI; ++x) {
-        const int it = wi + x * 16 + (lane >> 4) * 4;
-        const long long i = i0 + it;
-        const int have = a.ni - i < 4 ? (int)(a.ni - i) : 4;
-        if (have <= 0) continue;
-        float bias[4];
-#pragma unroll
-        for (int e = 0; e < 4; ++e) bias[e] = EPI == EPI_FORWARD && a.bias && e < have ? (float)a.bias[i + e] : 0.0f;
-#pragma unroll
-        for (int y = 0; y < FJ; ++y) {
-            const int jt = wj + y * 16 + (lane & 15);
-            const long long j = j0 + jt;
-            if (j >= a.nj) continue;
-            unsigned mask = (1u << have) - 1;       // of the four elements
-            if (AGAIN && bad) {
-#pragma unroll
-                for (int e = 0; e < 4; ++e)
-                    if (e < have && !(fabsf(acc[x][y][e]) < INFINITY)) {
-                        mask &= ~(1u << e);
-                        atomicOr(&again[(jt * BI + it + e) >> 5], 1u << ((it + e) & 31));
-                    }
-            }
-            finish<T, EPI, 4>(a, split, i, j, mask, bias, acc[x][y]);
-        }
-    }
-    if (AGAIN && bad) {
+    for (int half = 0; half < HALVES; ++half) {
         __syncthreads();
-        for (int n = threadIdx.x; n < BI * BJ; n += 256) {
-            if (!(again[n >> 5] >> (n & 31) & 1)) continue;
-            const long long i = i0 + n % BI, j = j0 + n / BI;
-            const float bias[1] = {EPI == EPI_FORWARD && a.bias ? (float)a.bias[i] : 0.0f};
-            const float f[1] = {plain_sum<T, PL, QL, DZ>(a.p, a.q, i, j, r0, r1)};
-            finish<T, EPI, 1>(a, split, i, j, 1u, bias, f);
+        if (wj / ROWS == half) {
+#pragma unroll
+            for (int y = 0; y < FJ; ++y)
+#pragma unroll
+                for (int x = 0; x < FI; ++x) *(f32x4*)&res[(wj % ROWS + y * 16 + (lane & 15)) * PITCH + wi + x * 16 + (lane >> 4) * 4] = acc[x][y];
+        }
+        __syncthreads();
+        const int rows = (int)min((long long)ROWS, a.nj - j0 - half * ROWS);
+        if (have > 0) {
+#pragma unroll 2
+            for (int jt = threadIdx.x / (BI / 4); jt < rows; jt += 1024 / BI) {
+                const long long j = j0 + half * ROWS + jt;
+                f32x4 f = *(const f32x4*)&res[jt * PITCH + it];
+                if (NP == 3) {
+#pragma unroll
+                    for (int e = 0; e < 4; ++e)
+                        if (!(fabsf(f[e]) < INFINITY) && e < have) f[e] = plain_sum<T, PL, QL, DZ>(a.p, a.q, i + e, j, r0, r1);
+                }
+                finish<T, EPI, 4>(a, split, i, j, mask, bias, f);
+            }
         }
     }
 }

@@ -15,28 +15,41 @@ __global__ __launch_bounds__(256) void slope_pass(long long m, long long n, cons
     }
 }
 
-// ---- sums of the splits: out[c] = sum_s partial[s][c], in the order of s within a group of rows, then of the groups ----
-template <typename T, int COLS>
-__global__ __launch_bounds__(256) void add_splits(const float* __restrict__ partial, int splits, long long n, T* __restrict__ out) {
-    constexpr int G = 256 / COLS;
-    __shared__ float part[G][COLS];
+// ---- sums of the splits: column c of [splits][ld], in the order of the splits within a group and then of the groups ----
+// The first n columns go to out, the next ones to sums; either may be null.
+template <typename T, int COLS, int GROUPS>
+__global__ __launch_bounds__(COLS * GROUPS) void add_splits(const float* __restrict__ partial, int splits, long long ld, long long n, T* __restrict__ out,
+                                                            T* __restrict__ sums) {
+    __shared__ float part[GROUPS][COLS];
     const int c = threadIdx.x % COLS, g = threadIdx.x / COLS;
     const long long at = (long long)blockIdx.x * COLS + c;
+    const bool here = at < ld && (at < n ? out : sums) != nullptr;
     float s = 0.0f;
-    if (at < n)
-        for (int k = g; k < splits; k += G) s += partial[(long long)k * n + at];
+    if (here) {
+        int k = g;
+        for (; k + 3 * GROUPS < splits; k += 4 * GROUPS) {
+            float v[4];
+#pragma unroll
+            for (int u = 0; u < 4; ++u) v[u] = partial[(k + u * GROUPS) * ld + at];
+#pragma unroll
+            for (int u = 0; u < 4; ++u) s += v[u];
+        }
+        for (; k < splits; k += GROUPS) s += partial[k * ld + at];
+    }
     part[g][c] = s;
     __syncthreads();
-    if (g == 0 && at < n) {
-        for (int k = 1; k < G; ++k) s += part[k][c];
-        out[at] = (T)s;
+    if (g == 0 && here) {
+        for (int k = 1; k < GROUPS; ++k) s += part[k][c];
+        if (at < n) out[at] = (T)s;
+        else sums[at - n] = (T)s;
     }
 }
 
+// Few columns and many splits take 64 threads a column, many columns have threads enough with 4.
 template <typename T>
-inline hipError_t launch_add_splits(const float* partial, int splits, long long n, T* out, hipStream_t st) {
-    if (n >= 65536) hipLaunchKernelGGL((add_splits<T, 64>), dim3((unsigned)((n + 63) / 64)), dim3(256), 0, st, partial, splits, n, out);
-    else hipLaunchKernelGGL((add_splits<T, 16>), dim3((unsigned)((n + 15) / 16)), dim3(256), 0, st, partial, splits, n, out);
+inline hipError_t launch_add_splits(const float* partial, int splits, long long ld, long long n, T* out, T* sums, hipStream_t st) {
+    if (ld >= 65536) hipLaunchKernelGGL((add_splits<T, 64, 4>), dim3((unsigned)((ld + 63) / 64)), dim3(256), 0, st, partial, splits, ld, n, out, sums);
+    else hipLaunchKernelGGL((add_splits<T, 16, 64>), dim3((unsigned)((ld + 15) / 16)), dim3(1024), 0, st, partial, splits, ld, n, out, sums);
     return hipGetLastError();
 }
 
@@ -77,7 +90,10 @@ inline WeightPlan weight_plan(int bk, long long m, long long n, long long k) {
     p.bi = k <= 16 ? 16 : n <= 16 || k <= 64 || n <= 64 ? 64 : 128;
     p.bj = p.bi == 128 ? 128 : p.bi == 64 && n <= 16 ? 16 : 64;
     const long long tiles = tiles_of(k, p.bi) * tiles_of(n, p.bj);
-    long long s = 1024 / tiles;
+#ifndef TARGET
+#define TARGET 1024
+#endif
+    long long s = TARGET / tiles;
     const long long most = tiles_of(m, 4 * bk);      // at least four steps each
     if (s > most) s = most;
     if (s < 1) s = 1;
@@ -96,7 +112,7 @@ struct LinearRun {
     static long long backward_workspace(int act, long long m, long long n, long long k) {
         if (m == 0) return 0;
         const WeightPlan p = weight_plan(Piece<T>::BK, m, n, k);
-        return (own_dz(act, k) ? round_up(m * n * (long long)sizeof(T)) : 0) + round_up(p.splits * n * k * 4) + round_up(p.splits * n * 4);
+        return (own_dz(act, k) ? round_up(m * n * (long long)sizeof(T)) : 0) + p.splits * (n * k + n) * 4;
     }
 
     static hipError_t forward(const LinearArgs& a, hipStream_t st) {
@@ -120,9 +136,7 @@ struct LinearRun {
     static hipError_t backward(const LinearArgs& a, hipStream_t st) {
         hipError_t e = hipSuccess;
         if (a.m == 0) {         // no rows: the gradients are empty sums
-            if (a.dw) e = launch_add_splits<T>(nullptr, 0, a.n * a.k, (T*)a.dw, st);
-            if (e == hipSuccess && a.db) e = launch_add_splits<T>(nullptr, 0, a.n, (T*)a.db, st);
-            return e;
+            return launch_add_splits<T>(nullptr, 0, a.n * a.k + a.n, a.n * a.k, (T*)a.dw, (T*)a.db, st);
         }
         char* ws = (char*)a.ws;
         Operand<T> dz = {(const T*)a.dy, a.lddy, (a.m - 1) * a.lddy + a.n, a.act != MPE_ACT_NONE ? a.pre : nullptr, a.n, a.m * a.n, a.act};
@@ -151,10 +165,10 @@ struct LinearRun {
             g.q = dz;
             g.ni = a.k; g.nj = a.n; g.nr = a.m; g.r_split = p.r_split;
             g.partial = (float*)ws;
-            g.partial_sum = a.db ? (float*)(ws + round_up(p.splits * a.n * a.k * 4)) : nullptr;
+            g.partial_ld = a.n * a.k + a.n;
+            g.with_sums = a.db != nullptr;
             e = dz.pre ? weights<true>(g, p, st) : weights<false>(g, p, st);
-            if (e == hipSuccess && a.dw) e = launch_add_splits<T>(g.partial, p.splits, a.n * a.k, (T*)a.dw, st);
-            if (e == hipSuccess && a.db) e = launch_add_splits<T>(g.partial_sum, p.splits, a.n, (T*)a.db, st);
+            if (e == hipSuccess) e = launch_add_splits<T>(g.partial, p.splits, g.partial_ld, a.n * a.k, (T*)a.dw, (T*)a.db, st);
         }
         return e;
     }
