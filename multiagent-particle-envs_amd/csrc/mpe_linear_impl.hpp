@@ -145,9 +145,9 @@ __device__ inline void shift_down(V& v, int by) {
 
 // Loads a BO x BK tile of an operand into registers and writes it to LDS in pieces.  A thread's unit is one 16-byte chunk:
 // eight consecutive r of one o.  R_INNER reads a unit as one run; O_INNER reads U neighbouring o at eight r and turns them
-// by naming registers differently.  Loads ask nothing: they take whatever lies in the vector's place (Window keeps it
-// inside the matrix).  Only in a step that reaches the end of the sum or of the matrix does fix() put the elements into
-// their places and zeros where the sum has ended; rows and columns of the output that do not exist may hold anything.
+// by naming registers differently.  Loads ask nothing: they take whatever lies in the vector's place.  Only in the steps
+// that reach the end of the sum or of the matrix does a Window keep them inside it, and fix() puts the elements into their
+// places and zeros where the sum has ended; rows and columns of the output that do not exist may hold anything.
 template <typename T, int BO, int LAYOUT, bool DZ>
 struct Loader {
     typedef Piece<T> P;
@@ -164,6 +164,13 @@ struct Loader {
     vec v[NV];
     zvec z[DZ ? NV : 1];
 
+    // What stays the same from step to step: the vectors' offsets within the tile and, uniform, the place of the next step
+    // and how many steps lie wholly inside the matrix (their loads are plain and need no fix()).
+    unsigned off[LAYOUT == R_INNER ? U : 1], off_pre[DZ ? (LAYOUT == R_INNER ? U : 1) : 1];
+    const char *next, *next_pre;
+    long long row_bytes, row_bytes_pre;
+    int inside;
+
     static __device__ inline int row_of(int u) { return LAYOUT == R_INNER ? (threadIdx.x + u * 256) / CH : ((int)threadIdx.x % (BO / U)) * U + u; }
     static __device__ inline int chunk_of(int u) { return LAYOUT == R_INNER ? (threadIdx.x + u * 256) % CH : (int)threadIdx.x / (BO / U); }
     // offset of vector i within the tile
@@ -171,9 +178,70 @@ struct Loader {
         return LAYOUT == R_INNER ? (unsigned)min(row_of(i), left_o - 1) * ld + chunk_of(i) * 8 : (unsigned)(chunk_of(0) * 8 + i) * ld + row_of(0);
     }
     static __device__ inline long long first(long long o0, long long r0, long long ld) { return LAYOUT == R_INNER ? o0 * ld + r0 : r0 * ld + o0; }
+    static __device__ inline unsigned pre_size(const Operand<T>& op) { return op.act == MPE_ACT_RELU ? (unsigned)sizeof(T) : 4u; }
 
-    __device__ inline void load(const Operand<T>& op, long long o0, long long no, long long r0) {
-        if (SOME && (int)threadIdx.x >= UNITS) return;
+    // steps from r0 on, of `steps`, whose vectors all end inside the matrix
+    static __device__ inline int steps_inside(long long extent, long long ld, long long o0, long long r0, int steps) {
+        const long long room = extent - first(o0, r0, ld) - (LAYOUT == R_INNER ? (long long)(BO - 1) * ld + BK : (long long)(BK - 1) * ld + BO);
+        const long long stride = LAYOUT == R_INNER ? (long long)BK : BK * ld;
+        if (room < 0) return 0;
+        return stride == 0 ? steps : (int)min((long long)steps, room / stride + 1);
+    }
+
+    __device__ inline void init(const Operand<T>& op, long long o0, long long no, long long r0, long long r1) {
+        const int left_o = (int)min(no - o0, (long long)BO);
+#pragma unroll
+        for (int i = 0; i < (LAYOUT == R_INNER ? U : 1); ++i) {
+            off[i] = offset(i, (unsigned)op.ld, left_o) * (unsigned)sizeof(T);
+            if (DZ) off_pre[i] = op.pre ? offset(i, (unsigned)op.ld_pre, left_o) * pre_size(op) : 0u;
+        }
+        next = (const char*)(op.data + first(o0, r0, op.ld));
+        row_bytes = op.ld * (long long)sizeof(T);
+        row_bytes_pre = DZ && op.pre ? op.ld_pre * pre_size(op) : 0;
+        inside = steps_inside(op.extent, op.ld, o0, r0, (int)((r1 - r0) / BK));      // the step in which the sum ends is not one of them
+        if (DZ && op.pre) {
+            next_pre = (const char*)op.pre + first(o0, r0, op.ld_pre) * pre_size(op);
+            inside = min(inside, steps_inside(op.extent_pre, op.ld_pre, o0, r0, inside));
+        }
+    }
+
+    __device__ inline void load(const Operand<T>& op, long long o0, long long no, long long r0, int step) {
+        if (!SOME || (int)threadIdx.x < UNITS) {
+            if (step < inside) {
+                const char* p = next;
+#pragma unroll
+                for (int i = 0; i < NV; ++i) {
+                    __builtin_memcpy(&v[i], p + off[LAYOUT == R_INNER ? i : 0], W * sizeof(T));
+                    if (LAYOUT == O_INNER) p += row_bytes;
+                }
+                if (DZ && op.pre) {
+                    const char* q = next_pre;
+                    if (op.act == MPE_ACT_RELU) {
+#pragma unroll
+                        for (int i = 0; i < NV; ++i) {
+                            vec t;
+                            __builtin_memcpy(&t, q + off_pre[LAYOUT == R_INNER ? i : 0], W * sizeof(T));
+                            if (LAYOUT == O_INNER) q += row_bytes_pre;
+#pragma unroll
+                            for (int e = 0; e < W; ++e) z[i][e] = (float)t[e];
+                        }
+                    } else {
+#pragma unroll
+                        for (int i = 0; i < NV; ++i) {
+                            __builtin_memcpy(&z[i], q + off_pre[LAYOUT == R_INNER ? i : 0], W * 4);
+                            if (LAYOUT == O_INNER) q += row_bytes_pre;
+                        }
+                    }
+                }
+            } else {
+                load_edge(op, o0, no, r0);
+            }
+        }
+        next += LAYOUT == R_INNER ? (long long)(BK * sizeof(T)) : BK * row_bytes;
+        if (DZ && op.pre) next_pre += LAYOUT == R_INNER ? (long long)(BK * pre_size(op)) : BK * row_bytes_pre;
+    }
+
+    __device__ inline void load_edge(const Operand<T>& op, long long o0, long long no, long long r0) {
         const int left_o = (int)min(no - o0, (long long)BO);
         const Window w(op.extent, first(o0, r0, op.ld), W);
         const char* base = (const char*)(op.data + w.base);
@@ -196,13 +264,6 @@ struct Loader {
                 for (int i = 0; i < NV; ++i) __builtin_memcpy(&z[i], bp + wp.at(offset(i, (unsigned)op.ld_pre, left_o)) * 4u, W * 4);
             }
         }
-    }
-
-    // true for all if this step needs fix()
-    static __device__ inline bool reaches_end(const Operand<T>& op, long long o0, long long r0, long long r1) {
-        const long long span = LAYOUT == R_INNER ? (long long)(BO - 1) * op.ld + BK : (long long)(BK - 1) * op.ld + BO;
-        const long long span_pre = LAYOUT == R_INNER ? (long long)(BO - 1) * op.ld_pre + BK : (long long)(BK - 1) * op.ld_pre + BO;
-        return r0 + BK > r1 || first(o0, r0, op.ld) + span > op.extent || (DZ && op.pre && first(o0, r0, op.ld_pre) + span_pre > op.extent_pre);
     }
 
     __device__ inline void fix(const Operand<T>& op, long long o0, long long no, long long r0, long long r1) {
@@ -393,7 +454,7 @@ __device__ inline unsigned xcd_run(unsigned b, unsigned n) {
 }
 
 template <typename T, int EPI, int PL, int QL, bool DZ, int BI, int BJ, int WI, int WJ>
-__global__ __launch_bounds__(256, BI * BJ > 8192 ? 2 : 3) void product(const ProductArgs<T> a) {
+__global__ __launch_bounds__(256, BI * BJ > 8192 ? 2 : BI * BJ > 4096 ? 3 : 4) void product(const ProductArgs<T> a) {
     typedef Piece<T> P;
     typedef typename P::type PT;
     typedef PT pt8 __attribute__((ext_vector_type(8)));
@@ -425,17 +486,20 @@ __global__ __launch_bounds__(256, BI * BJ > 8192 ? 2 : 3) void product(const Pro
 
     LP gp;
     LQ gq;
-    gp.load(a.p, i0, a.ni, r0);
-    gq.load(a.q, j0, a.nj, r0);
-    for (long long r = r0; r < r1; r += BK) {
-        if (LP::reaches_end(a.p, i0, r, r1)) gp.fix(a.p, i0, a.ni, r, r1);
-        if (LQ::reaches_end(a.q, j0, r, r1)) gq.fix(a.q, j0, a.nj, r, r1);
+    gp.init(a.p, i0, a.ni, r0, r1);
+    gq.init(a.q, j0, a.nj, r0, r1);
+    const int steps = (int)((r1 - r0 + BK - 1) / BK);
+    gp.load(a.p, i0, a.ni, r0, 0);
+    gq.load(a.q, j0, a.nj, r0, 0);
+    for (int step = 0; step < steps; ++step) {
+        if (step >= gp.inside) gp.fix(a.p, i0, a.ni, r0 + (long long)step * BK, r1);
+        if (step >= gq.inside) gq.fix(a.q, j0, a.nj, r0 + (long long)step * BK, r1);
         gp.store(a.p, lp, nullptr);
         gq.store(a.q, lq, want_sums ? sums : nullptr);
         __syncthreads();
-        if (r + BK < r1) {
-            gp.load(a.p, i0, a.ni, r + BK);
-            gq.load(a.q, j0, a.nj, r + BK);
+        if (step + 1 < steps) {
+            gp.load(a.p, i0, a.ni, r0 + (long long)(step + 1) * BK, step + 1);
+            gq.load(a.q, j0, a.nj, r0 + (long long)(step + 1) * BK, step + 1);
         }
 #pragma unroll
         for (int kk = 0; kk < BK / 32; ++kk) {
