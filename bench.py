@@ -106,7 +106,7 @@ def source_hash():
     import hashlib
     h = hashlib.sha256()
     csrc = os.path.join(ROOT, "multiagent-particle-envs_amd", "csrc")
-    files = sorted(os.path.join(csrc, f) for f in os.listdir(csrc) if f.endswith((".hip", ".hpp")))
+    files = sorted(os.path.join(csrc, f) for f in os.listdir(csrc) if f.endswith((".hip", ".hpp", ".cpp")))
     for fn in files + [os.path.join(ROOT, "include", "mpe_hip.h")]:
         h.update(os.path.basename(fn).encode() + b"\0")
         h.update(open(fn, "rb").read())
