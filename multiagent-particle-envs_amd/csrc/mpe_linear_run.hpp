@@ -1,6 +1,6 @@
 // The launches of a layer's two passes for one element type (mpe_linear_<type>.hip instantiate it).
 #pragma once
-#include "mpe_linear_impl.hpp"
+#include "mpe_linear_skinny.hpp"
 
 namespace mpe {
 
@@ -121,6 +121,10 @@ struct LinearRun {
         g.ni = a.n; g.nj = a.m; g.nr = a.k;
         g.out = (T*)a.y; g.ldo = a.ldy;
         g.bias = (const T*)a.bias; g.residual = (const T*)a.residual; g.ldr = a.ldr; g.pre = a.pre; g.act = a.act;
+        // Up to two small workgroups a CU: their waves share the sum, where a tile's steps would follow one another (4 x 1024
+        // -> 4096 bf16: 3.9 us against 14.1 in tiles; 2048 x 64 -> 64 f32 3.7 against 7.0; with 512 workgroups 1024 x 258 ->
+        // 512 f32 10.4 against 13.6, 512 x 1024 -> 1024 bf16 12.6 against 11.4; with 1024 of them 10.9 against 7.6).
+        if ((a.m <= 16 || tiles_of(a.m, 64) * tiles_of(a.n, 16) <= 512) && g.p.extent >= 8 && g.q.extent >= 8) return launch_forward_skinny<T>(g, st);
         return launch_rows<T, EPI_FORWARD, R_INNER, R_INNER, false>(g, st);
     }
 
