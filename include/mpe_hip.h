@@ -435,9 +435,10 @@ int mpe_gae(int device, int mode, int64_t n_envs, int32_t n_agents, int32_t n_st
  *   bias      T[n] or NULL
  *   residual  T[m][n], row stride ldr >= n, or 0: one row for all; NULL: none
  *   y         T[m][n], row stride ldy >= n; must not overlap an input, except that y may be the residual itself
- *   pre       float[m][n] contiguous or NULL: x w^T + bias, which the backward pass of every activation other than
- *             MPE_ACT_NONE reads (float32 whatever T is: rounded to 16 bits it would cost the gradients more than any
- *             other step; MPE_ACT_RELU, of which only the sign matters, keeps T[m][n])
+ *   pre       [m][n] contiguous or NULL: what the backward pass of every activation other than MPE_ACT_NONE reads, in a
+ *             form that the element type and the activation settle: MPE_ACT_RELU x w^T + bias in T (only the sign
+ *             matters); else with MPE_BF16 2^14 times the slope f'(x w^T + bias) in float16, and with MPE_F32 and MPE_F16
+ *             x w^T + bias in float32 (rounded to 16 bits it would cost the gradients more than any other step)
  * Products are summed in float32; one rounding to T at the end.  m may be 0; n, k and the row strides of x, w and dy
  * reach at most 2^22.
  * mpe_linear_workspace gives the bytes the two passes need (0 may come back: workspace may then be NULL).
@@ -457,7 +458,7 @@ int mpe_linear_forward(int device, int dtype, int activation, int64_t m, int64_t
  *   dz = dy f'(pre),  dx = dz w  T[m][k] (row stride lddx),  dw = dz^T x  T[n][k],  db = column sums of dz  T[n]
  * The residual's gradient is dy itself.  dx, dw, db: NULL for what is not wanted.  `pre` is what the forward wrote
  * (for MPE_ACT_RELU any T[m][n] with the same signs will do, e.g. y where there was no residual; with
- * MPE_ACT_TANH_OUT, which only this pass knows, it is float32 tanh(x w^T + bias)); NULL with MPE_ACT_NONE.
+ * MPE_ACT_TANH_OUT, which only this pass knows and only for MPE_F32, it is tanh(x w^T + bias)); NULL with MPE_ACT_NONE.
  * dz is rounded to T where the products are 16-bit.
  * The outputs must not overlap each other or an input.  Sums do not change their order from run to run.
  */

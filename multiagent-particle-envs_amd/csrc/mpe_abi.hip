@@ -656,8 +656,8 @@ static bool overlap(const void* a, int64_t na, const void* b, int64_t nb) {
 // bytes from the first to behind the last element of a [rows][cols] matrix
 static int64_t extent(int64_t rows, int64_t cols, int64_t ld, int64_t size) { return rows > 0 ? ((rows - 1) * ld + cols) * size : 0; }
 
-// what the forward pass saves: float32 pre-activations; of relu only the sign is read and the element type will do
-static int64_t pre_bytes(int dtype, int activation) { return activation == MPE_ACT_RELU ? dtype_bytes(dtype) : 4; }
+// an element of what the forward pass keeps
+static int64_t pre_bytes(int dtype, int activation) { return activation == MPE_ACT_RELU ? dtype_bytes(dtype) : dtype == MPE_BF16 ? 2 : 4; }
 
 static bool bad_stride(int64_t rows, int64_t ld, int64_t cols, bool broadcast) {
     if (broadcast && ld == 0) return false;
@@ -708,6 +708,7 @@ int mpe_linear_backward(int device, int dtype, int activation, int64_t m, int64_
     int rc = check_learn("mpe_linear_backward", dtype, m, n, k);
     if (rc != MPE_OK) return rc;
     if (activation < MPE_ACT_NONE || activation > MPE_ACT_TANH_OUT) return fail(nullptr, MPE_ERR_INVALID, "mpe_linear_backward: unknown activation %d", activation);
+    if (activation == MPE_ACT_TANH_OUT && dtype != MPE_F32) return fail(nullptr, MPE_ERR_INVALID, "mpe_linear_backward: MPE_ACT_TANH_OUT is for MPE_F32");
     if (!dx && !dw && !db) return MPE_OK;
     if (m > 0 && (!dy || !x || !w || (activation != MPE_ACT_NONE && !pre)))
         return fail(nullptr, MPE_ERR_INVALID, "mpe_linear_backward: dy, x, w and, with an activation, pre must not be NULL");

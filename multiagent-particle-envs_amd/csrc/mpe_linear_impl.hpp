@@ -79,9 +79,28 @@ __device__ inline float act_slope(int act, float z) {
         case MPE_ACT_RELU: return z > 0.0f ? 1.0f : z != z ? z : 0.0f;
         case MPE_ACT_GELU: { const Normal n = normal_of(z); return fmaf(z * 0.39894228040143268f, n.e, n.phi); }
         case MPE_ACT_SILU: { const float s = sigmoid(z); return s * (1.0f + z * (1.0f - s)); }
+        case 16: return z;      // ACT_SLOPE
         default: return 1.0f;
     }
 }
+
+// What the forward pass keeps for the backward pass.  relu: anything with the pre-activation's sign, in the element type.
+// bfloat16: the slope itself, times 2^14, in float16 (eight times as exact as the rounding of dz that follows, and with
+// the factor as exact down to slopes of 4e-9).  Otherwise the float32 pre-activation, rounded to 16 bits it would cost the
+// gradients more than any other step, or float32 tanh's output.
+constexpr int ACT_SLOPE = 16;       // the kept array holds slopes
+constexpr float SLOPE_SCALE = 16384.0f;
+template <typename T> struct Kept { static constexpr bool SLOPE = false; };
+template <> struct Kept<bf16> { static constexpr bool SLOPE = true; };
+template <typename T>
+__device__ __host__ inline int kept_act(int act) { return Kept<T>::SLOPE && act != MPE_ACT_NONE && act != MPE_ACT_RELU ? ACT_SLOPE : act; }
+
+// one kept value in the element type's size
+template <typename T>
+__device__ inline float kept_small(int act, T v) {
+    return act == ACT_SLOPE ? (float)__builtin_bit_cast(f16, v) * (1.0f / SLOPE_SCALE) : (float)v;
+}
+template <> __device__ inline float kept_small<float>(int, float v) { return v; }
 
 // ---- pieces ----
 template <typename T> struct Piece {                // 16-bit types: the element itself
@@ -100,6 +119,32 @@ __device__ inline f32x4 mfma(f16 __attribute__((ext_vector_type(8))) a, f16 __at
     return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
 }
 
+// Eight float32 numbers as three times eight bfloat16 ones, f = h + m + l.  In pairs, so that one instruction rounds two
+// numbers and the pair's halves become float32 again by a shift and a mask.
+typedef bf16 bf16x8 __attribute__((ext_vector_type(8)));
+template <typename F>
+__device__ inline void split3(const F& f, bf16x8& h, bf16x8& m, bf16x8& l) {
+    typedef float f32x2 __attribute__((ext_vector_type(2)));
+    typedef bf16 bf16x2 __attribute__((ext_vector_type(2)));
+    typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
+    u32x4 p[3];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+        f32x2 rest = {f[2 * e], f[2 * e + 1]};
+#pragma unroll
+        for (int c = 0; c < 3; ++c) {
+            p[c][e] = __builtin_bit_cast(unsigned, __builtin_convertvector(rest, bf16x2));
+            if (c < 2) {
+                rest[0] -= __builtin_bit_cast(float, p[c][e] << 16);
+                rest[1] -= __builtin_bit_cast(float, p[c][e] & 0xffff0000u);
+            }
+        }
+    }
+    h = __builtin_bit_cast(bf16x8, p[0]);
+    m = __builtin_bit_cast(bf16x8, p[1]);
+    l = __builtin_bit_cast(bf16x8, p[2]);
+}
+
 // ---- operands ----
 enum { R_INNER, O_INNER };      // which index is contiguous in memory: the summed one, or the output's
 
@@ -109,14 +154,16 @@ struct Operand {
     const T* data;
     long long ld;               // may be 0 with DZ: one row for all
     long long extent;           // elements from the first to behind the last, at least 8
-    const void* pre;            // [rows][ld_pre], float (relu: T), or null: slope 1
+    const void* pre;            // [rows][ld_pre], what the forward pass kept, or null: slope 1
     long long ld_pre, extent_pre;
     int act;
 };
 
+__device__ inline bool small_pre(int act) { return act == MPE_ACT_RELU || act == ACT_SLOPE; }
+
 template <typename T>
 __device__ inline float pre_at(const Operand<T>& o, long long at) {
-    return o.act == MPE_ACT_RELU ? (float)((const T*)o.pre)[at] : ((const float*)o.pre)[at];
+    return small_pre(o.act) ? kept_small<T>(o.act, ((const T*)o.pre)[at]) : ((const float*)o.pre)[at];
 }
 
 // Where a tile's vectors of W elements lie: a uniform base, and offsets from it that fit 32 bits (the host sees to it that
@@ -178,7 +225,7 @@ struct Loader {
         return LAYOUT == R_INNER ? (unsigned)min(row_of(i), left_o - 1) * ld + chunk_of(i) * 8 : (unsigned)(chunk_of(0) * 8 + i) * ld + row_of(0);
     }
     static __device__ inline long long first(long long o0, long long r0, long long ld) { return LAYOUT == R_INNER ? o0 * ld + r0 : r0 * ld + o0; }
-    static __device__ inline unsigned pre_size(const Operand<T>& op) { return op.act == MPE_ACT_RELU ? (unsigned)sizeof(T) : 4u; }
+    static __device__ inline unsigned pre_size(const Operand<T>& op) { return small_pre(op.act) ? (unsigned)sizeof(T) : 4u; }
 
     // steps from r0 on, of `steps`, whose vectors all end inside the matrix
     static __device__ inline int steps_inside(long long extent, long long ld, long long o0, long long r0, int steps) {
@@ -216,14 +263,14 @@ struct Loader {
                 }
                 if (DZ && op.pre) {
                     const char* q = next_pre;
-                    if (op.act == MPE_ACT_RELU) {
+                    if (small_pre(op.act)) {
 #pragma unroll
                         for (int i = 0; i < NV; ++i) {
                             vec t;
                             __builtin_memcpy(&t, q + off_pre[LAYOUT == R_INNER ? i : 0], W * sizeof(T));
                             if (LAYOUT == O_INNER) q += row_bytes_pre;
 #pragma unroll
-                            for (int e = 0; e < W; ++e) z[i][e] = (float)t[e];
+                            for (int e = 0; e < W; ++e) z[i][e] = kept_small<T>(op.act, t[e]);
                         }
                     } else {
 #pragma unroll
@@ -249,14 +296,14 @@ struct Loader {
         for (int i = 0; i < NV; ++i) __builtin_memcpy(&v[i], base + w.at(offset(i, (unsigned)op.ld, left_o)) * (unsigned)sizeof(T), W * sizeof(T));
         if (DZ && op.pre) {
             const Window wp(op.extent_pre, first(o0, r0, op.ld_pre), W);
-            if (op.act == MPE_ACT_RELU) {
+            if (small_pre(op.act)) {
                 const char* bp = (const char*)((const T*)op.pre + wp.base);
 #pragma unroll
                 for (int i = 0; i < NV; ++i) {
                     vec t;
                     __builtin_memcpy(&t, bp + wp.at(offset(i, (unsigned)op.ld_pre, left_o)) * (unsigned)sizeof(T), W * sizeof(T));
 #pragma unroll
-                    for (int e = 0; e < W; ++e) z[i][e] = (float)t[e];
+                    for (int e = 0; e < W; ++e) z[i][e] = kept_small<T>(op.act, t[e]);
                 }
             } else {
                 const char* bp = (const char*)((const float*)op.pre + wp.base);
@@ -317,20 +364,16 @@ struct Loader {
 #pragma unroll
                 for (int e = 0; e < 8; ++e) sums[u] += f[e];
             }
-#pragma unroll
-            for (int e = 0; e < 8; ++e) h[e] = (PT)f[e];
-            *(pt8*)to = h;
-            if (P::N == 3) {
+            if constexpr (P::N == 3) {
                 pt8 m, l;
-#pragma unroll
-                for (int e = 0; e < 8; ++e) {
-                    const float rest = f[e] - (float)h[e];
-                    m[e] = (PT)rest;
-                    l[e] = (PT)(rest - (float)m[e]);
-                }
+                split3(f, h, m, l);
                 *(pt8*)(to + PLANE) = m;
                 *(pt8*)(to + 2 * PLANE) = l;
+            } else {
+#pragma unroll
+                for (int e = 0; e < 8; ++e) h[e] = (PT)f[e];
             }
+            *(pt8*)to = h;
         }
     }
 };
@@ -406,6 +449,11 @@ __device__ inline void finish(const ProductArgs<T>& a, unsigned split, long long
 #pragma unroll
                 for (int e = 0; e < N; ++e) o[e] = (T)f[e];
                 put<T, N>((T*)a.pre + j * a.ni + i, o, mask);
+            } else if (Kept<T>::SLOPE) {
+                f16 z[N];
+#pragma unroll
+                for (int e = 0; e < N; ++e) z[e] = (f16)(act_slope(a.act, f[e]) * SLOPE_SCALE);
+                put<f16, N>((f16*)a.pre + j * a.ni + i, z, mask);
             } else {
                 put<float, N>((float*)a.pre + j * a.ni + i, f, mask);
             }
@@ -454,7 +502,7 @@ __device__ inline unsigned xcd_run(unsigned b, unsigned n) {
 }
 
 template <typename T, int EPI, int PL, int QL, bool DZ, int BI, int BJ, int WI, int WJ>
-__global__ __launch_bounds__(256, BI * BJ > 8192 ? 2 : BI * BJ > 4096 ? 3 : 4) void product(const ProductArgs<T> a) {
+__global__ __launch_bounds__(256, BI * BJ > 8192 ? (Piece<T>::N == 1 && EPI == EPI_PARTIAL ? 3 : 2) : BI * BJ > 4096 ? 3 : 4) void product(const ProductArgs<T> a) {
     typedef Piece<T> P;
     typedef typename P::type PT;
     typedef PT pt8 __attribute__((ext_vector_type(8)));
@@ -501,6 +549,8 @@ __global__ __launch_bounds__(256, BI * BJ > 8192 ? 2 : BI * BJ > 4096 ? 3 : 4) v
             gp.load(a.p, i0, a.ni, r0 + (long long)(step + 1) * BK, step + 1);
             gq.load(a.q, j0, a.nj, r0 + (long long)(step + 1) * BK, step + 1);
         }
+        // float32's steps alternate between splitting and multiplying: who multiplies goes first (65536 x 1024 -> 1024: 749 -> 699 us)
+        if (NP == 3) __builtin_amdgcn_s_setprio(1);
 #pragma unroll
         for (int kk = 0; kk < BK / 32; ++kk) {
             pt8 fp[FI][NP];
@@ -530,6 +580,7 @@ __global__ __launch_bounds__(256, BI * BJ > 8192 ? 2 : BI * BJ > 4096 ? 3 : 4) v
                 for (int x = 0; x < FI; ++x) acc[x][y] = mfma(fp[x][0], fq[0], acc[x][y]);
             }
         }
+        if (NP == 3) __builtin_amdgcn_s_setprio(0);
         __syncthreads();
     }
 

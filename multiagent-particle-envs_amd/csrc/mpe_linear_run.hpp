@@ -1,6 +1,9 @@
 // The launches of a layer's two passes for one element type (mpe_linear_<type>.hip instantiate it).
 #pragma once
+#include <algorithm>
+
 #include "mpe_linear_skinny.hpp"
+#include "mpe_linear_wide.hpp"
 
 namespace mpe {
 
@@ -10,8 +13,51 @@ __global__ __launch_bounds__(256) void slope_pass(long long m, long long n, cons
                                                   int act, T* __restrict__ dz) {
     for (long long at = (long long)blockIdx.x * 256 + threadIdx.x; at < m * n; at += (long long)gridDim.x * 256) {
         const long long j = at / n, i = at - j * n;
-        const float z = act == MPE_ACT_RELU ? (float)((const T*)pre)[at] : ((const float*)pre)[at];
+        const float z = small_pre(act) ? kept_small<T>(act, ((const T*)pre)[at]) : ((const float*)pre)[at];
         dz[at] = (T)((float)dy[j * lddy + i] * act_slope(act, z));
+    }
+}
+
+// The same for rows of whole 16-byte vectors, with the column sums of dz as it is rounded: a workgroup takes 256 columns of
+// `rows` rows and leaves sums[blockIdx.y][n].  Without pre (no activation) dz is dy and only the sums are made.
+template <typename T>
+__global__ __launch_bounds__(256) void slope_sums(long long m, long long n, const T* __restrict__ dy, long long lddy, const void* __restrict__ pre,
+                                                  int act, T* __restrict__ dz, int rows, float* __restrict__ sums) {
+    constexpr int E = 8;
+    __shared__ float part[8][32][E + 1];
+    const int c = threadIdx.x & 31, g = threadIdx.x >> 5;
+    const long long i = ((long long)blockIdx.x * 32 + c) * E, j1 = min((long long)(blockIdx.y + 1) * rows, m);
+    float s[E] = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
+    if (i < n)
+#pragma unroll 4
+        for (long long j = (long long)blockIdx.y * rows + g; j < j1; j += 8) {
+            T d[E];
+            __builtin_memcpy(d, dy + j * lddy + i, sizeof(d));
+            if (pre) {
+                float z[E];
+                if (small_pre(act)) {
+                    T t[E];
+                    __builtin_memcpy(t, (const T*)pre + j * n + i, sizeof(t));
+#pragma unroll
+                    for (int e = 0; e < E; ++e) z[e] = kept_small<T>(act, t[e]);
+                } else {
+                    __builtin_memcpy(z, (const float*)pre + j * n + i, sizeof(z));
+                }
+#pragma unroll
+                for (int e = 0; e < E; ++e) d[e] = (T)((float)d[e] * act_slope(act, z[e]));
+                __builtin_memcpy(dz + j * n + i, d, sizeof(d));
+            }
+#pragma unroll
+            for (int e = 0; e < E; ++e) s[e] += (float)d[e];
+        }
+#pragma unroll
+    for (int e = 0; e < E; ++e) part[g][c][e] = s[e];
+    __syncthreads();
+    const int col = threadIdx.x;
+    if (sums && (long long)blockIdx.x * 256 + col < n) {
+        float t = 0.0f;
+        for (int k = 0; k < 8; ++k) t += part[k][col / E][col % E];
+        sums[blockIdx.y * n + (long long)blockIdx.x * 256 + col] = t;
     }
 }
 
@@ -53,6 +99,9 @@ inline hipError_t launch_add_splits(const float* partial, int splits, long long 
     return hipGetLastError();
 }
 
+#ifndef WIDE_TILES
+#define WIDE_TILES 256
+#endif
 inline long long tiles_of(long long n, int b) { return (n + b - 1) / b; }
 
 template <typename T, int EPI, int PL, int QL, bool DZ, int BI, int BJ, int WI, int WJ>
@@ -73,20 +122,38 @@ inline hipError_t launch_product(ProductArgs<T> a, int splits, hipStream_t st) {
 // Tiles of the products that write rows of m: by the output's width.
 template <typename T, int EPI, int PL, int QL, bool DZ>
 inline hipError_t launch_rows(const ProductArgs<T>& a, hipStream_t st) {
+    if constexpr (sizeof(T) == 2 && !DZ) {
+        if (a.nr >= 64 && tiles_of(a.ni, Wide::BI) * tiles_of(a.nj, Wide::BJ) >= WIDE_TILES && a.ni > 64 && wide_operand(a.p, PL, a.ni) && wide_operand(a.q, QL, a.nj))
+            return launch_product_wide<T, EPI, PL, QL>(a, 1, st);
+    }
     if (a.ni <= 16) return launch_product<T, EPI, PL, QL, DZ, 16, 128, 1, 4>(a, 1, st);
     if (tiles_of(a.ni, 128) * tiles_of(a.nj, 128) < 256) return launch_product<T, EPI, PL, QL, DZ, 64, 64, 2, 2>(a, 1, st);
     if (a.ni <= 64) return launch_product<T, EPI, PL, QL, DZ, 64, 128, 2, 2>(a, 1, st);
     return launch_product<T, EPI, PL, QL, DZ, 128, 128, 2, 2>(a, 1, st);
 }
 
+#ifndef WIDE_WGS
+#define WIDE_WGS 512
+#endif
 // Weight gradients: the sum over m is long and the output small, so it is split over workgroups that leave float32 partial
 // sums.  One rule for the launch and the workspace.
 struct WeightPlan {
+    bool wide;              // product_wide, the column sums by slope_sums
     int bi, bj, splits;
     long long r_split;
 };
-inline WeightPlan weight_plan(int bk, long long m, long long n, long long k) {
+inline WeightPlan weight_plan(int bk, bool wide, long long m, long long n, long long k) {
     WeightPlan p;
+    p.wide = wide;
+    if (wide) {
+        const long long tiles = tiles_of(k, Wide::BI) * tiles_of(n, Wide::BJ);
+        long long s = WIDE_WGS / tiles;        // two workgroups a CU
+        if (s > tiles_of(m, 512)) s = tiles_of(m, 512);
+        if (s < 1) s = 1;
+        p.r_split = tiles_of(tiles_of(m, s), Wide::BK) * Wide::BK;
+        p.splits = (int)tiles_of(m, p.r_split);
+        return p;
+    }
     p.bi = k <= 16 ? 16 : n <= 16 || k <= 64 || n <= 64 ? 64 : 128;
     p.bj = p.bi == 128 ? 128 : p.bi == 64 && n <= 16 ? 16 : 64;
     const long long tiles = tiles_of(k, p.bi) * tiles_of(n, p.bj);
@@ -101,6 +168,12 @@ inline WeightPlan weight_plan(int bk, long long m, long long n, long long k) {
     return p;
 }
 
+// Large weight gradients of 16-bit types, if the operands' addresses allow it too (wide_operand).
+inline bool wide_weights(int size, long long m, long long n, long long k) {
+    return size == 2 && k >= 256 && n >= 128 && k % 8 == 0 && n % 8 == 0 && m >= 4096;
+}
+constexpr int SUM_ROWS = 512;       // rows a workgroup of slope_sums takes
+
 // dz becomes an array of its own where it would otherwise be recomputed for more than one tile of k, twice
 inline bool own_dz(int act, long long k) { return act != MPE_ACT_NONE && k > 128; }
 
@@ -110,8 +183,13 @@ template <typename T>
 struct LinearRun {
     static long long backward_workspace(int act, long long m, long long n, long long k) {
         if (m == 0) return 0;
-        const WeightPlan p = weight_plan(Piece<T>::BK, m, n, k);
-        return (own_dz(act, k) ? round_up(m * n * (long long)sizeof(T)) : 0) + p.splits * (n * k + n) * 4;
+        const WeightPlan p = weight_plan(Piece<T>::BK, false, m, n, k);
+        long long sums = p.splits * (n * k + n);
+        if (wide_weights(sizeof(T), m, n, k)) {
+            const WeightPlan w = weight_plan(Piece<T>::BK, true, m, n, k);
+            sums = std::max(sums, w.splits * n * k + tiles_of(m, SUM_ROWS) * n);
+        }
+        return (own_dz(act, k) ? round_up(m * n * (long long)sizeof(T)) : 0) + sums * 4;
     }
 
     static hipError_t forward(const LinearArgs& a, hipStream_t st) {
@@ -141,17 +219,27 @@ struct LinearRun {
         if (a.m == 0) {         // no rows: the gradients are empty sums
             return launch_add_splits<T>(nullptr, 0, a.n * a.k + a.n, a.n * a.k, (T*)a.dw, (T*)a.db, st);
         }
-        char* ws = (char*)a.ws;
-        Operand<T> dz = {(const T*)a.dy, a.lddy, (a.m - 1) * a.lddy + a.n, a.act != MPE_ACT_NONE ? a.pre : nullptr, a.n, a.m * a.n, a.act};
+        const int act = kept_act<T>(a.act);
+        Operand<T> dz = {(const T*)a.dy, a.lddy, (a.m - 1) * a.lddy + a.n, a.act != MPE_ACT_NONE ? a.pre : nullptr, a.n, a.m * a.n, act};
+        const Operand<T> x = {(const T*)a.x, a.ldx, (a.m - 1) * a.ldx + a.k, nullptr, 0, 0, 0};
         const bool own = own_dz(a.act, a.k);
-        if (own) {
-            const long long want = (a.m * a.n + 255) / 256;
-            hipLaunchKernelGGL((slope_pass<T>), dim3((unsigned)(want < 8192 ? want : 8192)), dim3(256), 0, st, a.m, a.n, (const T*)a.dy, a.lddy, (const void*)a.pre, a.act, (T*)ws);
+        const bool wide = a.dw && wide_weights(sizeof(T), a.m, a.n, a.k) && wide_operand(x, O_INNER, a.k) && (own || wide_operand(dz, O_INNER, a.n));
+        char* const ws = (char*)a.ws;
+        float* const partial = (float*)(ws + (own ? round_up(a.m * a.n * (long long)sizeof(T)) : 0));
+        const WeightPlan p = weight_plan(Piece<T>::BK, wide, a.m, a.n, a.k);
+        const int strips = (int)tiles_of(a.m, SUM_ROWS);
+        float* const sums = wide && a.db ? partial + p.splits * a.n * a.k : nullptr;
+        if ((own && a.n % 8 == 0) || sums) {
+            hipLaunchKernelGGL((slope_sums<T>), dim3((unsigned)tiles_of(a.n, 256), (unsigned)strips), dim3(256), 0, st, a.m, a.n, (const T*)a.dy, a.lddy,
+                               own ? (const void*)a.pre : nullptr, act, (T*)ws, SUM_ROWS, sums);
             e = hipGetLastError();
-            if (e != hipSuccess) return e;
-            dz = {(const T*)ws, a.n, a.m * a.n, nullptr, 0, 0, MPE_ACT_NONE};
-            ws += round_up(a.m * a.n * (long long)sizeof(T));
+        } else if (own) {
+            const long long want = (a.m * a.n + 255) / 256;
+            hipLaunchKernelGGL((slope_pass<T>), dim3((unsigned)(want < 8192 ? want : 8192)), dim3(256), 0, st, a.m, a.n, (const T*)a.dy, a.lddy, (const void*)a.pre, act, (T*)ws);
+            e = hipGetLastError();
         }
+        if (e != hipSuccess) return e;
+        if (own) dz = {(const T*)ws, a.n, a.m * a.n, nullptr, 0, 0, MPE_ACT_NONE};
         if (a.dx) {
             ProductArgs<T> g = {};
             g.p = {(const T*)a.w, a.ldw, (a.n - 1) * a.ldw + a.k, nullptr, 0, 0, 0};
@@ -162,12 +250,20 @@ struct LinearRun {
             if (e != hipSuccess) return e;
         }
         if (a.dw || a.db) {
-            const WeightPlan p = weight_plan(Piece<T>::BK, a.m, a.n, a.k);
             ProductArgs<T> g = {};
-            g.p = {(const T*)a.x, a.ldx, (a.m - 1) * a.ldx + a.k, nullptr, 0, 0, 0};
+            g.p = x;
             g.q = dz;
             g.ni = a.k; g.nj = a.n; g.nr = a.m; g.r_split = p.r_split;
-            g.partial = (float*)ws;
+            g.partial = partial;
+            if (wide) {
+                if constexpr (sizeof(T) == 2) {
+                    g.partial_ld = a.n * a.k;
+                    e = launch_product_wide<T, EPI_PARTIAL, O_INNER, O_INNER>(g, p.splits, st);
+                    if (e == hipSuccess) e = launch_add_splits<T>(partial, p.splits, g.partial_ld, a.n * a.k, (T*)a.dw, nullptr, st);
+                    if (e == hipSuccess && sums) e = launch_add_splits<T>(sums, strips, a.n, 0, nullptr, (T*)a.db, st);
+                }
+                return e;
+            }
             g.partial_ld = a.n * a.k + a.n;
             g.with_sums = a.db != nullptr;
             e = dz.pre ? weights<true>(g, p, st) : weights<false>(g, p, st);

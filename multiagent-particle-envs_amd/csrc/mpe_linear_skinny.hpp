@@ -13,15 +13,11 @@ template <typename T> struct Frag {
     pt8 c[N];
     template <typename V>
     __device__ inline void set(const V& f) {
+        if constexpr (N == 3) {
+            split3(f, c[0], c[1], c[2]);
+        } else {
 #pragma unroll
-        for (int e = 0; e < 8; ++e) c[0][e] = (PT)f[e];
-        if (N == 3) {
-#pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                const float rest = (float)f[e] - (float)c[0][e];
-                c[N / 2][e] = (PT)rest;
-                c[N - 1][e] = (PT)(rest - (float)c[N / 2][e]);
-            }
+            for (int e = 0; e < 8; ++e) c[0][e] = (PT)f[e];
         }
     }
 };

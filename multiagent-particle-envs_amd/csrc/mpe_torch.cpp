@@ -113,7 +113,7 @@ Tensor linear_forward(const Tensor& x, const Tensor& w, const Tensor& b, const T
     auto shape = x.sizes().vec();
     shape.back() = n;
     Tensor y = at::empty(shape, x.options());
-    if (keep) *pre = at::empty({m, n}, act == MPE_ACT_RELU ? x.options() : x.options().dtype(at::kFloat));
+    if (keep) *pre = at::empty({m, n}, act == MPE_ACT_RELU ? x.options() : x.options().dtype(code == MPE_BF16 ? at::kHalf : at::kFloat));
     int64_t need = 0;
     check(api.linear_workspace(code, act, m, n, k, &need, nullptr));
     const Tensor ws = bytes_like(need, x);

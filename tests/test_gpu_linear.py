@@ -4,8 +4,9 @@ The bounds are the arithmetic's worst case, written down before any run.  u = ha
 fp32 2^-24), v = 2^-24.  A sum of K products in 32 bits is off by at most (K + 8) v sum |x||w| whatever its order (a float32
 product that is summed from parts in 16 bits included: what the parts drop stays below 4 v |x||w|), an activation of slope at
 most 1.13 carries that on and adds a few v of its own value, and the result is rounded once: u |y|.  The backward pass reads
-pre-activations rounded to the type (u |z|, and the slopes change by at most 0.9 a unit of z), rounds dz once (u |dz|) and
-sums like the forward; smallest numbers add one underflow step."""
+pre-activations rounded to the type at worst (u |z|, and the slopes change by at most 0.9 a unit of z), rounds dz once (u |dz|)
+and sums like the forward; smallest numbers add one underflow step.  bfloat16 keeps the slopes themselves in float16, which is
+2^-11 |dz| more where z is small and the bound by u |z| does not cover it."""
 import math
 
 import pytest
@@ -96,7 +97,7 @@ def check_backward(x, w, b, r, dy, act, need_x=True):
     sl, d = slope64(z, act), dy.double()
     dz = d * sl
     zoff = 0.0 if act in ("none", "relu") else 0.9 * (U[dt] * z.abs() + (k + 8) * V * size)
-    e = d.abs() * (zoff + 16 * V * (1 + z.abs())) * (act != "none") + U[dt] * dz.abs() * (1 + U[dt]) + TINY[dt]
+    e = d.abs() * (zoff + 16 * V * (1 + z.abs())) * (act != "none") + (U[dt] + (2.0 ** -11 if dt == torch.bfloat16 else 0)) * dz.abs() * (1 + U[dt]) + TINY[dt]
     xd, wd = x.double(), w.double()
     it = iter(grads)
     if need_x:
@@ -179,6 +180,17 @@ def test_matrices_that_end_where_memory_ends(dt, n):
             one, two = (mpe_hip.linear(q[0], q[1], q[2], activation=act, residual=q[3]) for q in (a, f))
             assert torch.equal(one, two)
             assert all(torch.equal(p, q) for p, q in zip(torch.autograd.grad(one, a, dy), torch.autograd.grad(two, f, framed(dy))))
+
+
+@pytest.mark.parametrize("dt", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("m,k,n,ld", [(8192, 256, 1024, 256), (8200, 320, 1032, 320), (16421, 258, 512, 258), (70001, 72, 136, 74), (4097, 512, 264, 514),
+                                      (5000, 1000, 1304, 1001)])
+def test_large_products(m, k, n, ld, dt):
+    """The sizes that take the copies to LDS, whole and ragged in every direction, and one whose odd row stride keeps them out."""
+    x, w, b, r, dy = make(m, k, n, dt, residual=True, ld=ld)
+    check_forward(x, w, b, r, "gelu")
+    check_backward(x, w, b, r, dy, "silu")
+    check_backward(x, w, b, None, dy, "none")
 
 
 @pytest.mark.parametrize("dt", DTYPES)

@@ -39,7 +39,7 @@ def test_linear_forward_refuses(kw, text):
 
 
 @pytest.mark.parametrize("kw, text", [
-    (dict(dtype=1), "dtype"), (dict(act=7), "activation"), (dict(dy=None), "NULL"), (dict(pre=None), "NULL"), (dict(lddy=3), "stride"), (dict(lddx=2), "stride"),
+    (dict(dtype=1), "dtype"), (dict(act=7), "activation"), (dict(act=5, dtype=2), "TANH_OUT"), (dict(dy=None), "NULL"), (dict(pre=None), "NULL"), (dict(lddy=3), "stride"), (dict(lddx=2), "stride"),
     (dict(dx=2 * A), "overlap"), (dict(dw=5 * A + 8), "overlap"), (dict(db=1 * A + 124), "overlap"), (dict(dw=6 * A + 1), "aligned"), (dict(pre=4 * A + 2), "aligned"),
     (dict(m=1 << 20, ws=None, ldx=3), "workspace"), (dict(m=1 << 12, ws=8 * A + 8), "workspace"), (dict(m=1 << 12, wsb=0), "workspace")])
 def test_linear_backward_refuses(kw, text):
