@@ -84,6 +84,63 @@ __device__ inline float act_slope(int act, float z) {
     }
 }
 
+// The value, and the slope too: they share what is dear.  Four elements share the question which activation it is.
+template <int N>
+__device__ inline void act_both(int act, float* z, float* slope) {
+    switch (act) {
+        case MPE_ACT_TANH:
+#pragma unroll
+            for (int e = 0; e < N; ++e) {
+                z[e] = tanh_of(z[e]);
+                slope[e] = fmaf(-z[e], z[e], 1.0f);
+            }
+            break;
+        case MPE_ACT_GELU:
+#pragma unroll
+            for (int e = 0; e < N; ++e) {
+                const Normal n = normal_of(z[e]);
+                slope[e] = fmaf(z[e] * 0.39894228040143268f, n.e, n.phi);
+                z[e] *= n.phi;
+            }
+            break;
+        case MPE_ACT_SILU:
+#pragma unroll
+            for (int e = 0; e < N; ++e) {
+                const float s = sigmoid(z[e]), v = z[e] * s;
+                slope[e] = fmaf(v, 1.0f - s, s);
+                z[e] = v;
+            }
+            break;
+        default:
+#pragma unroll
+            for (int e = 0; e < N; ++e) {
+                slope[e] = act_slope(act, z[e]);
+                z[e] = act_value(act, z[e]);
+            }
+    }
+}
+template <int N>
+__device__ inline void act_values(int act, float* z) {
+    switch (act) {
+        case MPE_ACT_NONE: break;
+        case MPE_ACT_TANH:
+#pragma unroll
+            for (int e = 0; e < N; ++e) z[e] = tanh_of(z[e]);
+            break;
+        case MPE_ACT_RELU:
+#pragma unroll
+            for (int e = 0; e < N; ++e) z[e] = act_value(MPE_ACT_RELU, z[e]);
+            break;
+        case MPE_ACT_GELU:
+#pragma unroll
+            for (int e = 0; e < N; ++e) z[e] *= normal_of(z[e]).phi;
+            break;
+        default:
+#pragma unroll
+            for (int e = 0; e < N; ++e) z[e] *= sigmoid(z[e]);
+    }
+}
+
 // What the forward pass keeps for the backward pass.  relu: anything with the pre-activation's sign, in the element type.
 // bfloat16: the slope itself, times 2^14, in float16 (eight times as exact as the rounding of dz that follows, and with
 // the factor as exact down to slopes of 4e-9).  Otherwise the float32 pre-activation, rounded to 16 bits it would cost the
@@ -411,19 +468,39 @@ struct ProductArgs {
     int with_sums;
 };
 
-// Finishes N consecutive elements of row j: those whose bit is set in mask.
-template <typename U, int N>
-__device__ inline void put(U* to, const U* v, unsigned mask) {
-    if (mask == (1u << N) - 1) __builtin_memcpy(to, v, N * sizeof(U));
-    else {
+// N consecutive elements as one register value: arrays of 16-bit elements get copied in odd pieces
+template <typename U, int N> struct Run { typedef U type __attribute__((ext_vector_type(N))); };
+template <typename U> struct Run<U, 1> { typedef U type; };
+
+template <typename T, int N>
+__device__ inline void load_residual(const ProductArgs<T>& a, long long i, long long j, unsigned mask, typename Run<T, N>::type& res) {
+    const T* from = a.residual + j * a.ldr + i;
+    if (mask == (1u << N) - 1) __builtin_memcpy(&res, from, N * sizeof(T));
+    else if constexpr (N > 1) {
+#pragma unroll
+        for (int e = 0; e < N; ++e) res[e] = mask >> e & 1 ? from[e] : (T)0.0f;
+    }
+}
+
+template <typename U, int N, typename V>
+__device__ inline void put(U* to, const V& v, unsigned mask) {
+    if (mask == (1u << N) - 1) {
+        typename Run<U, N>::type r;
+        if constexpr (N > 1) {
+#pragma unroll
+            for (int e = 0; e < N; ++e) r[e] = v[e];
+        } else r = v[0];
+        __builtin_memcpy(to, &r, N * sizeof(U));
+    } else {
 #pragma unroll
         for (int e = 0; e < N; ++e)
             if (mask >> e & 1) to[e] = v[e];
     }
 }
 
+// Finishes N consecutive elements of row j: those whose bit is set in mask.
 template <typename T, int EPI, int N, typename F>
-__device__ inline void finish(const ProductArgs<T>& a, unsigned split, long long i, long long j, unsigned mask, const float* bias, const F& sum) {
+__device__ inline void finish(const ProductArgs<T>& a, unsigned split, long long i, long long j, unsigned mask, const float* bias, const typename Run<T, N>::type& res, const F& sum) {
     float f[N];
 #pragma unroll
     for (int e = 0; e < N; ++e) f[e] = sum[e];
@@ -433,41 +510,66 @@ __device__ inline void finish(const ProductArgs<T>& a, unsigned split, long long
     }
     T o[N];
     if (EPI == EPI_FORWARD) {
-        T res[N];
-        if (a.residual) {
-            const T* from = a.residual + j * a.ldr + i;
-            if (mask == (1u << N) - 1) __builtin_memcpy(res, from, sizeof(res));
-            else {
-#pragma unroll
-                for (int e = 0; e < N; ++e) res[e] = mask >> e & 1 ? from[e] : (T)0.0f;
-            }
-        }
 #pragma unroll
         for (int e = 0; e < N; ++e) f[e] += bias[e];
-        if (a.pre) {
-            if (a.act == MPE_ACT_RELU) {
+        if (a.pre && Kept<T>::SLOPE && a.act != MPE_ACT_RELU) {
+            float slope[N];
+            f16 z[N];
+            act_both<N>(a.act, f, slope);
+#pragma unroll
+            for (int e = 0; e < N; ++e) z[e] = (f16)(slope[e] * SLOPE_SCALE);
+            put<f16, N>((f16*)a.pre + j * a.ni + i, z, mask);
+        } else {
+            if (a.pre && a.act == MPE_ACT_RELU) {
 #pragma unroll
                 for (int e = 0; e < N; ++e) o[e] = (T)f[e];
                 put<T, N>((T*)a.pre + j * a.ni + i, o, mask);
-            } else if (Kept<T>::SLOPE) {
-                f16 z[N];
-#pragma unroll
-                for (int e = 0; e < N; ++e) z[e] = (f16)(act_slope(a.act, f[e]) * SLOPE_SCALE);
-                put<f16, N>((f16*)a.pre + j * a.ni + i, z, mask);
-            } else {
+            } else if (a.pre) {
                 put<float, N>((float*)a.pre + j * a.ni + i, f, mask);
             }
+            act_values<N>(a.act, f);
         }
-#pragma unroll
-        for (int e = 0; e < N; ++e) f[e] = act_value(a.act, f[e]);
         if (a.residual) {
+            if constexpr (N == 1) f[0] += (float)res;
+            else
 #pragma unroll
-            for (int e = 0; e < N; ++e) f[e] += (float)res[e];
+                for (int e = 0; e < N; ++e) f[e] += (float)res[e];
         }
     }
 #pragma unroll
     for (int e = 0; e < N; ++e) o[e] = (T)f[e];
     put<T, N>(a.out + j * a.ldo + i, o, mask);
+}
+
+// A thread's share of `rows` rows of results in LDS: N columns of every STEP-th row from jt on.  What the residual holds is
+// asked for two rows ahead: the compiler may not do that, since y may be the residual itself.
+template <typename T, int EPI, int N, int STEP, typename GET>
+__device__ inline void finish_rows(const ProductArgs<T>& a, unsigned split, long long i, long long j0, int jt, int rows, unsigned mask, const float* bias, GET&& get) {
+    constexpr int AHEAD = 2;
+    typename Run<T, N>::type res[AHEAD];
+    const bool with_residual = EPI == EPI_FORWARD && a.residual;
+    const auto ask = [&](int from) {
+#pragma unroll
+        for (int u = 0; u < AHEAD; ++u)
+            if (from + u * STEP < rows) load_residual<T, N>(a, i, j0 + from + u * STEP, mask, res[u]);
+    };
+    if (with_residual) ask(jt);
+#pragma unroll 1
+    for (; jt < rows; jt += AHEAD * STEP) {
+        typename Run<T, N>::type now[AHEAD];
+        if (with_residual) {
+#pragma unroll
+            for (int u = 0; u < AHEAD; ++u) now[u] = res[u];
+            ask(jt + AHEAD * STEP);
+        }
+#pragma unroll
+        for (int u = 0; u < AHEAD; ++u)
+            if (jt + u * STEP < rows) {
+                __attribute__((aligned(16))) float f[N];
+                get(jt + u * STEP, f);
+                finish<T, EPI, N>(a, split, i, j0 + jt + u * STEP, mask, bias, now[u], f);
+            }
+    }
 }
 
 // Operands of fewer than eight elements, for which there is no vector to load: a thread an element of the output, whose sum
@@ -481,7 +583,9 @@ __global__ __launch_bounds__(256) void product_few(const ProductArgs<T> a, int s
         const long long r0 = split * a.r_split, r1 = EPI == EPI_PARTIAL ? min(r0 + a.r_split, a.nr) : a.nr;
         const float bias[1] = {EPI == EPI_FORWARD && a.bias ? (float)a.bias[i] : 0.0f};
         const float f[1] = {plain_sum<T, PL, QL, DZ>(a.p, a.q, i, j, r0, r1)};
-        finish<T, EPI, 1>(a, split, i, j, 1u, bias, f);
+        T res = (T)0.0f;
+        if (EPI == EPI_FORWARD && a.residual) load_residual<T, 1>(a, i, j, 1u, res);
+        finish<T, EPI, 1>(a, split, i, j, 1u, bias, res, f);
         if (EPI == EPI_PARTIAL && a.with_sums && i == 0) {
             float s = 0.0f;
             for (long long r = r0; r < r1; ++r) {
@@ -620,19 +724,15 @@ __global__ __launch_bounds__(256, BI * BJ > 8192 ? (Piece<T>::N == 1 && EPI == E
         }
         __syncthreads();
         const int rows = (int)min((long long)ROWS, a.nj - j0 - half * ROWS);
-        if (have > 0) {
-#pragma unroll 2
-            for (int jt = threadIdx.x / (BI / 4); jt < rows; jt += 1024 / BI) {
-                const long long j = j0 + half * ROWS + jt;
-                f32x4 f = *(const f32x4*)&res[jt * PITCH + it];
+        if (have > 0)
+            finish_rows<T, EPI, 4, 1024 / BI>(a, split, i, j0 + half * ROWS, threadIdx.x / (BI / 4), rows, mask, bias, [&](int jt, float* f) {
+                *(f32x4*)f = *(const f32x4*)&res[jt * PITCH + it];
                 if (NP == 3) {
 #pragma unroll
                     for (int e = 0; e < 4; ++e)
-                        if (!(fabsf(f[e]) < INFINITY) && e < have) f[e] = plain_sum<T, PL, QL, DZ>(a.p, a.q, i + e, j, r0, r1);
+                        if (!(fabsf(f[e]) < INFINITY) && e < have) f[e] = plain_sum<T, PL, QL, DZ>(a.p, a.q, i + e, j0 + half * ROWS + jt, r0, r1);
                 }
-                finish<T, EPI, 4>(a, split, i, j, mask, bias, f);
-            }
-        }
+            });
     }
 }
 

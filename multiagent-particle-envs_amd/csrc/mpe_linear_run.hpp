@@ -8,6 +8,37 @@
 namespace mpe {
 
 // ---- dz = dy f'(pre) as an array of its own ----
+// dense dy: eight elements a thread, whatever the rows' length
+template <typename T>
+__global__ __launch_bounds__(256) void slope_flat(long long total, const T* __restrict__ dy, const void* __restrict__ pre, int act, T* __restrict__ dz) {
+    typedef T vec8 __attribute__((ext_vector_type(8)));
+    typedef float z8 __attribute__((ext_vector_type(8)));
+    for (long long at = ((long long)blockIdx.x * 256 + threadIdx.x) * 8; at < total; at += (long long)gridDim.x * 2048) {
+        if (at + 8 <= total) {
+            vec8 d;
+            z8 z;
+            __builtin_memcpy(&d, dy + at, sizeof(d));
+            if (small_pre(act)) {
+                vec8 t;
+                __builtin_memcpy(&t, (const T*)pre + at, sizeof(t));
+#pragma unroll
+                for (int e = 0; e < 8; ++e) z[e] = kept_small<T>(act, t[e]);
+            } else {
+                __builtin_memcpy(&z, (const float*)pre + at, sizeof(z));
+            }
+#pragma unroll
+            for (int e = 0; e < 8; ++e) d[e] = (T)((float)d[e] * act_slope(act, z[e]));
+            __builtin_memcpy(dz + at, &d, sizeof(d));
+        } else {
+            for (long long k = at; k < total; ++k) {
+                const float z = small_pre(act) ? kept_small<T>(act, ((const T*)pre)[k]) : ((const float*)pre)[k];
+                dz[k] = (T)((float)dy[k] * act_slope(act, z));
+            }
+        }
+    }
+}
+
+// any dy
 template <typename T>
 __global__ __launch_bounds__(256) void slope_pass(long long m, long long n, const T* __restrict__ dy, long long lddy, const void* __restrict__ pre,
                                                   int act, T* __restrict__ dz) {
@@ -99,9 +130,6 @@ inline hipError_t launch_add_splits(const float* partial, int splits, long long 
     return hipGetLastError();
 }
 
-#ifndef WIDE_TILES
-#define WIDE_TILES 256
-#endif
 inline long long tiles_of(long long n, int b) { return (n + b - 1) / b; }
 
 template <typename T, int EPI, int PL, int QL, bool DZ, int BI, int BJ, int WI, int WJ>
@@ -123,7 +151,7 @@ inline hipError_t launch_product(ProductArgs<T> a, int splits, hipStream_t st) {
 template <typename T, int EPI, int PL, int QL, bool DZ>
 inline hipError_t launch_rows(const ProductArgs<T>& a, hipStream_t st) {
     if constexpr (sizeof(T) == 2 && !DZ) {
-        if (a.nr >= 64 && tiles_of(a.ni, Wide::BI) * tiles_of(a.nj, Wide::BJ) >= WIDE_TILES && a.ni > 64 && wide_operand(a.p, PL, a.ni) && wide_operand(a.q, QL, a.nj))
+        if (a.nr >= 64 && tiles_of(a.ni, Wide::BI) * tiles_of(a.nj, Wide::BJ) >= 256 && a.ni > 64 && wide_operand(a.p, PL, a.ni) && wide_operand(a.q, QL, a.nj))
             return launch_product_wide<T, EPI, PL, QL>(a, 1, st);
     }
     if (a.ni <= 16) return launch_product<T, EPI, PL, QL, DZ, 16, 128, 1, 4>(a, 1, st);
@@ -132,9 +160,6 @@ inline hipError_t launch_rows(const ProductArgs<T>& a, hipStream_t st) {
     return launch_product<T, EPI, PL, QL, DZ, 128, 128, 2, 2>(a, 1, st);
 }
 
-#ifndef WIDE_WGS
-#define WIDE_WGS 512
-#endif
 // Weight gradients: the sum over m is long and the output small, so it is split over workgroups that leave float32 partial
 // sums.  One rule for the launch and the workspace.
 struct WeightPlan {
@@ -147,7 +172,7 @@ inline WeightPlan weight_plan(int bk, bool wide, long long m, long long n, long 
     p.wide = wide;
     if (wide) {
         const long long tiles = tiles_of(k, Wide::BI) * tiles_of(n, Wide::BJ);
-        long long s = WIDE_WGS / tiles;        // two workgroups a CU
+        long long s = 512 / tiles;        // two workgroups a CU
         if (s > tiles_of(m, 512)) s = tiles_of(m, 512);
         if (s < 1) s = 1;
         p.r_split = tiles_of(tiles_of(m, s), Wide::BK) * Wide::BK;
@@ -157,9 +182,9 @@ inline WeightPlan weight_plan(int bk, bool wide, long long m, long long n, long 
     p.bi = k <= 16 ? 16 : n <= 16 || k <= 64 || n <= 64 ? 64 : 128;
     p.bj = p.bi == 128 ? 128 : p.bi == 64 && n <= 16 ? 16 : 64;
     const long long tiles = tiles_of(k, p.bi) * tiles_of(n, p.bj);
-    // three workgroups a CU (64/64 over 196 608 rows, product and sum of the splits: 38.3 us at 1024 workgroups, 36.9 at 768,
-    // 41.1 at 512, 57.7 at 256)
-    long long s = 768 / tiles;
+    // four workgroups a CU (64/64 f32 over 196 608 rows, product and sum of the splits: 38.6 us at 1024 workgroups, 41.2 at
+    // 768, 46.0 at 512)
+    long long s = 1024 / tiles;
     const long long most = tiles_of(m, 4 * bk);      // at least four steps each
     if (s > most) s = most;
     if (s < 1) s = 1;
@@ -172,7 +197,7 @@ inline WeightPlan weight_plan(int bk, bool wide, long long m, long long n, long 
 inline bool wide_weights(int size, long long m, long long n, long long k) {
     return size == 2 && k >= 256 && n >= 128 && k % 8 == 0 && n % 8 == 0 && m >= 4096;
 }
-constexpr int SUM_ROWS = 512;       // rows a workgroup of slope_sums takes
+constexpr int SUM_ROWS = 128;       // rows a workgroup of slope_sums takes
 
 // dz becomes an array of its own where it would otherwise be recomputed for more than one tile of k, twice
 inline bool own_dz(int act, long long k) { return act != MPE_ACT_NONE && k > 128; }
@@ -229,9 +254,13 @@ struct LinearRun {
         const WeightPlan p = weight_plan(Piece<T>::BK, wide, a.m, a.n, a.k);
         const int strips = (int)tiles_of(a.m, SUM_ROWS);
         float* const sums = wide && a.db ? partial + p.splits * a.n * a.k : nullptr;
-        if ((own && a.n % 8 == 0) || sums) {
+        if (sums) {
             hipLaunchKernelGGL((slope_sums<T>), dim3((unsigned)tiles_of(a.n, 256), (unsigned)strips), dim3(256), 0, st, a.m, a.n, (const T*)a.dy, a.lddy,
                                own ? (const void*)a.pre : nullptr, act, (T*)ws, SUM_ROWS, sums);
+            e = hipGetLastError();
+        } else if (own && a.lddy == a.n) {
+            const long long want = (a.m * a.n + 2047) / 2048;
+            hipLaunchKernelGGL((slope_flat<T>), dim3((unsigned)(want < 8192 ? want : 8192)), dim3(256), 0, st, a.m * a.n, (const T*)a.dy, (const void*)a.pre, act, (T*)ws);
             e = hipGetLastError();
         } else if (own) {
             const long long want = (a.m * a.n + 255) / 256;

@@ -110,7 +110,9 @@ __global__ __launch_bounds__(512) void forward_skinny(const ProductArgs<T> a) {
 #pragma unroll
         for (int w = 0; w < WAVES; ++w) f[0] += part[w][jt][threadIdx.x & 15];
         if (Frag<T>::N == 3 && !(fabsf(f[0]) < INFINITY)) f[0] = plain_sum<T, R_INNER, R_INNER, false>(a.p, a.q, i, j, 0, a.nr);
-        finish<T, EPI_FORWARD, 1>(a, 0, i, j, 1u, bias, f);
+        T res = (T)0.0f;
+        if (a.residual) load_residual<T, 1>(a, i, j, 1u, res);
+        finish<T, EPI_FORWARD, 1>(a, 0, i, j, 1u, bias, res, f);
     }
 }
 

@@ -58,22 +58,36 @@ struct WideTile {
         next += step;
     }
 
-    // the end of the sum, `left` < 32 of it, element by element, zeros behind it
-    static __device__ inline void copy_end(const Operand<T>& op, long long o0, long long no, long long r0, int left, char* lds) {
-        const int left_o = (int)min(no - o0, (long long)BO);
-#pragma unroll 1
-        for (int slot = threadIdx.x; slot < BO * 4; slot += 256) {
-            const int row = slot / RUN, chunk = swizzle(row, slot % RUN);
-            vec8 v = (T)0.0f;
-            if (LAYOUT == R_INNER) {
-                const T* p = op.data + (o0 + min(row, left_o - 1)) * op.ld + r0 + chunk * 8;
+    // The end of the sum, `left` < 32 of it, through registers: vectors kept inside the matrix by a Window, elements shifted
+    // to their places, zeros behind the end.  All loads first.
+    struct End {
+        vec8 v[COPIES];
+    };
+    static __device__ inline int end_slot(int u) { return threadIdx.x + u * 256; }
+    static __device__ inline unsigned end_off(int u, unsigned ld, int left_o) {
+        const int row = end_slot(u) / RUN, chunk = swizzle(row, end_slot(u) % RUN);
+        return LAYOUT == R_INNER ? (unsigned)min(row, left_o - 1) * ld + chunk * 8 : (unsigned)row * ld + min(chunk * 8, left_o - 8);
+    }
+    static __device__ inline void load_end(End& x, const Operand<T>& op, long long o0, long long no, long long r0) {
+        const Window w(op.extent, LAYOUT == R_INNER ? o0 * op.ld + r0 : r0 * op.ld + o0, 8);
+        const char* base = (const char*)(op.data + w.base);
 #pragma unroll
-                for (int e = 0; e < 8; ++e)
-                    if (chunk * 8 + e < left) v[e] = p[e];
-            } else if (row < left) {
-                __builtin_memcpy(&v, op.data + (r0 + row) * op.ld + o0 + min(chunk * 8, left_o - 8), 16);
+        for (int u = 0; u < COPIES; ++u) __builtin_memcpy(&x.v[u], base + w.at(end_off(u, (unsigned)op.ld, (int)min(no - o0, (long long)BO))) * 2u, 16);
+    }
+    static __device__ inline void store_end(End& x, const Operand<T>& op, long long o0, long long no, long long r0, int left, char* lds) {
+        const Window w(op.extent, LAYOUT == R_INNER ? o0 * op.ld + r0 : r0 * op.ld + o0, 8);
+#pragma unroll
+        for (int u = 0; u < COPIES; ++u) {
+            const int row = end_slot(u) / RUN, chunk = swizzle(row, end_slot(u) % RUN);
+            if (LAYOUT == R_INNER) {
+                const int by = w.moved(end_off(u, (unsigned)op.ld, (int)min(no - o0, (long long)BO)));
+                if (by > 0 && by < 8) shift_down<8>(x.v[u], by);
+#pragma unroll
+                for (int e = 0; e < 8; ++e) x.v[u][e] = chunk * 8 + e < left ? x.v[u][e] : (T)0.0f;
+            } else if (row >= left) {
+                x.v[u] = (T)0.0f;
             }
-            *(vec8*)(lds + slot * 16) = v;
+            *(vec8*)(lds + end_slot(u) * 16) = x.v[u];
         }
     }
 
@@ -136,8 +150,12 @@ __global__ __launch_bounds__(256, 2) void product_wide(const ProductArgs<T> a) {
         q.copy(base + s * STAGE + TP::BYTES, wave);
     }
     if (left) {         // the end of the sum first, in the stage that is still free
-        TP::copy_end(a.p, i0, a.ni, r1 - left, left, lds + 2 * STAGE);
-        TQ::copy_end(a.q, j0, a.nj, r1 - left, left, lds + 2 * STAGE + TP::BYTES);
+        typename TP::End ep;
+        typename TQ::End eq;
+        TP::load_end(ep, a.p, i0, a.ni, r1 - left);
+        TQ::load_end(eq, a.q, j0, a.nj, r1 - left);
+        TP::store_end(ep, a.p, i0, a.ni, r1 - left, left, lds + 2 * STAGE);
+        TQ::store_end(eq, a.q, j0, a.nj, r1 - left, left, lds + 2 * STAGE + TP::BYTES);
         __syncthreads();
         multiply(lds + 2 * STAGE);
     }
@@ -156,13 +174,14 @@ __global__ __launch_bounds__(256, 2) void product_wide(const ProductArgs<T> a) {
         stage = stage == 2 ? 0 : stage + 1;
     }
 
-    const int it = threadIdx.x % (BI / 4) * 4;      // a thread's four columns, the same in every row it takes
+    constexpr int N = EPI == EPI_FORWARD ? 8 : 4;       // a thread's columns
+    const int it = threadIdx.x % (BI / N) * N;          // a thread's columns, the same in every row it takes
     const long long i = i0 + it;
-    const int have = (int)max(0LL, min(4LL, a.ni - i));
+    const int have = (int)max(0LL, min((long long)N, a.ni - i));
     const unsigned mask = (1u << have) - 1;
-    float bias[4];
+    float bias[N];
 #pragma unroll
-    for (int e = 0; e < 4; ++e) bias[e] = EPI == EPI_FORWARD && a.bias && e < have ? (float)a.bias[i + e] : 0.0f;
+    for (int e = 0; e < N; ++e) bias[e] = EPI == EPI_FORWARD && a.bias && e < have ? (float)a.bias[i + e] : 0.0f;
     float* const res = (float*)lds;
 #pragma unroll
     for (int half = 0; half < HALVES; ++half) {
@@ -175,13 +194,11 @@ __global__ __launch_bounds__(256, 2) void product_wide(const ProductArgs<T> a) {
         }
         __syncthreads();
         const int rows = (int)max(0LL, min((long long)ROWS, a.nj - j0 - half * ROWS));
-        if (have > 0) {
-#pragma unroll 2
-            for (int jt = threadIdx.x / (BI / 4); jt < rows; jt += 1024 / BI) {
-                const f32x4 f = *(const f32x4*)&res[jt * PITCH + it];
-                finish<T, EPI, 4>(a, split, i, j0 + half * ROWS + jt, mask, bias, f);
-            }
-        }
+        if (have > 0)
+            finish_rows<T, EPI, N, 256 * N / BI>(a, split, i, j0 + half * ROWS, threadIdx.x / (BI / N), rows, mask, bias, [&](int jt, float* f) {
+#pragma unroll
+                for (int e = 0; e < N; e += 4) *(f32x4*)&f[e] = *(const f32x4*)&res[jt * PITCH + it + e];
+            });
     }
 }
 
