@@ -662,26 +662,24 @@ __global__ __launch_bounds__(256, BI * BJ > 8192 ? (Piece<T>::N == 1 && EPI == E
             for (int x = 0; x < FI; ++x)
 #pragma unroll
                 for (int c = 0; c < NP; ++c) fp[x][c] = *(const pt8*)(lp + c * LP::PLANE + LP::place(wi + x * 16 + (lane & 15), kk * 4 + (lane >> 4)));
+            // a result comes back after several issue slots: four sums at least take turns
+            constexpr int YB = FI >= 4 || FJ == 1 ? 1 : 2;
 #pragma unroll
-            for (int y = 0; y < FJ; ++y) {
-                pt8 fq[NP];
+            for (int y = 0; y < FJ; y += YB) {
+                pt8 fq[YB][NP];
 #pragma unroll
-                for (int c = 0; c < NP; ++c) fq[c] = *(const pt8*)(lq + c * LQ::PLANE + LQ::place(wj + y * 16 + (lane & 15), kk * 4 + (lane >> 4)));
-                if (NP == 3) {
-                    // smallest first
+                for (int b = 0; b < YB; ++b)
 #pragma unroll
-                    for (int x = 0; x < FI; ++x) acc[x][y] = mfma(fp[x][NP - 1], fq[0], acc[x][y]);
+                    for (int c = 0; c < NP; ++c) fq[b][c] = *(const pt8*)(lq + c * LQ::PLANE + LQ::place(wj + (y + b) * 16 + (lane & 15), kk * 4 + (lane >> 4)));
+                // float32: the partial products, smallest first
+                constexpr int PAIRS = NP == 3 ? 6 : 1;
+                constexpr int PC[6] = {NP == 3 ? 2 : 0, 0, NP / 2, NP / 2, 0, 0}, QC[6] = {0, NP - 1, NP / 2, 0, NP / 2, 0};
 #pragma unroll
-                    for (int x = 0; x < FI; ++x) acc[x][y] = mfma(fp[x][0], fq[NP - 1], acc[x][y]);
+                for (int c = 0; c < PAIRS; ++c)
 #pragma unroll
-                    for (int x = 0; x < FI; ++x) acc[x][y] = mfma(fp[x][NP / 2], fq[NP / 2], acc[x][y]);
+                    for (int b = 0; b < YB; ++b)
 #pragma unroll
-                    for (int x = 0; x < FI; ++x) acc[x][y] = mfma(fp[x][NP / 2], fq[0], acc[x][y]);
-#pragma unroll
-                    for (int x = 0; x < FI; ++x) acc[x][y] = mfma(fp[x][0], fq[NP / 2], acc[x][y]);
-                }
-#pragma unroll
-                for (int x = 0; x < FI; ++x) acc[x][y] = mfma(fp[x][0], fq[0], acc[x][y]);
+                        for (int x = 0; x < FI; ++x) acc[x][y + b] = mfma(fp[x][PC[c]], fq[b][QC[c]], acc[x][y + b]);
             }
         }
         if (NP == 3) __builtin_amdgcn_s_setprio(0);

@@ -97,7 +97,7 @@ __global__ __launch_bounds__(256) void slope_sums(long long m, long long n, cons
 template <typename T, int COLS, int GROUPS>
 __global__ __launch_bounds__(COLS * GROUPS) void add_splits(const float* __restrict__ partial, int splits, long long ld, long long n, T* __restrict__ out,
                                                             T* __restrict__ sums) {
-    __shared__ float part[GROUPS][COLS];
+    __shared__ float part[COLS < 64 ? GROUPS * COLS / 64 : GROUPS][COLS];
     const int c = threadIdx.x % COLS, g = threadIdx.x / COLS;
     const long long at = (long long)blockIdx.x * COLS + c;
     const bool here = at < ld && (at < n ? out : sums) != nullptr;
@@ -113,10 +113,16 @@ __global__ __launch_bounds__(COLS * GROUPS) void add_splits(const float* __restr
         }
         for (; k < splits; k += GROUPS) s += partial[k * ld + at];
     }
-    part[g][c] = s;
+    // groups that share a wave first
+    constexpr int SHARE = COLS < 64 ? 64 / COLS : 1;
+#pragma unroll
+    for (int o = COLS; o < 64; o *= 2) s += __shfl_xor(s, o);
+    if (g % SHARE == 0) part[g / SHARE][c] = s;
     __syncthreads();
     if (g == 0 && here) {
-        for (int k = 1; k < GROUPS; ++k) s += part[k][c];
+        s = 0.0f;
+#pragma unroll
+        for (int k = 0; k < GROUPS / SHARE; ++k) s += part[k][c];
         if (at < n) out[at] = (T)s;
         else sums[at - n] = (T)s;
     }

@@ -140,24 +140,33 @@ __device__ inline void write_totals(const double* tot, float value_coef, float e
     *loss = (float)((tot[0] + (double)value_coef * tot[1] - (double)entropy_coef * tot[2]) * inv);
 }
 
-// Sums over the workgroup; a launch of one workgroup is done with that, another leaves partial sums for ppo_finish.
+// Sums over a workgroup, sum i in thread i; all threads have to come here.
+template <int WAVES>
+__device__ inline double group_sums(const double* sum, double (*scratch)[NSTAT]) {
+    for (int i = 0; i < NSTAT; ++i) {
+        const double v = wave_sum(sum[i]);
+        if ((threadIdx.x & 63) == 0) scratch[threadIdx.x >> 6][i] = v;
+    }
+    __syncthreads();
+    double t = 0.0;
+    if (threadIdx.x < NSTAT)
+#pragma unroll
+        for (int w = 0; w < WAVES; ++w) t += scratch[w][threadIdx.x];
+    return t;
+}
+
+// A launch of one workgroup is done with its sums, another leaves partial sums for ppo_finish.
 template <int WAVES>
 __device__ inline void leave_sums(const PpoArgs& p, const double* sum, double (*scratch)[NSTAT]) {
-    double v[NSTAT];
-    for (int i = 0; i < NSTAT; ++i) v[i] = wave_sum(sum[i]);
-    if ((threadIdx.x & 63) == 0)
-        for (int i = 0; i < NSTAT; ++i) scratch[threadIdx.x >> 6][i] = v[i];
-    __syncthreads();
-    if (threadIdx.x == 0) {
-        double tot[NSTAT];
-        for (int i = 0; i < NSTAT; ++i) {
-            tot[i] = 0.0;
-            for (int w = 0; w < WAVES; ++w) tot[i] += scratch[w][i];
-        }
-        if (gridDim.x == 1) write_totals(tot, p.value_coef, p.entropy_coef, p.loss, p.stats);
-        else
-            for (int i = 0; i < NSTAT; ++i) p.ws[blockIdx.x * NSTAT + i] = tot[i];
+    const double t = group_sums<WAVES>(sum, scratch);
+    if (gridDim.x > 1) {
+        if (threadIdx.x < NSTAT) p.ws[blockIdx.x * NSTAT + threadIdx.x] = t;
+        return;
     }
+    __syncthreads();
+    if (threadIdx.x < NSTAT) scratch[0][threadIdx.x] = t;
+    __syncthreads();
+    if (threadIdx.x == 0) write_totals(scratch[0], p.value_coef, p.entropy_coef, p.loss, p.stats);
 }
 
 // Few words: a lane takes a row.  A workgroup's 256 rows are fetched into LDS (consecutive lanes read consecutive elements
@@ -394,17 +403,11 @@ __global__ __launch_bounds__(1024) void ppo_finish(const double* __restrict__ pa
     double tot[NSTAT] = {0, 0, 0, 0, 0, 0};
     for (int b = threadIdx.x; b < n; b += 1024)
         for (int i = 0; i < NSTAT; ++i) tot[i] += partial[b * NSTAT + i];
-    for (int i = 0; i < NSTAT; ++i) tot[i] = wave_sum(tot[i]);
-    if ((threadIdx.x & 63) == 0)
-        for (int i = 0; i < NSTAT; ++i) scratch[threadIdx.x >> 6][i] = tot[i];
+    const double t = group_sums<16>(tot, scratch);
     __syncthreads();
-    if (threadIdx.x == 0) {
-        for (int i = 0; i < NSTAT; ++i) {
-            tot[i] = 0.0;
-            for (int w = 0; w < 16; ++w) tot[i] += scratch[w][i];
-        }
-        write_totals(tot, value_coef, entropy_coef, loss, stats);
-    }
+    if (threadIdx.x < NSTAT) scratch[0][threadIdx.x] = t;
+    __syncthreads();
+    if (threadIdx.x == 0) write_totals(scratch[0], value_coef, entropy_coef, loss, stats);
 }
 
 template <typename T, bool BACK>
