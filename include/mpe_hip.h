@@ -435,8 +435,8 @@ int mpe_gae(int device, int mode, int64_t n_envs, int32_t n_agents, int32_t n_st
  *   bias      T[n] or NULL
  *   residual  T[m][n], row stride ldr >= n, or 0: one row for all; NULL: none
  *   y         T[m][n], row stride ldy >= n; must not overlap an input, except that y may be the residual itself
- *   pre       [m][n] contiguous or NULL: what the backward pass of every activation other than MPE_ACT_NONE reads, in a
- *             form that the element type and the activation settle: MPE_ACT_RELU x w^T + bias in T (only the sign
+ *   pre       [m][n] contiguous or NULL: what the backward pass of every activation other than MPE_ACT_NONE (with which it is
+ *             left as it is) reads, in a form that the element type and the activation settle: MPE_ACT_RELU x w^T + bias in T (only the sign
  *             matters); else with MPE_BF16 2^14 times the slope f'(x w^T + bias) in float16, and with MPE_F32 and MPE_F16
  *             x w^T + bias in float32 (rounded to 16 bits it would cost the gradients more than any other step)
  * Products are summed in float32; one rounding to T at the end.  m may be 0; n, k and the row strides of x, w and dy

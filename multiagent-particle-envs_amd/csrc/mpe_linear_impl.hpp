@@ -41,7 +41,7 @@ __device__ inline float tanh_of(float z) {
     return fabsf(z) < 0.3f ? fmaf(z * q, s, z) : big;
 }
 
-// Phi(z) and e^(-z^2/2).  erfc(x) e^(x^2) = t Q(t) with t = 1 / (1 + 0.33 x) and Q a polynomial fitted to it over x >= 0
+// Phi(z) and e^(-z^2/2).  erfc(x) e^(x^2) / 2 = t Q(t) with t = 1 / (1 + 0.33 x) and Q a polynomial fitted to it over x >= 0
 // (relative error 9.4e-8), so that the far tail keeps its relative precision.
 struct Normal {
     float phi, e;
@@ -50,27 +50,29 @@ __device__ inline Normal normal_of(float z) {
     Normal n;
     n.e = fast_exp(-0.5f * z * z);
     const float t = __builtin_amdgcn_rcpf(fmaf(fabsf(z), 0.33f * 0.70710678118654752f, 1.0f));
-    float q = fmaf(t, -0.1353444f, 0.46023187f);
-    q = fmaf(t, q, -0.351141f);
-    q = fmaf(t, q, 0.40849227f);
-    q = fmaf(t, q, 0.047224592f);
-    q = fmaf(t, q, 0.20122273f);
-    q = fmaf(t, q, 0.18295613f);
-    q = fmaf(t, q, 0.1863578f);
-    const float h = 0.5f * (t * q) * n.e;
+    float q = fmaf(t, -0.0676722f, 0.230115935f);
+    q = fmaf(t, q, -0.1755705f);
+    q = fmaf(t, q, 0.204246135f);
+    q = fmaf(t, q, 0.023612296f);
+    q = fmaf(t, q, 0.100611365f);
+    q = fmaf(t, q, 0.091478065f);
+    q = fmaf(t, q, 0.0931789f);
+    const float h = t * q * n.e;
     n.phi = z < 0.0f ? h : 1.0f - h;
     return n;
 }
 
-__device__ inline float act_value(int act, float z) {
-    switch (act) {
-        case MPE_ACT_TANH: return tanh_of(z);
-        case MPE_ACT_RELU: return z > 0.0f || z != z ? z : 0.0f;
-        case MPE_ACT_GELU: return z * normal_of(z).phi;
-        case MPE_ACT_SILU: return z * sigmoid(z);
-        default: return z;
-    }
+// tanh as exact as a 16-bit type can tell (2e-6 of it): the series' first two terms below 1/16
+__device__ inline float tanh_16(float z) {
+    const float big = fmaf(-2.0f, __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(z * (2.0f * 1.44269504088896341f))), 1.0f);
+    return fabsf(z) < 0.0625f ? fmaf(z * z * z, -1.0f / 3.0f, z) : big;
 }
+template <typename T>
+__device__ inline float tanh_for(float z) { return sizeof(T) == 2 ? tanh_16(z) : tanh_of(z); }
+
+__device__ inline float relu(float z) { return z > 0.0f || z != z ? z : 0.0f; }
+
+constexpr int ACT_SLOPE = 16;       // what was kept are the slopes
 
 __device__ inline float act_slope(int act, float z) {
     switch (act) {
@@ -79,19 +81,19 @@ __device__ inline float act_slope(int act, float z) {
         case MPE_ACT_RELU: return z > 0.0f ? 1.0f : z != z ? z : 0.0f;
         case MPE_ACT_GELU: { const Normal n = normal_of(z); return fmaf(z * 0.39894228040143268f, n.e, n.phi); }
         case MPE_ACT_SILU: { const float s = sigmoid(z); return s * (1.0f + z * (1.0f - s)); }
-        case 16: return z;      // ACT_SLOPE
+        case ACT_SLOPE: return z;
         default: return 1.0f;
     }
 }
 
 // The value, and the slope too: they share what is dear.  Four elements share the question which activation it is.
-template <int N>
+template <typename T, int N>
 __device__ inline void act_both(int act, float* z, float* slope) {
     switch (act) {
         case MPE_ACT_TANH:
 #pragma unroll
             for (int e = 0; e < N; ++e) {
-                z[e] = tanh_of(z[e]);
+                z[e] = tanh_for<T>(z[e]);
                 slope[e] = fmaf(-z[e], z[e], 1.0f);
             }
             break;
@@ -114,22 +116,21 @@ __device__ inline void act_both(int act, float* z, float* slope) {
         default:
 #pragma unroll
             for (int e = 0; e < N; ++e) {
-                slope[e] = act_slope(act, z[e]);
-                z[e] = act_value(act, z[e]);
+                slope[e] = 1.0f;        // no activation; relu keeps a sign
             }
     }
 }
-template <int N>
+template <typename T, int N>
 __device__ inline void act_values(int act, float* z) {
     switch (act) {
         case MPE_ACT_NONE: break;
         case MPE_ACT_TANH:
 #pragma unroll
-            for (int e = 0; e < N; ++e) z[e] = tanh_of(z[e]);
+            for (int e = 0; e < N; ++e) z[e] = tanh_for<T>(z[e]);
             break;
         case MPE_ACT_RELU:
 #pragma unroll
-            for (int e = 0; e < N; ++e) z[e] = act_value(MPE_ACT_RELU, z[e]);
+            for (int e = 0; e < N; ++e) z[e] = relu(z[e]);
             break;
         case MPE_ACT_GELU:
 #pragma unroll
@@ -145,7 +146,6 @@ __device__ inline void act_values(int act, float* z) {
 // bfloat16: the slope itself, times 2^14, in float16 (eight times as exact as the rounding of dz that follows, and with
 // the factor as exact down to slopes of 4e-9).  Otherwise the float32 pre-activation, rounded to 16 bits it would cost the
 // gradients more than any other step, or float32 tanh's output.
-constexpr int ACT_SLOPE = 16;       // the kept array holds slopes
 constexpr float SLOPE_SCALE = 16384.0f;
 template <typename T> struct Kept { static constexpr bool SLOPE = false; };
 template <> struct Kept<bf16> { static constexpr bool SLOPE = true; };
@@ -515,7 +515,7 @@ __device__ inline void finish(const ProductArgs<T>& a, unsigned split, long long
         if (a.pre && Kept<T>::SLOPE && a.act != MPE_ACT_RELU) {
             float slope[N];
             f16 z[N];
-            act_both<N>(a.act, f, slope);
+            act_both<T, N>(a.act, f, slope);
 #pragma unroll
             for (int e = 0; e < N; ++e) z[e] = (f16)(slope[e] * SLOPE_SCALE);
             put<f16, N>((f16*)a.pre + j * a.ni + i, z, mask);
@@ -527,7 +527,7 @@ __device__ inline void finish(const ProductArgs<T>& a, unsigned split, long long
             } else if (a.pre) {
                 put<float, N>((float*)a.pre + j * a.ni + i, f, mask);
             }
-            act_values<N>(a.act, f);
+            act_values<T, N>(a.act, f);
         }
         if (a.residual) {
             if constexpr (N == 1) f[0] += (float)res;

@@ -229,7 +229,7 @@ struct LinearRun {
         g.q = {(const T*)a.x, a.ldx, (a.m - 1) * a.ldx + a.k, nullptr, 0, 0, 0};
         g.ni = a.n; g.nj = a.m; g.nr = a.k;
         g.out = (T*)a.y; g.ldo = a.ldy;
-        g.bias = (const T*)a.bias; g.residual = (const T*)a.residual; g.ldr = a.ldr; g.pre = a.pre; g.act = a.act;
+        g.bias = (const T*)a.bias; g.residual = (const T*)a.residual; g.ldr = a.ldr; g.pre = a.act != MPE_ACT_NONE ? a.pre : nullptr; g.act = a.act;
         // Up to two small workgroups a CU: their waves share the sum, where a tile's steps would follow one another (4 x 1024
         // -> 4096 bf16: 3.9 us against 14.1 in tiles; 2048 x 64 -> 64 f32 3.7 against 7.0; with 512 workgroups 1024 x 258 ->
         // 512 f32 10.4 against 13.6, 512 x 1024 -> 1024 bf16 12.6 against 11.4; with 1024 of them 10.9 against 7.6).

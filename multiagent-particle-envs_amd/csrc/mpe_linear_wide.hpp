@@ -6,6 +6,8 @@
 // An operand whose contiguous index is the output's lies in LDS as it lies in memory, and ds_read_b64_tr_b16 turns it: 16
 // lanes read four rows of 16 elements and each gets one column.
 #pragma once
+#include <type_traits>
+
 #include "mpe_linear_impl.hpp"
 
 namespace mpe {
@@ -15,6 +17,13 @@ struct Wide {
 };
 
 typedef __attribute__((address_space(3))) void lds_void;
+
+// a pointer that is the same in all lanes, in scalar registers
+__device__ inline const char* uniform(const char* p) {
+    const unsigned long long a = (unsigned long long)p;
+    const unsigned lo = __builtin_amdgcn_readfirstlane((unsigned)a), hi = __builtin_amdgcn_readfirstlane((unsigned)(a >> 32));
+    return (const char*)((unsigned long long)hi << 32 | lo);
+}
 
 // 16 bytes a lane from base + off (bytes) to LDS address `to`, lane after lane
 __device__ inline void copy_to_lds(const char* base, unsigned off, unsigned to) {
@@ -58,36 +67,52 @@ struct WideTile {
         next += step;
     }
 
-    // The end of the sum, `left` < 32 of it, through registers: vectors kept inside the matrix by a Window, elements shifted
-    // to their places, zeros behind the end.  All loads first.
-    struct End {
-        vec8 v[COPIES];
-    };
-    static __device__ inline int end_slot(int u) { return threadIdx.x + u * 256; }
-    static __device__ inline unsigned end_off(int u, unsigned ld, int left_o) {
-        const int row = end_slot(u) / RUN, chunk = swizzle(row, end_slot(u) % RUN);
-        return LAYOUT == R_INNER ? (unsigned)min(row, left_o - 1) * ld + chunk * 8 : (unsigned)row * ld + min(chunk * 8, left_o - 8);
-    }
-    static __device__ inline void load_end(End& x, const Operand<T>& op, long long o0, long long no, long long r0) {
-        const Window w(op.extent, LAYOUT == R_INNER ? o0 * op.ld + r0 : r0 * op.ld + o0, 8);
-        const char* base = (const char*)(op.data + w.base);
-#pragma unroll
-        for (int u = 0; u < COPIES; ++u) __builtin_memcpy(&x.v[u], base + w.at(end_off(u, (unsigned)op.ld, (int)min(no - o0, (long long)BO))) * 2u, 16);
-    }
-    static __device__ inline void store_end(End& x, const Operand<T>& op, long long o0, long long no, long long r0, int left, char* lds) {
-        const Window w(op.extent, LAYOUT == R_INNER ? o0 * op.ld + r0 : r0 * op.ld + o0, 8);
+    // The end of the sum, `left` < 32 of it.  What lies wholly behind it is replaced by what is there anyway; the chunk the
+    // end lies in is copied whole, but in the matrix's last row (or a row repeated with stride 0), behind which there is nothing: there it starts back() elements
+    // earlier, an even number, because addresses are multiples of four bytes.  mend_end() then puts the elements into their
+    // places, with the one that an odd number leaves out, and zeros behind the end; a lane mends the chunks it has copied.
+    static __device__ inline int back(int left) { return (8 - left % 8) % 8 + (left & 1); }
+    static __device__ inline bool nothing_behind(const Operand<T>& op, long long row, long long no) { return row == no - 1 || op.ld == 0; }
+
+    __device__ inline void copy_end(unsigned lds, int wave, const Operand<T>& op, long long o0, long long no, int left) {
+        const int lane = threadIdx.x & 63, left_o = (int)min(no - o0, (long long)BO), before = LAYOUT == R_INNER ? 8 : 0;
+        const unsigned ld = (unsigned)op.ld;
+        const char* const base = uniform(next - before * 2);
 #pragma unroll
         for (int u = 0; u < COPIES; ++u) {
-            const int row = end_slot(u) / RUN, chunk = swizzle(row, end_slot(u) % RUN);
+            const int slot = (wave * COPIES + u) * 64 + lane, row = slot / RUN, chunk = swizzle(row, slot % RUN);
+            unsigned at;
             if (LAYOUT == R_INNER) {
-                const int by = w.moved(end_off(u, (unsigned)op.ld, (int)min(no - o0, (long long)BO)));
-                if (by > 0 && by < 8) shift_down<8>(x.v[u], by);
-#pragma unroll
-                for (int e = 0; e < 8; ++e) x.v[u][e] = chunk * 8 + e < left ? x.v[u][e] : (T)0.0f;
-            } else if (row >= left) {
-                x.v[u] = (T)0.0f;
+                const int r = min(row, left_o - 1), c = chunk * 8 < left ? chunk * 8 : 0;
+                at = (unsigned)r * ld + (unsigned)(c + before - (nothing_behind(op, o0 + r, no) && c + 8 > left ? back(left) : 0));
+            } else {
+                at = (unsigned)min(row, left - 1) * ld + (unsigned)min(chunk * 8, left_o - 8);
             }
-            *(vec8*)(lds + end_slot(u) * 16) = x.v[u];
+            copy_to_lds(base, at * 2u, lds + (wave * COPIES + u) * 1024);
+        }
+    }
+
+    static __device__ inline void mend_end(char* lds, int wave, const Operand<T>& op, long long o0, long long no, long long nr, int left) {
+        const int lane = threadIdx.x & 63, left_o = (int)min(no - o0, (long long)BO);
+#pragma unroll
+        for (int u = 0; u < COPIES; ++u) {
+            const int slot = (wave * COPIES + u) * 64 + lane, row = slot / RUN, chunk = swizzle(row, slot % RUN);
+            if (LAYOUT == R_INNER ? chunk * 8 + 8 <= left : row < left) continue;
+            vec8 v = (T)0.0f;
+            if (LAYOUT == R_INNER && chunk * 8 < left) {
+                v = *(const vec8*)(lds + slot * 16);
+                if (nothing_behind(op, o0 + min(row, left_o - 1), no)) {
+                    if (back(left) < 8) shift_down<8>(v, back(left));
+                    if (left & 1) {
+                        const T last = op.data[(no - 1) * op.ld + nr - 1];
+#pragma unroll
+                        for (int e = 0; e < 8; ++e) v[e] = chunk * 8 + e == left - 1 ? last : v[e];
+                    }
+                }
+#pragma unroll
+                for (int e = 0; e < 8; ++e) v[e] = chunk * 8 + e < left ? v[e] : (T)0.0f;
+            }
+            *(vec8*)(lds + slot * 16) = v;
         }
     }
 
@@ -105,6 +130,76 @@ struct WideTile {
         return __builtin_bit_cast(vec8, v);
     }
 };
+
+typedef unsigned u32x2 __attribute__((ext_vector_type(2)));
+
+// A wave's 64 x 128 sums, four consecutive columns from i0 + x 16 + 4 (lane / 16) on of row j0 + y 16 + lane % 16 in acc[x][y],
+// become results in LDS, rows of `pitch` bytes from to on, and in kept[x][y] what is kept, if that has the results' size (if it
+// is float32 it is stored at once).  The activation is a template parameter, since a switch would stand 32 times in the
+// unrolled code.
+template <typename T, int ACT, bool KEPT>
+__device__ __forceinline__ void seal(const ProductArgs<T>& a, const f32x4 (&acc)[4][8], u32x2 (&kept)[4][8], long long i0, long long j0, char* to, int pitch) {
+    typedef typename Run<T, 4>::type vec4;
+    typedef f16 half4 __attribute__((ext_vector_type(4)));
+    const int lane = threadIdx.x & 63, jl = lane & 15, left_j = (int)min(a.nj - j0, 128LL);
+    // what is read is kept inside its row and the matrix; results that are not there get whatever it holds
+    const auto four = [&](const T* row, long long i) __attribute__((always_inline)) {
+        vec4 v;
+        const long long at = min(i, a.ni - 4);
+        __builtin_memcpy(&v, row + at, 8);
+        if (at < i) shift_down<4>(v, (int)min(i - at, 3LL));
+        return v;
+    };
+#pragma unroll
+    for (int x = 0; x < 4; ++x) {
+        const long long i = i0 + x * 16 + (lane >> 4) * 4;
+        const unsigned mask = (1u << (int)max(0LL, min(4LL, a.ni - i))) - 1;
+        float bias[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+        if (a.bias) {
+            const vec4 b = four(a.bias, i);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) bias[e] = (float)b[e];
+        }
+        vec4 res[4];
+#pragma unroll
+        for (int y = 0; y < 8; ++y) {
+            if (a.residual && y % 4 == 0)
+#pragma unroll
+                for (int u = 0; u < 4; ++u) res[u] = four(a.residual + min(j0 + (y + u) * 16 + jl, a.nj - 1) * a.ldr, i);
+            float f[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) f[e] = acc[x][y][e] + bias[e];
+            if (KEPT && Kept<T>::SLOPE && ACT != MPE_ACT_RELU) {
+                float slope[4];
+                act_both<T, 4>(ACT, f, slope);
+                half4 z;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) z[e] = (f16)(slope[e] * SLOPE_SCALE);
+                kept[x][y] = __builtin_bit_cast(u32x2, z);
+            } else {
+                if (KEPT && ACT == MPE_ACT_RELU) {
+                    vec4 z;
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) z[e] = (T)f[e];
+                    kept[x][y] = __builtin_bit_cast(u32x2, z);
+                } else if (KEPT && y * 16 + jl < left_j) {
+                    put<float, 4>((float*)a.pre + (j0 + y * 16 + jl) * a.ni + i, f, mask);
+                }
+                act_values<T, 4>(ACT, f);
+            }
+            if (a.residual) {
+#pragma unroll
+                for (int e = 0; e < 4; ++e) f[e] += (float)res[y % 4][e];
+            }
+            vec4 o;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) o[e] = (T)f[e];
+            __builtin_memcpy(to + (y * 16 + jl) * pitch + (x * 16 + (lane >> 4) * 4) * 2, &o, 8);
+            if (KEPT && (Kept<T>::SLOPE || ACT == MPE_ACT_RELU)) asm volatile("" : "+v"(kept[x][y]));      // two words from here on, not four halves
+            __builtin_amdgcn_sched_barrier(0);      // else the scheduler starts on all blocks at once and runs out of registers
+        }
+    }
+}
 
 template <typename T, int EPI, int PL, int QL>
 __global__ __launch_bounds__(256, 2) void product_wide(const ProductArgs<T> a) {
@@ -144,44 +239,85 @@ __global__ __launch_bounds__(256, 2) void product_wide(const ProductArgs<T> a) {
     TQ q;
     p.init(a.p, i0, a.ni, r0);
     q.init(a.q, j0, a.nj, r0);
-    const int steps = (int)((r1 - r0) / BK), left = (int)((r1 - r0) % BK);
-    for (int s = 0; s < 2 && s < steps; ++s) {
-        p.copy(base + s * STAGE, wave);
-        q.copy(base + s * STAGE + TP::BYTES, wave);
-    }
-    if (left) {         // the end of the sum first, in the stage that is still free
-        typename TP::End ep;
-        typename TQ::End eq;
-        TP::load_end(ep, a.p, i0, a.ni, r1 - left);
-        TQ::load_end(eq, a.q, j0, a.nj, r1 - left);
-        TP::store_end(ep, a.p, i0, a.ni, r1 - left, left, lds + 2 * STAGE);
-        TQ::store_end(eq, a.q, j0, a.nj, r1 - left, left, lds + 2 * STAGE + TP::BYTES);
-        __syncthreads();
-        multiply(lds + 2 * STAGE);
-    }
+    const int whole = (int)((r1 - r0) / BK), left = (int)((r1 - r0) % BK), steps = whole + (left ? 1 : 0);
+    const auto copy = [&](int s, unsigned to) __attribute__((always_inline)) {
+        if (s < whole) {
+            p.copy(to, wave);
+            q.copy(to + TP::BYTES, wave);
+        } else {
+            p.copy_end(to, wave, a.p, i0, a.ni, left);
+            q.copy_end(to + TP::BYTES, wave, a.q, j0, a.nj, left);
+        }
+    };
+    for (int s = 0; s < 2 && s < steps; ++s) copy(s, base + s * STAGE);
     int stage = 0;
     for (int s = 0; s < steps; ++s) {
         // stage s has landed when at most the copies of stage s + 1 are under way; the barrier makes that true of every
         // wave's share, and says that nobody reads stage s - 1 any more, into which stage s + 2 goes
         if (s + 1 < steps) asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" ::"n"(TP::COPIES + TQ::COPIES) : "memory");
-        else asm volatile("s_waitcnt vmcnt(0)\n\ts_barrier" ::: "memory");
-        if (s + 2 < steps) {
-            const unsigned to = base + (stage == 0 ? 2 : stage - 1) * STAGE;
-            p.copy(to, wave);
-            q.copy(to + TP::BYTES, wave);
+        else if (!left) asm volatile("s_waitcnt vmcnt(0)\n\ts_barrier" ::: "memory");
+        else {
+            asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+            TP::mend_end(lds + stage * STAGE, wave, a.p, i0, a.ni, r1, left);
+            TQ::mend_end(lds + stage * STAGE + TP::BYTES, wave, a.q, j0, a.nj, r1, left);
+            __syncthreads();
         }
+        if (s + 2 < steps) copy(s + 2, base + (stage == 0 ? 2 : stage - 1) * STAGE);
         multiply(lds + stage * STAGE);
         stage = stage == 2 ? 0 : stage + 1;
     }
 
-    constexpr int N = EPI == EPI_FORWARD ? 8 : 4;       // a thread's columns
+    if constexpr (EPI != EPI_PARTIAL) {
+        // Results become what is stored while they are in registers, pass through LDS and leave as whole rows.
+        constexpr int PITCH = BI * 2 + 16;
+        static_assert(BJ * PITCH <= Wide::STAGES * STAGE, "the results pass through the stages' memory");
+        const int it = threadIdx.x % (BI / 8) * 8;
+        const int have = (int)max(0LL, min(8LL, a.ni - i0 - it)), rows = (int)min((long long)BJ, a.nj - j0);
+        const auto leave = [&](T* to, long long ld) __attribute__((always_inline)) {
+            T* const column = to + j0 * ld + i0 + it;
+            __syncthreads();
+            if (have > 0)
+#pragma unroll 4
+                for (int jt = threadIdx.x / (BI / 8); jt < rows; jt += 256 / (BI / 8))
+                    put<T, 8>(column + jt * ld, *(const vec8*)(lds + jt * PITCH + it * 2), (1u << have) - 1);
+        };
+        // one path an activation, to the end: where paths meet again the compiler holds the tile twice
+        const auto finish_as = [&](auto act, auto keep) __attribute__((always_inline)) {
+            constexpr bool SMALL = decltype(keep)::value && (Kept<T>::SLOPE || decltype(act)::value == MPE_ACT_RELU);
+            u32x2 kept[FI][FJ];
+            char* const mine = lds + wj * PITCH + wi * 2;
+            __syncthreads();
+            seal<T, decltype(act)::value, decltype(keep)::value>(a, acc, kept, i0 + wi, j0 + wj, mine, PITCH);
+            leave(a.out, a.ldo);
+            if constexpr (SMALL) {
+                __syncthreads();
+#pragma unroll
+                for (int y = 0; y < FJ; ++y)
+#pragma unroll
+                    for (int x = 0; x < FI; ++x) *(u32x2*)(mine + (y * 16 + (lane & 15)) * PITCH + (x * 16 + (lane >> 4) * 4) * 2) = kept[x][y];
+                leave((T*)a.pre, a.ni);
+            }
+        };
+        const auto with = [&](auto act) __attribute__((always_inline)) {
+            if (a.pre) finish_as(act, std::true_type());
+            else finish_as(act, std::false_type());
+        };
+        if constexpr (EPI == EPI_STORE) return finish_as(std::integral_constant<int, MPE_ACT_NONE>(), std::false_type());
+        switch (a.act) {
+            case MPE_ACT_NONE: return finish_as(std::integral_constant<int, MPE_ACT_NONE>(), std::false_type());
+            case MPE_ACT_TANH: return with(std::integral_constant<int, MPE_ACT_TANH>());
+            case MPE_ACT_RELU: return with(std::integral_constant<int, MPE_ACT_RELU>());
+            case MPE_ACT_GELU: return with(std::integral_constant<int, MPE_ACT_GELU>());
+            default: return with(std::integral_constant<int, MPE_ACT_SILU>());
+        }
+    }
+    // partial sums are float32 and pass in two halves
+    constexpr int N = 4;                                // a thread's columns
     const int it = threadIdx.x % (BI / N) * N;          // a thread's columns, the same in every row it takes
     const long long i = i0 + it;
     const int have = (int)max(0LL, min((long long)N, a.ni - i));
     const unsigned mask = (1u << have) - 1;
-    float bias[N];
-#pragma unroll
-    for (int e = 0; e < N; ++e) bias[e] = EPI == EPI_FORWARD && a.bias && e < have ? (float)a.bias[i + e] : 0.0f;
+    const float bias[N] = {};
     float* const res = (float*)lds;
 #pragma unroll
     for (int half = 0; half < HALVES; ++half) {
