@@ -440,7 +440,7 @@ int mpe_gae(int device, int mode, int64_t n_envs, int32_t n_agents, int32_t n_st
  *             matters); else with MPE_BF16 2^14 times the slope f'(x w^T + bias) in float16, and with MPE_F32 and MPE_F16
  *             x w^T + bias in float32 (rounded to 16 bits it would cost the gradients more than any other step)
  * Products are summed in float32; one rounding to T at the end.  m may be 0; n, k and the row strides of x, w and dy
- * reach at most 2^22.
+ * reach at most 2^22, m 2^29, and m n and m k 2^37.
  * mpe_linear_workspace gives the bytes the two passes need (0 may come back: workspace may then be NULL).
  */
 #define MPE_ACT_NONE 0
@@ -500,8 +500,8 @@ int mpe_ppo_loss_backward(int device, int dtype, int64_t rows, int64_t v, const 
  * Global norm over n tensors, and clipping to it: norm = sqrt(sum of squares of every element), dst = src * f with
  * f = max_norm / norm where norm > max_norm, else 1 (NaN if the norm is).  src, dst, counts (elements, 0 allowed) and
  * dtypes are HOST arrays of length n, read before the call returns; the tensors are dense.  dst NULL: the norm alone;
- * dst[i] == src[i]: in place.  Any other overlap among the tensors is an error of the caller's.  norm: one device float,
- * or NULL.  The squares are summed in float64, in an order that does not change from run to run.
+ * dst[i] == src[i]: in place.  Any other overlap of a destination with a tensor is refused (sources may overlap each
+ * other).  norm: one device float, or NULL.  The squares are summed in float64, in an order that does not change from run to run.
  */
 #define MPE_CLIP_WORKSPACE_BYTES 16384
 int mpe_clip_grad_norm(int device, int32_t n, const void* const* src, void* const* dst, const int64_t* counts, const int32_t* dtypes,

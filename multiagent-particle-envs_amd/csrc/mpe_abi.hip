@@ -5,6 +5,8 @@
 #include <stdio.h>
 #include <string.h>
 
+#include <algorithm>
+#include <memory>
 #include <new>
 
 #include "mpe_launch.hpp"
@@ -640,6 +642,13 @@ static int check_learn(const char* who, int dtype, int64_t rows, int64_t a, int6
     return MPE_OK;
 }
 
+// A product's tiles are counted in 24 bits, and the smallest tile is 64 x 64 (128 rows of up to 16 columns).
+static int check_product(const char* who, int64_t m, int64_t n, int64_t k) {
+    const int64_t rows = (int64_t)1 << 29, elems = (int64_t)1 << 37;
+    if (m > rows || (m > 0 && (n > elems / m || k > elems / m))) return fail(nullptr, MPE_ERR_INVALID, "%s: at most 2^29 rows, and 2^37 elements in them", who);
+    return MPE_OK;
+}
+
 static bool misaligned(const void* p, int64_t bytes) { return ((uintptr_t)p & (uintptr_t)(bytes - 1)) != 0; }
 
 static int check_workspace(const char* who, const void* ws, int64_t have, int64_t need) {
@@ -665,7 +674,8 @@ static bool bad_stride(int64_t rows, int64_t ld, int64_t cols, bool broadcast) {
 }
 
 int mpe_linear_workspace(int dtype, int activation, int64_t m, int64_t n, int64_t k, int64_t* forward_bytes, int64_t* backward_bytes) {
-    const int rc = check_learn("mpe_linear_workspace", dtype, m, n, k);
+    int rc = check_learn("mpe_linear_workspace", dtype, m, n, k);
+    if (rc == MPE_OK) rc = check_product("mpe_linear_workspace", m, n, k);
     if (rc != MPE_OK) return rc;
     if (activation < MPE_ACT_NONE || activation > MPE_ACT_TANH_OUT) return fail(nullptr, MPE_ERR_INVALID, "mpe_linear_workspace: unknown activation %d", activation);
     if (forward_bytes) *forward_bytes = linear_forward_workspace(dtype, m, n, k);
@@ -677,6 +687,7 @@ int mpe_linear_forward(int device, int dtype, int activation, int64_t m, int64_t
                        int64_t ldw, const void* bias, const void* residual, int64_t ldr, void* y, int64_t ldy, void* pre, void* workspace,
                        int64_t workspace_bytes, mpe_stream_t stream) {
     int rc = check_learn("mpe_linear_forward", dtype, m, n, k);
+    if (rc == MPE_OK) rc = check_product("mpe_linear_forward", m, n, k);
     if (rc != MPE_OK) return rc;
     if (activation < MPE_ACT_NONE || activation > MPE_ACT_SILU) return fail(nullptr, MPE_ERR_INVALID, "mpe_linear_forward: unknown activation %d", activation);
     if (m == 0) return MPE_OK;
@@ -706,6 +717,7 @@ int mpe_linear_backward(int device, int dtype, int activation, int64_t m, int64_
                         int64_t ldx, const void* w, int64_t ldw, const void* pre, void* dx, int64_t lddx, void* dw, void* db, void* workspace,
                         int64_t workspace_bytes, mpe_stream_t stream) {
     int rc = check_learn("mpe_linear_backward", dtype, m, n, k);
+    if (rc == MPE_OK) rc = check_product("mpe_linear_backward", m, n, k);
     if (rc != MPE_OK) return rc;
     if (activation < MPE_ACT_NONE || activation > MPE_ACT_TANH_OUT) return fail(nullptr, MPE_ERR_INVALID, "mpe_linear_backward: unknown activation %d", activation);
     if (activation == MPE_ACT_TANH_OUT && dtype != MPE_F32) return fail(nullptr, MPE_ERR_INVALID, "mpe_linear_backward: MPE_ACT_TANH_OUT is for MPE_F32");
@@ -816,6 +828,38 @@ int mpe_ppo_loss_backward(int device, int dtype, int64_t rows, int64_t v, const 
     return e == hipSuccess ? MPE_OK : hip_fail(nullptr, e, "mpe_ppo_loss_backward");
 }
 
+// Destinations lie apart from each other, and from every source but their own, which they may be.
+static int check_destinations(const char* who, int32_t n, const void* const* src, void* const* dst, const int64_t* counts, const int32_t* dtypes) {
+    struct Span {
+        uintptr_t from, to;
+        int32_t i;
+    };
+    Span* const spans = new (std::nothrow) Span[n > 0 ? n : 1];
+    if (!spans) return fail(nullptr, MPE_ERR_HIP, "%s: out of host memory", who);
+    const std::unique_ptr<Span[]> owner(spans);
+    bool in_place = true;
+    int32_t here = 0;
+    for (int32_t i = 0; i < n; ++i)
+        if (counts[i] > 0) {
+            spans[here++] = {(uintptr_t)dst[i], (uintptr_t)dst[i] + (uintptr_t)(counts[i] * dtype_bytes(dtypes[i])), i};
+            in_place = in_place && dst[i] == src[i];
+        }
+    std::sort(spans, spans + here, [](const Span& a, const Span& b) { return a.from < b.from; });
+    for (int32_t k = 1; k < here; ++k)
+        if (spans[k].from < spans[k - 1].to)
+            return fail(nullptr, MPE_ERR_INVALID, "%s: a tensor is given twice, or two share memory (destinations %d and %d)", who, spans[k - 1].i, spans[k].i);
+    if (in_place) return MPE_OK;
+    for (int32_t i = 0; i < n; ++i) {
+        if (counts[i] == 0) continue;
+        const uintptr_t from = (uintptr_t)src[i], to = from + (uintptr_t)(counts[i] * dtype_bytes(dtypes[i]));
+        const Span* s = std::upper_bound(spans, spans + here, from, [](uintptr_t at, const Span& a) { return at < a.to; });
+        for (; s != spans + here && s->from < to; ++s)
+            if (s->i != i || dst[i] != src[i])
+                return fail(nullptr, MPE_ERR_INVALID, "%s: destination %d overlaps the source of tensor %d", who, s->i, i);
+    }
+    return MPE_OK;
+}
+
 int mpe_clip_grad_norm(int device, int32_t n, const void* const* src, void* const* dst, const int64_t* counts, const int32_t* dtypes, double max_norm,
                        float* norm, void* workspace, int64_t workspace_bytes, mpe_stream_t stream) {
     if (n < 0 || (n > 0 && (!src || !counts || !dtypes))) return fail(nullptr, MPE_ERR_INVALID, "mpe_clip_grad_norm: src, counts and dtypes must not be NULL");
@@ -829,10 +873,10 @@ int mpe_clip_grad_norm(int device, int32_t n, const void* const* src, void* cons
         const int64_t s = dtype_bytes(dtypes[i]);
         if (!src[i] || (dst && !dst[i]) || misaligned(src[i], s) || (dst && misaligned(dst[i], s)))
             return fail(nullptr, MPE_ERR_INVALID, "mpe_clip_grad_norm: tensor %d: NULL or misaligned", i);
-        if (dst && dst[i] != src[i] && overlap(dst[i], counts[i] * s, src[i], counts[i] * s))
-            return fail(nullptr, MPE_ERR_INVALID, "mpe_clip_grad_norm: tensor %d: source and destination overlap", i);
     }
-    const int rc = check_workspace("mpe_clip_grad_norm", workspace, workspace_bytes, MPE_CLIP_WORKSPACE_BYTES);
+    int rc = MPE_OK;
+    if (dst) rc = check_destinations("mpe_clip_grad_norm", n, src, dst, counts, dtypes);
+    if (rc == MPE_OK) rc = check_workspace("mpe_clip_grad_norm", workspace, workspace_bytes, MPE_CLIP_WORKSPACE_BYTES);
     if (rc != MPE_OK) return rc;
     DeviceScope scope(device);
     if (scope.status != hipSuccess) return hip_fail(nullptr, scope.status, "hipSetDevice");

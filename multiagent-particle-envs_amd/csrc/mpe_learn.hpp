@@ -1,4 +1,4 @@
-// Shared by the trainer-side kernels (mpe_linear.hip, mpe_ppo.hip, mpe_clip.hip): element types, their conversions, the
+// Shared by the trainer-side kernels (mpe_linear*.hip, mpe_ppo.hip, mpe_clip.hip): element types, their conversions, the
 // reductions, and the launcher entry points.  Every sum, softmax statistic and norm is held in 32 bits or more; a value
 // is rounded to 16 bits only where it leaves a kernel in that type or enters a matrix instruction of that type.
 #pragma once
@@ -26,25 +26,19 @@ inline hipError_t with_dtype(int dtype, F&& f) {
     }
 }
 
-__device__ inline float wave_sum(float v) {
-    for (int o = 32; o; o >>= 1) v += __shfl_xor(v, o);
-    return v;
-}
 __device__ inline double wave_sum(double v) {
     for (int o = 32; o; o >>= 1) v += __shfl_xor(v, o);
     return v;
 }
-__device__ inline float wave_max(float v) {
-    for (int o = 32; o; o >>= 1) v = fmaxf(v, __shfl_xor(v, o));
-    return v;
-}
+
+// exp by the hardware's 2^x: off by the rounding of x log2(e), |x| 2^-24, and one step
+__device__ inline float fast_exp(float x) { return __builtin_amdgcn_exp2f(x * 1.44269504088896341f); }
 
 // Sum over a workgroup of WAVES waves, in a fixed order; the result is valid in every thread.  `scratch` holds WAVES
 // doubles and may be reused after the call's next barrier.
 template <int WAVES>
 __device__ inline double block_sum(double v, double* scratch) {
     v = wave_sum(v);
-    if (WAVES == 1) return v;
     __syncthreads();
     if ((threadIdx.x & 63) == 0) scratch[threadIdx.x >> 6] = v;
     __syncthreads();

@@ -23,9 +23,6 @@ namespace mpe {
 
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 
-// exp by the hardware's 2^x: off by the rounding of x log2(e), |x| 2^-24, and one step
-__device__ inline float fast_exp(float x) { return __builtin_amdgcn_exp2f(x * 1.44269504088896341f); }
-
 // 1 / (1 + e^-z); e^-z overflows to infinity and gives 0
 __device__ inline float sigmoid(float z) { return __builtin_amdgcn_rcpf(1.0f + fast_exp(-z)); }
 

@@ -150,25 +150,32 @@ __device__ __forceinline__ void seal(const ProductArgs<T>& a, const f32x4 (&acc)
         if (at < i) shift_down<4>(v, (int)min(i - at, 3LL));
         return v;
     };
+    const long long i0l = i0 + (lane >> 4) * 4;
+    // everything is asked for at once; the four blocks of a row after one another, since they share lines
+    vec4 res[4][8];
+    if (a.residual) {
 #pragma unroll
-    for (int x = 0; x < 4; ++x) {
-        const long long i = i0 + x * 16 + (lane >> 4) * 4;
-        const unsigned mask = (1u << (int)max(0LL, min(4LL, a.ni - i))) - 1;
-        float bias[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-        if (a.bias) {
-            const vec4 b = four(a.bias, i);
+        for (int y = 0; y < 8; ++y)
 #pragma unroll
-            for (int e = 0; e < 4; ++e) bias[e] = (float)b[e];
+            for (int x = 0; x < 4; ++x) res[x][y] = four(a.residual + min(j0 + y * 16 + jl, a.nj - 1) * a.ldr, i0l + x * 16);
+    }
+    float bias[4][4] = {};
+    if (a.bias) {
+#pragma unroll
+        for (int x = 0; x < 4; ++x) {
+            const vec4 b = four(a.bias, i0l + x * 16);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) bias[x][e] = (float)b[e];
         }
-        vec4 res[4];
+    }
 #pragma unroll
-        for (int y = 0; y < 8; ++y) {
-            if (a.residual && y % 4 == 0)
+    for (int y = 0; y < 8; ++y) {
 #pragma unroll
-                for (int u = 0; u < 4; ++u) res[u] = four(a.residual + min(j0 + (y + u) * 16 + jl, a.nj - 1) * a.ldr, i);
+        for (int x = 0; x < 4; ++x) {
+            const long long i = i0l + x * 16;
             float f[4];
 #pragma unroll
-            for (int e = 0; e < 4; ++e) f[e] = acc[x][y][e] + bias[e];
+            for (int e = 0; e < 4; ++e) f[e] = acc[x][y][e] + bias[x][e];
             if (KEPT && Kept<T>::SLOPE && ACT != MPE_ACT_RELU) {
                 float slope[4];
                 act_both<T, 4>(ACT, f, slope);
@@ -183,13 +190,13 @@ __device__ __forceinline__ void seal(const ProductArgs<T>& a, const f32x4 (&acc)
                     for (int e = 0; e < 4; ++e) z[e] = (T)f[e];
                     kept[x][y] = __builtin_bit_cast(u32x2, z);
                 } else if (KEPT && y * 16 + jl < left_j) {
-                    put<float, 4>((float*)a.pre + (j0 + y * 16 + jl) * a.ni + i, f, mask);
+                    put<float, 4>((float*)a.pre + (j0 + y * 16 + jl) * a.ni + i, f, (1u << (int)max(0LL, min(4LL, a.ni - i))) - 1);
                 }
                 act_values<T, 4>(ACT, f);
             }
             if (a.residual) {
 #pragma unroll
-                for (int e = 0; e < 4; ++e) f[e] += (float)res[y % 4][e];
+                for (int e = 0; e < 4; ++e) f[e] += (float)res[x][y][e];
             }
             vec4 o;
 #pragma unroll
@@ -348,7 +355,6 @@ inline bool wide_operand(const Operand<T>& o, int layout, long long outputs) {
 template <typename T, int EPI, int PL, int QL>
 inline hipError_t launch_product_wide(ProductArgs<T> a, int splits, hipStream_t st) {
     const long long ti = (a.ni + Wide::BI - 1) / Wide::BI, tiles = ti * ((a.nj + Wide::BJ - 1) / Wide::BJ);
-    if (tiles * splits > 0x7fffffffLL) return hipErrorInvalidValue;
     a.ti = (int)ti;
     a.tiles = (unsigned)tiles;
     hipLaunchKernelGGL((product_wide<T, EPI, PL, QL>), dim3((unsigned)(tiles * splits)), dim3(256), 0, st, a);

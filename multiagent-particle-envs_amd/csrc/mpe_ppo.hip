@@ -5,7 +5,7 @@
 //   loss = sum w (-s + cv v - ce H) / sum w
 //   d loss / d l_k = w / sum w * (g (1[k = a] - p_k) + ce p_k (log p_k + H)),   g = -q A where q A <= the clamped term, else 0
 // A row counts only if its weight is not zero and its action lies in [0, v), is allowed and has a logit above -inf (so
-// that at least one word is left); any other row is not read further and its gradients are zero.
+// that at least one word is left); any other row's gradients are zero.
 //
 // The backward pass takes no softmax statistics from the forward pass: it has to read the logits again anyway and
 // recomputes them while the row is at hand.
@@ -59,9 +59,6 @@ __device__ inline void value_terms(const PpoArgs& p, const Row& x, double& loss,
         }
     }
 }
-
-// exp by the hardware's 2^x: off by the rounding of d log2(e), |d| 2^-24, and one step
-__device__ inline float fast_exp(float d) { return __builtin_amdgcn_exp2f(d * 1.44269504088896341f); }
 
 __device__ inline float fast_log(float x) { return __builtin_amdgcn_logf(x) * 0.69314718055994531f; }
 

@@ -296,6 +296,7 @@ Tensor clip(const std::vector<Tensor>& ts, double max_norm, const std::optional<
         count[i] = t.numel();
         if (!outs) continue;
         const Tensor& o = (*outs)[i];
+        TORCH_CHECK_VALUE(!at::GradMode::is_enabled() || !o.requires_grad(), "clip_grad_norm: out ", i, " requires gradients, which clipping does not have");
         if (!o.is_same(t))
             TORCH_CHECK_VALUE(o.layout() == at::kStrided && o.scalar_type() == t.scalar_type() && o.device() == dev && o.sizes() == t.sizes() &&
                                   ((o.is_contiguous() && t.is_contiguous()) || o.strides() == t.strides()),

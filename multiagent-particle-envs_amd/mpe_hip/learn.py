@@ -81,14 +81,16 @@ def _list(tensors):
 
 def grad_norm(tensors):
     """``sqrt`` of the sum of all squares over ``tensors`` (float32, bfloat16, float16, mixed; summed in float64): a float32
-    scalar on their GPU.  A tensor given twice counts twice."""
+    scalar on their GPU, which carries no gradient.  A tensor given twice counts twice."""
     return (_module or _native()).clip(_list(tensors), 0.0, None)
 
 
 def clip_grad_norm(tensors, max_norm, out):
     """Writes ``t * f`` into the tensors of ``out``, one for each of ``tensors``, ``f = max_norm / norm`` where the global norm
     is above ``max_norm`` and 1 otherwise (NaN if the norm is; an infinite norm makes it 0).  Returns the norm before
-    clipping, a float32 scalar on the GPU; nothing waits for it."""
+    clipping, a float32 scalar on the GPU; nothing waits for it.  A tensor may be its own ``out``; any other overlap of an
+    ``out`` with a tensor is refused.  Nothing here is differentiable: an ``out`` that requires gradients is refused
+    unless they are off."""
     return (_module or _native()).clip(_list(tensors), max_norm, _list(out))
 
 

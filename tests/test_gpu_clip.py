@@ -155,3 +155,20 @@ def test_refusals():
         mpe_hip.clip_grad_norm([p], 1.0, out=[p])           # written in place: autograd is told
     with pytest.raises(RuntimeError, match="modified"):
         q.backward()
+
+
+def test_destinations_that_meet_other_sources_or_carry_gradients_are_refused():
+    import mpe_hip
+    a, b = torch.ones(8, device=DEV), torch.ones(8, device=DEV)
+    with pytest.raises(mpe_hip.MpeError, match="overlaps the source"):
+        mpe_hip.clip_grad_norm([a, b], 1.0, out=[b, a])
+    p = torch.ones(8, device=DEV, requires_grad=True)
+    with pytest.raises(ValueError, match="requires gradients"):
+        mpe_hip.clip_grad_norm([a], 1.0, out=[p])
+    with torch.no_grad():
+        mpe_hip.clip_grad_norm([a], 1.0, out=[p])
+    assert torch.allclose(p.detach(), torch.full_like(a, 8 ** -0.5), rtol=2.0 ** -23, atol=0)
+    # a source may be given twice, with two destinations
+    c, d = torch.empty_like(a), torch.empty_like(a)
+    norm = mpe_hip.clip_grad_norm([a, a], 2.0, out=[c, d])
+    assert float(norm) == 4.0 and torch.equal(c, torch.full_like(a, 0.5)) and torch.equal(d, c)

@@ -193,6 +193,65 @@ def test_large_products(m, k, n, ld, dt):
     check_backward(x, w, b, None, dy, "none")
 
 
+@pytest.mark.parametrize("dt", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("act", ACTS)
+def test_every_activation_in_large_tiles(act, dt):
+    x, w, b, r, dy = make(8193, 96, 1028, dt, residual=True, exact=act == "relu")
+    check_forward(x, w, b, r, act)
+    check_forward(x, w, None, None, act)
+    check_backward(x, w, b, r, dy, act)
+
+
+@pytest.mark.parametrize("dt", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("k", [65, 67, 70, 71, 88, 95])
+def test_large_sums_that_end_where_memory_ends(k, dt):
+    """Copies to LDS at the end of the sum, every kind of last chunk: the last row ends with its buffer, NaN behind it and in
+    the gap between the rows."""
+    import mpe_hip
+    m, n, ld = 16400, 520, k + (k & 1)
+    x, w, b, r, dy = make(m, k, n, dt, residual=True)
+    def framed(t):
+        flat = torch.full(((t.shape[0] + 1) * ld + 64,), math.nan, device=DEV).to(dt)
+        v = flat[34:34 + t.shape[0] * ld].view(t.shape[0], ld)[:, :t.shape[1]]
+        v.copy_(t)
+        return v
+    one, two = mpe_hip.linear(x, w, b, "silu", r), mpe_hip.linear(framed(x), framed(w), b, "silu", r)
+    check_forward(framed(x), framed(w), b, r, "silu")
+    assert k & 1 or torch.equal(one, two)           # an odd row stride goes another way
+
+
+@pytest.mark.parametrize("dt", [torch.bfloat16, torch.float16])
+def test_one_upstream_row_for_all_in_large_tiles(dt):
+    """dy expanded over the rows, its end inside a chunk and at the end of its memory."""
+    import mpe_hip
+    m, k, n = 65537, 128, 270
+    x, w, b, _, _ = make(m, k, n, dt)
+    row = torch.full((2 * n + 64,), math.nan, device=DEV).to(dt)[32:32 + n].copy_(torch.randn(n, device=DEV).to(dt))
+    q = [t.detach().clone().requires_grad_(True) for t in (x, w, b)]
+    y = mpe_hip.linear(*q)
+    got = torch.autograd.grad(y, q, row.expand(m, n))
+    want = torch.autograd.grad(mpe_hip.linear(*q), q, row.expand(m, n).contiguous())
+    assert torch.equal(got[0], want[0])
+    # two orders of m float32 additions, then one rounding each
+    mags = (row.double().abs()[:, None] * x.double().abs().sum(0), m * row.double().abs())
+    for a, c, mag in zip(got[1:], want[1:], mags):
+        fits = mag < torch.finfo(dt).max / 2 if dt == torch.float16 else torch.ones_like(mag, dtype=torch.bool)       # 65537 equal numbers pass float16's range: sums of them have to do so both times
+        assert torch.equal(a[~fits].isinf(), c[~fits].isinf())
+        inside(a[fits], c[fits].double(), (2 * (m + 8) * V * mag + 2 * U[dt] * c.double().abs() + TINY[dt])[fits], "two orders")
+
+
+def test_more_rows_than_a_grid_dimension_of_strips():
+    """Column sums over 8.4 M rows.  Values of -1, 0 and 1: every sum stays below 2^24 and is exact in float32."""
+    import mpe_hip
+    period, times = 1024, 8204
+    g = torch.Generator(DEV).manual_seed(5)
+    xp, dp = (torch.randint(-1, 2, (period, c), device=DEV, generator=g).to(torch.bfloat16) for c in (256, 128))
+    w, b = torch.zeros(128, 256, device=DEV, dtype=torch.bfloat16).requires_grad_(True), torch.zeros(128, device=DEV, dtype=torch.bfloat16).requires_grad_(True)
+    dw, db = torch.autograd.grad(mpe_hip.linear(xp.repeat(times, 1), w, b), (w, b), dp.repeat(times, 1))
+    assert torch.equal(dw, (dp.double().T @ xp.double() * times).to(torch.bfloat16))
+    assert torch.equal(db, (dp.double().sum(0) * times).to(torch.bfloat16))
+
+
 @pytest.mark.parametrize("dt", DTYPES)
 def test_long_reduction_over_rows(dt):
     """The weight gradient of a whole rollout step: many rows, few columns."""

@@ -102,6 +102,37 @@ def test_clip_refuses():
         assert text in _err(lib), (kw, _err(lib))
 
 
+def test_clip_refuses_destinations_that_meet_other_tensors():
+    _, lib = _lib()
+    arr = lambda t, *v: (t * len(v))(*v)
+    cnt, typ = arr(C.c_int64, 10, 20, 0), arr(C.c_int32, 0, 2, 0)
+    call = lambda src, dst: lib.mpe_clip_grad_norm(0, 3, arr(C.c_void_p, *src), arr(C.c_void_p, *dst), cnt, typ, 1.0, 3 * A, 4 * A, 1 << 19, None)
+    for src, dst, text in (((A, 2 * A, None), (2 * A, A, None), "overlaps the source"),                 # swapped
+                           ((A, 2 * A, None), (5 * A, A + 36, None), "overlaps the source of tensor 0"),    # its last element
+                           ((A, 2 * A, None), (5 * A, 5 * A + 38, None), "given twice"),
+                           ((A, A, None), (A, A, None), "given twice"),
+                           ((A, A, None), (A, 2 * A, None), "overlaps the source of tensor 1")):
+        assert call(src, dst) == -1 and text in _err(lib), (src, dst, _err(lib))
+
+
+@pytest.mark.parametrize("kw", [dict(m=(1 << 29) + 1, n=1, k=1), dict(m=1 << 20, n=(1 << 17) + 1, k=1), dict(m=1 << 20, n=1, k=(1 << 17) + 1)])
+def test_linear_refuses_more_tiles_than_a_grid_has(kw):
+    _, lib = _lib()
+    far = {n: (i + 1) << 44 for i, n in enumerate(("x", "w", "bias", "res", "y", "pre"))}
+    assert _forward(lib, **far, **kw, ldx=kw["k"], ldw=kw["k"], ldr=kw["n"], ldy=kw["n"]) == -1 and "2^29 rows" in _err(lib), _err(lib)
+    far = {n: (i + 1) << 44 for i, n in enumerate(("dy", "x", "w", "pre", "dx", "dw", "db", "ws"))}
+    assert _backward(lib, **far, **kw, lddy=kw["n"], ldx=kw["k"], ldw=kw["k"], lddx=kw["k"]) == -1 and "2^29 rows" in _err(lib), _err(lib)
+
+
+def test_linear_workspace_counts_whole_strips_of_many_rows():
+    """The column sums of a large 16-bit weight gradient: at most 32768 strips, whatever m."""
+    _, lib = _lib()
+    b = C.c_int64(-1)
+    for m in (1 << 22, (1 << 22) + 1, 1 << 25, 1 << 29):
+        assert lib.mpe_linear_workspace(2, 0, m, 128, 256, None, C.byref(b)) == 0
+        assert b.value <= 4 * (512 * 128 * 256 + 32768 * 128), (m, b.value)
+
+
 def test_python_entry_points_refuse_cpu_tensors_and_bad_arguments():
     import mpe_hip
     x, w = torch.zeros(4, 3), torch.zeros(2, 3)
