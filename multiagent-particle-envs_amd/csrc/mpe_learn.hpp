@@ -26,13 +26,32 @@ inline hipError_t with_dtype(int dtype, F&& f) {
     }
 }
 
-__device__ inline double wave_sum(double v) {
-    for (int o = 32; o; o >>= 1) v += __shfl_xor(v, o);
-    return v;
-}
-
 // exp by the hardware's 2^x: off by the rounding of x log2(e), |x| 2^-24, and one step
 __device__ inline float fast_exp(float x) { return __builtin_amdgcn_exp2f(x * 1.44269504088896341f); }
+
+// f over the lanes of a wave, the result in all of them.  Within 16 lanes by DPP, which costs a few cycles where a shuffle
+// through LDS costs some 70: neighbours, pairs, then the mirror image of 8 and of 16 lanes.
+template <int CTRL>
+__device__ inline float dpp(float v) { return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), CTRL, 0xf, 0xf, true)); }
+template <int CTRL>
+__device__ inline double dpp(double v) {
+    typedef int i32x2 __attribute__((ext_vector_type(2)));
+    const i32x2 a = __builtin_bit_cast(i32x2, v);
+    const i32x2 r = {__builtin_amdgcn_update_dpp(0, a[0], CTRL, 0xf, 0xf, true), __builtin_amdgcn_update_dpp(0, a[1], CTRL, 0xf, 0xf, true)};
+    return __builtin_bit_cast(double, r);
+}
+template <typename V, typename F>
+__device__ inline V wave_reduce(V v, F&& f) {
+    v = f(v, dpp<0xb1>(v));
+    v = f(v, dpp<0x4e>(v));
+    v = f(v, dpp<0x141>(v));
+    v = f(v, dpp<0x140>(v));
+    v = f(v, __shfl_xor(v, 16));
+    return f(v, __shfl_xor(v, 32));
+}
+
+template <typename V>
+__device__ inline V wave_sum(V v) { return wave_reduce(v, [](V a, V b) { return a + b; }); }
 
 // Sum over a workgroup of WAVES waves, in a fixed order; the result is valid in every thread.  `scratch` holds WAVES
 // doubles and may be reused after the call's next barrier.

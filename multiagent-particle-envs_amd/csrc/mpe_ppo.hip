@@ -356,9 +356,14 @@ __global__ __launch_bounds__(256) void ppo_many(const PpoArgs p) {
                 }
             }
         }
-        for (int o = 32; o; o >>= 1) {
-            const Soft b = {__shfl_xor(q.m, o), __shfl_xor(q.s, o), __shfl_xor(q.t, o)};
-            q = merge(q, b);
+        // the wave's maximum first: then its sums are plain sums
+        {
+            const float m = wave_reduce(q.m, [](float a, float b) { return fmaxf(a, b); });
+            const float d = q.m == -INFINITY ? -INFINITY : q.m - m, e = fast_exp(d);       // a thread that holds nothing has the factor 0
+            const float t = e * q.t + q.s * weighted(e, d);
+            q.m = m;
+            q.t = wave_sum(t);
+            q.s = wave_sum(q.s * e);
         }
         if (W > 1) {
             __syncthreads();
