@@ -247,20 +247,28 @@ __global__ __launch_bounds__(256, 2) void product_wide(const ProductArgs<T> a) {
     p.init(a.p, i0, a.ni, r0);
     q.init(a.q, j0, a.nj, r0);
     const int whole = (int)((r1 - r0) / BK), left = (int)((r1 - r0) % BK), steps = whole + (left ? 1 : 0);
-    const auto copy = [&](int s, unsigned to) __attribute__((always_inline)) {
-        if (s < whole) {
-            p.copy(to, wave);
-            q.copy(to + TP::BYTES, wave);
-        } else {
-            p.copy_end(to, wave, a.p, i0, a.ni, left);
-            q.copy_end(to + TP::BYTES, wave, a.q, j0, a.nj, left);
-        }
+    const auto copy = [&](unsigned to) __attribute__((always_inline)) {
+        p.copy(to, wave);
+        q.copy(to + TP::BYTES, wave);
     };
-    for (int s = 0; s < 2 && s < steps; ++s) copy(s, base + s * STAGE);
-    int stage = 0;
-    for (int s = 0; s < steps; ++s) {
-        // stage s has landed when at most the copies of stage s + 1 are under way; the barrier makes that true of every
-        // wave's share, and says that nobody reads stage s - 1 any more, into which stage s + 2 goes
+    const auto copy_end = [&](unsigned to) __attribute__((always_inline)) {
+        p.copy_end(to, wave, a.p, i0, a.ni, left);
+        q.copy_end(to + TP::BYTES, wave, a.q, j0, a.nj, left);
+    };
+    for (int s = 0; s < 2 && s < steps; ++s) {
+        if (s < whole) copy(base + s * STAGE);
+        else copy_end(base + s * STAGE);
+    }
+    // Stage s has landed when at most the copies of stage s + 1 are under way; the barrier makes that true of every wave's
+    // share, and says that nobody reads stage s - 1 any more, into which stage s + 2 goes.  The loop that runs long asks nothing.
+    int s = 0, stage = 0;
+    for (; s + 2 < whole; ++s) {
+        asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" ::"n"(TP::COPIES + TQ::COPIES) : "memory");
+        copy(base + (stage == 0 ? 2 : stage - 1) * STAGE);
+        multiply(lds + stage * STAGE);
+        stage = stage == 2 ? 0 : stage + 1;
+    }
+    for (; s < steps; ++s) {
         if (s + 1 < steps) asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" ::"n"(TP::COPIES + TQ::COPIES) : "memory");
         else if (!left) asm volatile("s_waitcnt vmcnt(0)\n\ts_barrier" ::: "memory");
         else {
@@ -269,7 +277,7 @@ __global__ __launch_bounds__(256, 2) void product_wide(const ProductArgs<T> a) {
             TQ::mend_end(lds + stage * STAGE + TP::BYTES, wave, a.q, j0, a.nj, r1, left);
             __syncthreads();
         }
-        if (s + 2 < steps) copy(s + 2, base + (stage == 0 ? 2 : stage - 1) * STAGE);
+        if (s + 2 < steps) copy_end(base + (stage == 0 ? 2 : stage - 1) * STAGE);
         multiply(lds + stage * STAGE);
         stage = stage == 2 ? 0 : stage + 1;
     }
