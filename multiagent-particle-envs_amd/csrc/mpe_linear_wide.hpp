@@ -260,13 +260,16 @@ __global__ __launch_bounds__(256, 2) void product_wide(const ProductArgs<T> a) {
         else copy_end(base + s * STAGE);
     }
     // Stage s has landed when at most the copies of stage s + 1 are under way; the barrier makes that true of every wave's
-    // share, and says that nobody reads stage s - 1 any more, into which stage s + 2 goes.  The loop that runs long asks nothing.
+    // share, and says that nobody reads stage s - 1 any more, into which stage s + 2 goes.  The loop that runs long asks nothing
+    // and knows its stages.
     int s = 0, stage = 0;
-    for (; s + 2 < whole; ++s) {
-        asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" ::"n"(TP::COPIES + TQ::COPIES) : "memory");
-        copy(base + (stage == 0 ? 2 : stage - 1) * STAGE);
-        multiply(lds + stage * STAGE);
-        stage = stage == 2 ? 0 : stage + 1;
+    for (; s + 4 < whole; s += 3) {
+#pragma unroll
+        for (int u = 0; u < 3; ++u) {
+            asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" ::"n"(TP::COPIES + TQ::COPIES) : "memory");
+            copy(base + (u + 2) % 3 * STAGE);
+            multiply(lds + u * STAGE);
+        }
     }
     for (; s < steps; ++s) {
         if (s + 1 < steps) asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" ::"n"(TP::COPIES + TQ::COPIES) : "memory");
@@ -277,7 +280,9 @@ __global__ __launch_bounds__(256, 2) void product_wide(const ProductArgs<T> a) {
             TQ::mend_end(lds + stage * STAGE + TP::BYTES, wave, a.q, j0, a.nj, r1, left);
             __syncthreads();
         }
-        if (s + 2 < steps) copy_end(base + (stage == 0 ? 2 : stage - 1) * STAGE);
+        const unsigned to = base + (stage == 0 ? 2 : stage - 1) * STAGE;
+        if (s + 2 < whole) copy(to);
+        else if (s + 2 < steps) copy_end(to);
         multiply(lds + stage * STAGE);
         stage = stage == 2 ? 0 : stage + 1;
     }
