@@ -11,10 +11,11 @@ namespace mpe {
 
 namespace {
 
-// Four workgroups a CU: the norm of 302 M bfloat16 elements takes 133 us at 1024 workgroups (4.5 TB/s), 140 at 2048.
+// Four workgroups a CU: the norm of 302 M bfloat16 elements takes 133 us at 1024 workgroups (4.5 TB/s), 140 at 2048.  Scaling
+// them takes 217 us (1.2 GB moved, 5.6 TB/s: part of it is still in the Infinity Cache).
 constexpr int BLOCKS = 1024;
 static_assert(BLOCKS * 8 <= MPE_CLIP_WORKSPACE_BYTES, "a partial sum for every workgroup");
-// One workgroup takes everything below this: 10 630 elements in 8.3 us, where the two launches take 7.0 us on the GPU but
+// One workgroup takes everything below this: 10 630 elements in 7.9 us, where the two launches take 7.0 us on the GPU but
 // some 4 us more of the host, which bounds calls of this size.
 constexpr int TINY = 16384;
 constexpr int CHUNK = 8192;         // elements a workgroup takes at a time

@@ -1,5 +1,6 @@
 // The forward product for a few rows (one world's agents, one decision): the weights are the traffic, and the time is that of
-// a single memory access if enough of them are in flight.
+// a single memory access if enough of them are in flight (4 x 1024 -> 4096 bf16: 8.4 MB in 3.9 us, 3 x 14 -> 64 f32 2.4 us, of
+// which an empty launch takes 1.8).
 #pragma once
 #include "mpe_linear_impl.hpp"
 
