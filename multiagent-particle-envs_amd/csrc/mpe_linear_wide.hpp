@@ -264,21 +264,22 @@ __global__ __launch_bounds__(256, 2) void product_wide(const ProductArgs<T> a) {
         if (s < whole) copy(base + s * STAGE);
         else copy_end(base + s * STAGE);
     }
-    // Stage s has landed when at most the copies of stage s + 1 are under way; the barrier makes that true of every wave's
-    // share, and says that nobody reads stage s - 1 any more, into which stage s + 2 goes.  The loop that runs long asks nothing
-    // and knows its stages.
+    // Stage s has landed when at most the copies of stage s + 1 are under way, and a wave is done with stage s - 1 when its reads
+    // have returned: the compiler leaves the last of them, and the products that want them, for after the barrier, so the wait
+    // for them stands with it.  The barrier makes both true of every wave, and stage s + 2 goes where stage s - 1 was.  The loop
+    // that runs long asks nothing and knows its stages.
     int s = 0, stage = 0;
     for (; s + 4 < whole; s += 3) {
 #pragma unroll
         for (int u = 0; u < 3; ++u) {
-            asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" ::"n"(TP::COPIES + TQ::COPIES) : "memory");
+            asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(TP::COPIES + TQ::COPIES) : "memory");
             copy(base + (u + 2) % 3 * STAGE);
             multiply(lds + u * STAGE);
         }
     }
     for (; s < steps; ++s) {
-        if (s + 1 < steps) asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" ::"n"(TP::COPIES + TQ::COPIES) : "memory");
-        else if (!left) asm volatile("s_waitcnt vmcnt(0)\n\ts_barrier" ::: "memory");
+        if (s + 1 < steps) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(TP::COPIES + TQ::COPIES) : "memory");
+        else if (!left) asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
         else {
             asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
             TP::mend_end(lds + stage * STAGE, wave, a.p, i0, a.ni, r1, left);

@@ -193,6 +193,21 @@ def test_large_products(m, k, n, ld, dt):
     check_backward(x, w, b, None, dy, "none")
 
 
+@pytest.mark.parametrize("k", [1024, 1000])
+def test_large_tiles_give_the_same_every_time(k):
+    """A stage of LDS that is overwritten before every wave has read it shows in a few elements of a few runs."""
+    import mpe_hip
+    m, n = 32768, 1024
+    x, w, b, r, dy = make(m, k, n, torch.bfloat16, residual=True)
+    q = [t.requires_grad_(True) for t in (x, w, b)]
+    first = None
+    for _ in range(24):
+        y = mpe_hip.linear(*q, "gelu", r)
+        got = (y.detach(),) + torch.autograd.grad(y, q, dy)
+        first = first or got
+        assert all(torch.equal(a, c) for a, c in zip(got, first))
+
+
 @pytest.mark.parametrize("dt", [torch.bfloat16, torch.float16])
 @pytest.mark.parametrize("act", ACTS)
 def test_every_activation_in_large_tiles(act, dt):
