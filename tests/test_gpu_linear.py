@@ -193,6 +193,26 @@ def test_large_products(m, k, n, ld, dt):
     check_backward(x, w, b, None, dy, "none")
 
 
+@pytest.mark.parametrize("m,k,n", [(1884, 817, 1), (8192, 256, 128), (5000, 70, 37), (3001, 1000, 300)])
+def test_bias_gradient_sums_what_is_not_rounded(m, k, n):
+    """Its terms cancel: float16 dz rounded before the sum would be off by up to 2^-11 of their sizes; the float32 sum and the
+    slopes of float32 pre-activations are off by the arithmetic's bound without that."""
+    import mpe_hip
+    dt = torch.float16
+    x, w, b, _, dy = make(m, k, n, dt)
+    b.requires_grad_(True)
+    db, = torch.autograd.grad(mpe_hip.linear(x, w, b, "tanh"), (b,), dy)
+    w2 = w.clone().requires_grad_(True)
+    both = torch.autograd.grad(mpe_hip.linear(x, w2, b, "tanh"), (w2, b), dy)
+    z, size, _ = forward64(x, w, b.detach(), None, "tanh")
+    d = dy.double()
+    want = (d * slope64(z, "tanh")).sum(0)
+    e = d.abs() * (0.9 * (k + 8) * V * size + 16 * V * (1 + z.abs()))
+    bound = (e.sum(0) + (m + 8) * V * (d * slope64(z, "tanh")).abs().sum(0)) * (1 + U[dt]) + U[dt] * want.abs() + TINY[dt]
+    inside(db, want, bound, "db")
+    inside(both[1], want, bound, "db beside dw")
+
+
 @pytest.mark.parametrize("k", [1024, 1000])
 def test_large_tiles_give_the_same_every_time(k):
     """A stage of LDS that is overwritten before every wave has read it shows in a few elements of a few runs."""
