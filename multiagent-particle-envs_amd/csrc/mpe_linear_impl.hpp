@@ -265,6 +265,9 @@ struct Loader {
     static constexpr int U = UNITS >= 256 ? UNITS / 256 : 1;
     static constexpr bool SOME = UNITS < 256;       // only the first UNITS threads have one
     static constexpr int PLANE = BO * BK * 2;       // bytes of one piece's tile
+    // 16-bit dz made here is two pieces, value and rest: its rounding would double the gradients' error, and the layers it is
+    // made for wait for memory anyway
+    static constexpr int PIECES = P::N == 1 && DZ ? 2 : P::N;
     static constexpr int NV = LAYOUT == R_INNER ? U : 8, W = LAYOUT == R_INNER ? 8 : U;      // vectors and their width
 
     typedef T vec __attribute__((ext_vector_type(W)));      // two 16-bit elements a register
@@ -433,6 +436,15 @@ struct Loader {
             } else {
 #pragma unroll
                 for (int e = 0; e < 8; ++e) h[e] = (PT)f[e];
+                if (PIECES == 2) {
+                    pt8 rest;
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) {
+                        const float d = f[e] - (float)h[e];
+                        rest[e] = (PT)(fabsf(d) < INFINITY ? d : 0.0f);       // of an infinity or a NaN nothing is left
+                    }
+                    *(pt8*)(to + PLANE) = rest;
+                }
             }
             *(pt8*)to = h;
         }
@@ -619,7 +631,7 @@ __global__ __launch_bounds__(256, BI * BJ > 8192 ? (Piece<T>::N == 1 && EPI == E
     constexpr int NP = P::N, BK = P::BK, FI = BI / WI / 16, FJ = BJ / WJ / 16;
     // the results pass through LDS too, ROWS rows at a time, so that they leave as whole rows from a loop of little code
     constexpr int HALVES = BI * BJ > 8192 ? 2 : 1, ROWS = BJ / HALVES, PITCH = BI + 4;
-    constexpr int TILES = NP * (LP::PLANE + LQ::PLANE), RESULTS = ROWS * PITCH * 4;
+    constexpr int NQ = LQ::PIECES, TILES = NP * LP::PLANE + NQ * LQ::PLANE, RESULTS = ROWS * PITCH * 4;
     __shared__ __attribute__((aligned(16))) char lds[TILES > RESULTS ? TILES : RESULTS];
     char* const lp = lds;
     char* const lq = lds + NP * LP::PLANE;
@@ -670,14 +682,14 @@ __global__ __launch_bounds__(256, BI * BJ > 8192 ? (Piece<T>::N == 1 && EPI == E
             constexpr int YB = FI >= 4 || FJ == 1 ? 1 : 2;
 #pragma unroll
             for (int y = 0; y < FJ; y += YB) {
-                pt8 fq[YB][NP];
+                pt8 fq[YB][NQ];
 #pragma unroll
                 for (int b = 0; b < YB; ++b)
 #pragma unroll
-                    for (int c = 0; c < NP; ++c) fq[b][c] = *(const pt8*)(lq + c * LQ::PLANE + LQ::place(wj + (y + b) * 16 + (lane & 15), kk * 4 + (lane >> 4)));
-                // float32: the partial products, smallest first
-                constexpr int PAIRS = NP == 3 ? 6 : 1;
-                constexpr int PC[6] = {NP == 3 ? 2 : 0, 0, NP / 2, NP / 2, 0, 0}, QC[6] = {0, NP - 1, NP / 2, 0, NP / 2, 0};
+                    for (int c = 0; c < NQ; ++c) fq[b][c] = *(const pt8*)(lq + c * LQ::PLANE + LQ::place(wj + (y + b) * 16 + (lane & 15), kk * 4 + (lane >> 4)));
+                // the partial products, smallest first
+                constexpr int PAIRS = NP == 3 ? 6 : NQ;
+                constexpr int PC[6] = {NP == 3 ? 2 : 0, 0, NP / 2, NP / 2, 0, 0}, QC[6] = {NP == 3 ? 0 : NQ - 1, NP - 1, NP / 2, 0, NP / 2, 0};
 #pragma unroll
                 for (int c = 0; c < PAIRS; ++c)
 #pragma unroll

@@ -55,19 +55,19 @@ __global__ __launch_bounds__(256) void slope_pass(long long m, long long n, cons
 }
 
 // The same for 16-bit types with the column sums of dz before it is rounded (the bias's gradient would see every rounding where
-// its terms cancel): a workgroup takes 256 columns of `rows` rows and leaves sums[blockIdx.y][n].  Without pre (no activation) dz
-// is dy and only the sums are made.  65 536 x 1024 bf16: 402 MB in 93 us, 4.3 TB/s.
-template <typename T>
+// its terms cancel): a workgroup takes 8 WIDE columns (WIDE up to 32, by n) of `rows` rows and leaves sums[blockIdx.y][n].  Without
+// pre (no activation) dz is dy and only the sums are made.  65 536 x 1024 bf16: 402 MB in 93 us, 4.3 TB/s.
+template <typename T, int WIDE>
 __global__ __launch_bounds__(256) void slope_sums(long long m, long long n, const T* __restrict__ dy, long long lddy, const void* __restrict__ pre,
                                                   int act, T* __restrict__ dz, int rows, float* __restrict__ sums) {
-    constexpr int E = 8;
-    __shared__ float part[8][32][E + 1];
-    const int c = threadIdx.x & 31, g = threadIdx.x >> 5;
-    const long long i = ((long long)blockIdx.x * 32 + c) * E, j1 = min((long long)(blockIdx.y + 1) * rows, m);
+    constexpr int E = 8, STEP = 256 / WIDE;
+    __shared__ float part[STEP][WIDE][E + 1];
+    const int c = threadIdx.x % WIDE, g = threadIdx.x / WIDE;
+    const long long i = ((long long)blockIdx.x * WIDE + c) * E, j1 = min((long long)(blockIdx.y + 1) * rows, m);
     float s[E] = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
     if (i + E <= n) {
 #pragma unroll 4
-        for (long long j = (long long)blockIdx.y * rows + g; j < j1; j += 8) {
+        for (long long j = (long long)blockIdx.y * rows + g; j < j1; j += STEP) {
             T d[E];
             float f[E];
             __builtin_memcpy(d, dy + j * lddy + i, sizeof(d));
@@ -94,7 +94,7 @@ __global__ __launch_bounds__(256) void slope_sums(long long m, long long n, cons
             for (int e = 0; e < E; ++e) s[e] += f[e];
         }
     } else if (i < n) {         // the last columns
-        for (long long j = (long long)blockIdx.y * rows + g; j < j1; j += 8)
+        for (long long j = (long long)blockIdx.y * rows + g; j < j1; j += STEP)
 #pragma unroll
             for (int e = 0; e < E; ++e)
                 if (i + e < n) {
@@ -111,11 +111,21 @@ __global__ __launch_bounds__(256) void slope_sums(long long m, long long n, cons
     for (int e = 0; e < E; ++e) part[g][c][e] = s[e];
     __syncthreads();
     const int col = threadIdx.x;
-    if ((long long)blockIdx.x * 256 + col < n) {
+    if (col < WIDE * E && (long long)blockIdx.x * (WIDE * E) + col < n) {
         float t = 0.0f;
-        for (int k = 0; k < 8; ++k) t += part[k][col / E][col % E];
-        sums[blockIdx.y * n + (long long)blockIdx.x * 256 + col] = t;
+        for (int k = 0; k < STEP; ++k) t += part[k][col / E][col % E];
+        sums[blockIdx.y * n + (long long)blockIdx.x * (WIDE * E) + col] = t;
     }
+}
+
+// As many columns side by side as there are: 131 072 x 128 bf16 19.4 us (dw and db together 56; 67 with 32 wherever n is).
+template <typename T, int WIDE = 32>
+inline hipError_t launch_slope_sums(long long m, long long n, const T* dy, long long lddy, const void* pre, int act, T* dz, int rows, float* sums, hipStream_t st) {
+    if constexpr (WIDE > 2) {
+        if (n <= WIDE * 4) return launch_slope_sums<T, WIDE / 2>(m, n, dy, lddy, pre, act, dz, rows, sums, st);
+    }
+    hipLaunchKernelGGL((slope_sums<T, WIDE>), dim3((unsigned)tiles_of(n, WIDE * 8), (unsigned)tiles_of(m, rows)), dim3(256), 0, st, m, n, dy, lddy, pre, act, dz, rows, sums);
+    return hipGetLastError();
 }
 
 // ---- sums of the splits: column c of [splits][ld], in the order of the splits within a group and then of the groups ----
@@ -300,9 +310,7 @@ struct LinearRun {
         float* const sums = a.db && (wide || own_sums(a.act, a.k)) ? partial + p.splits * a.n * a.k : nullptr;
         if (sums) {
             if constexpr (sizeof(T) == 2)
-                hipLaunchKernelGGL((slope_sums<T>), dim3((unsigned)tiles_of(a.n, 256), (unsigned)strips), dim3(256), 0, st, a.m, a.n, (const T*)a.dy, a.lddy,
-                                   own ? (const void*)a.pre : nullptr, act, (T*)ws, strip, sums);
-            e = hipGetLastError();
+                e = launch_slope_sums<T>(a.m, a.n, (const T*)a.dy, a.lddy, own ? (const void*)a.pre : nullptr, act, (T*)ws, strip, sums, st);
         } else if (own && a.lddy == a.n) {
             const long long want = (a.m * a.n + 2047) / 2048;
             hipLaunchKernelGGL((slope_flat<T>), dim3((unsigned)(want < 8192 ? want : 8192)), dim3(256), 0, st, a.m * a.n, (const T*)a.dy, (const void*)a.pre, act, (T*)ws);
