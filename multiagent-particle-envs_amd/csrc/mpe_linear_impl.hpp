@@ -741,7 +741,7 @@ __global__ __launch_bounds__(256, BI * BJ > 8192 ? (Piece<T>::N == 1 && EPI == E
         if (have > 0)
             finish_rows<T, EPI, 4, 1024 / BI>(a, split, i, j0 + half * ROWS, threadIdx.x / (BI / 4), rows, mask, bias, [&](int jt, float* f) {
                 *(f32x4*)f = *(const f32x4*)&res[jt * PITCH + it];
-                if (NP == 3) {
+                if (NP == 3 || NQ == 2) {       // an infinity times a piece of zero
 #pragma unroll
                     for (int e = 0; e < 4; ++e)
                         if (!(fabsf(f[e]) < INFINITY) && e < have) f[e] = plain_sum<T, PL, QL, DZ>(a.p, a.q, i + e, j0 + half * ROWS + jt, r0, r1);

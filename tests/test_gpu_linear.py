@@ -389,6 +389,31 @@ def test_infinities_and_nan_stay_in_their_rows(dt, m, k, n):
     assert torch.equal(got[rows], mpe_hip.linear(x, w2, b)[rows]) and not torch.isnan(clean).any()
 
 
+@pytest.mark.parametrize("dt", DTYPES)
+@pytest.mark.parametrize("k", [12, 40, 96])
+def test_gradients_of_infinite_inputs_and_weights_are_infinite(k, dt):
+    """One infinity in x or w: where it meets a dz that is not zero the gradient is infinite, not NaN, and elsewhere finite."""
+    import mpe_hip
+    m, n = 70, 24
+    x, w, b, _, dy = make(m, k, n, dt)
+    dy = dy.abs() + 0.5                                  # exact in no type's second piece, never zero
+    dy[:, ::2] *= -1
+    w = w.abs() + 0.25
+    x = x.abs() + 0.25
+    for t, at in ((x, (3, 2)), (w, (1, 0))):
+        q = [x.clone(), w.clone()]
+        q[0 if t is x else 1][at] = math.inf
+        q = [t.requires_grad_(True) for t in q]
+        dx, dw = torch.autograd.grad(mpe_hip.linear(q[0], q[1], None, "relu"), q, dy)
+        if t is x:
+            assert torch.equal(dw[:, 2].float(), torch.copysign(torch.full((n,), math.inf, device=DEV), dy[3].float()))
+            keep = [c for c in range(k) if c != 2]
+            assert torch.isfinite(dx).all() and torch.isfinite(dw[:, keep]).all()
+        else:
+            assert torch.equal(dx[:, 0].float(), torch.copysign(torch.full((m,), math.inf, device=DEV), dy[:, 1].float()))
+            assert torch.isfinite(dw).all() and torch.isfinite(dx[:, 1:]).all()
+
+
 def test_float32_extremes():
     """The largest and the smallest float32 go through products and come out as float32 would have them."""
     import mpe_hip
