@@ -459,7 +459,7 @@ int mpe_linear_forward(int device, int dtype, int activation, int64_t m, int64_t
  * The residual's gradient is dy itself.  dx, dw, db: NULL for what is not wanted.  `pre` is what the forward wrote
  * (for MPE_ACT_RELU any T[m][n] with the same signs will do, e.g. y where there was no residual; with
  * MPE_ACT_TANH_OUT, which only this pass knows and only for MPE_F32, it is tanh(x w^T + bias)); NULL with MPE_ACT_NONE.
- * With 16-bit types and k above 64 dz is rounded to T for dx and dw; db sums it before.
+ * With 16-bit types dz enters dx and dw as two numbers of T, value and rest, so that a gradient is rounded once; db sums it before.
  * The outputs must not overlap each other or an input.  Sums do not change their order from run to run.
  */
 int mpe_linear_backward(int device, int dtype, int activation, int64_t m, int64_t n, int64_t k, const void* dy, int64_t lddy, const void* x,

@@ -206,18 +206,35 @@ __device__ inline void split3(const F& f, bf16x8& h, bf16x8& m, bf16x8& l) {
     l = __builtin_bit_cast(bf16x8, p[2]);
 }
 
+// 16-bit dz enters a product as two pieces, value and rest: rounded to one it would add as much to the gradients' error again
+// as their own rounding does.  The rests are summed apart, so that an infinity of the other operand, which times a rest of zero
+// is NaN, spoils only what is then left out: the values alone tell what such a sum is.
+template <typename T>
+__device__ inline void split2(float f, T& h, T& rest) {
+    // f as it is: the compiler folds the product that made it into its rounding to float16 (one rounding instead of two), but not
+    // where it becomes a float again, and next to a tie the rest would belong to another h
+    asm("" : "+v"(f));
+    h = (T)f;
+    const float d = f - (float)h;
+    rest = (T)(fabsf(d) < INFINITY ? d : 0.0f);         // of an infinity or a NaN nothing is left
+}
+__device__ inline float join2(float sum, float rests) { return fabsf(rests) < INFINITY ? sum + rests : sum; }
+
 // ---- operands ----
 enum { R_INNER, O_INNER };      // which index is contiguous in memory: the summed one, or the output's
+// what an operand is read from: its matrix; dy and what the forward pass kept (data * slope(pre)); or dz in two pieces, rows of
+// the values and `rest` elements behind them of the rests
+enum { SRC_PLAIN, SRC_DZ, SRC_SPLIT };
 
-// an operand's matrix; with DZ, what is read is data * slope(pre)
 template <typename T>
 struct Operand {
     const T* data;
-    long long ld;               // may be 0 with DZ: one row for all
-    long long extent;           // elements from the first to behind the last, at least 8
+    long long ld;               // may be 0 with SRC_DZ: one row for all
+    long long extent;           // elements from the first to behind the last, at least 8 (SRC_SPLIT: of the values' last row, and at least 8 more)
     const void* pre;            // [rows][ld_pre], what the forward pass kept, or null: slope 1
     long long ld_pre, extent_pre;
     int act;
+    long long rest;
 };
 
 __device__ inline bool small_pre(int act) { return act == MPE_ACT_RELU || act == ACT_SLOPE; }
@@ -256,23 +273,23 @@ __device__ inline void shift_down(V& v, int by) {
 // by naming registers differently.  Loads ask nothing: they take whatever lies in the vector's place.  Only in the steps
 // that reach the end of the sum or of the matrix does a Window keep them inside it, and fix() puts the elements into their
 // places and zeros where the sum has ended; rows and columns of the output that do not exist may hold anything.
-template <typename T, int BO, int LAYOUT, bool DZ>
+template <typename T, int BO, int LAYOUT, int SRC>
 struct Loader {
     typedef Piece<T> P;
+    static constexpr bool DZ = SRC == SRC_DZ, SPLIT = SRC == SRC_SPLIT;
     typedef typename P::type PT;
     typedef PT pt8 __attribute__((ext_vector_type(8)));
     static constexpr int BK = P::BK, CH = BK / 8, UNITS = BO * CH;
     static constexpr int U = UNITS >= 256 ? UNITS / 256 : 1;
     static constexpr bool SOME = UNITS < 256;       // only the first UNITS threads have one
     static constexpr int PLANE = BO * BK * 2;       // bytes of one piece's tile
-    // 16-bit dz made here is two pieces, value and rest: its rounding would double the gradients' error, and the layers it is
-    // made for wait for memory anyway
-    static constexpr int PIECES = P::N == 1 && DZ ? 2 : P::N;
+    static constexpr int PIECES = P::N == 1 && SRC != SRC_PLAIN ? 2 : P::N;
+    static_assert(!SPLIT || P::N == 1, "float32 dz is one number");
     static constexpr int NV = LAYOUT == R_INNER ? U : 8, W = LAYOUT == R_INNER ? 8 : U;      // vectors and their width
 
     typedef T vec __attribute__((ext_vector_type(W)));      // two 16-bit elements a register
     typedef float zvec __attribute__((ext_vector_type(W)));
-    vec v[NV];
+    vec v[NV], rest[SPLIT ? NV : 1];
     zvec z[DZ ? NV : 1];
 
     // What stays the same from step to step: the vectors' offsets within the tile and, uniform, the place of the next step
@@ -323,6 +340,7 @@ struct Loader {
 #pragma unroll
                 for (int i = 0; i < NV; ++i) {
                     __builtin_memcpy(&v[i], p + off[LAYOUT == R_INNER ? i : 0], W * sizeof(T));
+                    if (SPLIT) __builtin_memcpy(&rest[i], p + op.rest * (long long)sizeof(T) + off[LAYOUT == R_INNER ? i : 0], W * sizeof(T));
                     if (LAYOUT == O_INNER) p += row_bytes;
                 }
                 if (DZ && op.pre) {
@@ -357,7 +375,11 @@ struct Loader {
         const Window w(op.extent, first(o0, r0, op.ld), W);
         const char* base = (const char*)(op.data + w.base);
 #pragma unroll
-        for (int i = 0; i < NV; ++i) __builtin_memcpy(&v[i], base + w.at(offset(i, (unsigned)op.ld, left_o)) * (unsigned)sizeof(T), W * sizeof(T));
+        for (int i = 0; i < NV; ++i) {
+            const unsigned at = w.at(offset(i, (unsigned)op.ld, left_o)) * (unsigned)sizeof(T);
+            __builtin_memcpy(&v[i], base + at, W * sizeof(T));
+            if (SPLIT) __builtin_memcpy(&rest[i], base + op.rest * (long long)sizeof(T) + at, W * sizeof(T));
+        }
         if (DZ && op.pre) {
             const Window wp(op.extent_pre, first(o0, r0, op.ld_pre), W);
             if (small_pre(op.act)) {
@@ -385,7 +407,10 @@ struct Loader {
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
             const int by = w.moved(offset(i, (unsigned)op.ld, left_o));
-            if (by > 0 && by < W) shift_down<W>(v[i], by);
+            if (by > 0 && by < W) {
+                shift_down<W>(v[i], by);
+                if (SPLIT) shift_down<W>(rest[i], by);
+            }
             if (DZ && op.pre) {
                 const int byp = wp.moved(offset(i, (unsigned)op.ld_pre, left_o));
                 if (byp > 0 && byp < W) shift_down<W>(z[i], byp);
@@ -394,6 +419,7 @@ struct Loader {
             for (int e = 0; e < W; ++e) {
                 const bool in = (LAYOUT == R_INNER ? chunk_of(i) * 8 + e : chunk_of(0) * 8 + i) < left_r;
                 v[i][e] = in ? v[i][e] : (T)0.0f;
+                if (SPLIT) rest[i][e] = in ? rest[i][e] : (T)0.0f;
                 if (DZ) z[i][e] = in ? z[i][e] : 0.0f;
             }
         }
@@ -415,6 +441,11 @@ struct Loader {
 #pragma unroll
                 for (int e = 0; e < 8; ++e) h[e] = LAYOUT == R_INNER ? (PT)v[u][e] : (PT)v[e][u];
                 *(pt8*)to = h;
+                if (SPLIT) {
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) h[e] = LAYOUT == R_INNER ? (PT)rest[u][e] : (PT)rest[e][u];
+                    *(pt8*)(to + PLANE) = h;
+                }
                 continue;
             }
             float f[8];
@@ -433,18 +464,19 @@ struct Loader {
                 split3(f, h, m, l);
                 *(pt8*)(to + PLANE) = m;
                 *(pt8*)(to + 2 * PLANE) = l;
+            } else if constexpr (PIECES == 2) {
+                pt8 r;
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    PT one, two;
+                    split2<PT>(f[e], one, two);
+                    h[e] = one;
+                    r[e] = two;
+                }
+                *(pt8*)(to + PLANE) = r;
             } else {
 #pragma unroll
                 for (int e = 0; e < 8; ++e) h[e] = (PT)f[e];
-                if (PIECES == 2) {
-                    pt8 rest;
-#pragma unroll
-                    for (int e = 0; e < 8; ++e) {
-                        const float d = f[e] - (float)h[e];
-                        rest[e] = (PT)(fabsf(d) < INFINITY ? d : 0.0f);       // of an infinity or a NaN nothing is left
-                    }
-                    *(pt8*)(to + PLANE) = rest;
-                }
             }
             *(pt8*)to = h;
         }
@@ -590,8 +622,9 @@ __device__ inline void finish_rows(const ProductArgs<T>& a, unsigned split, long
 
 // Operands of fewer than eight elements, for which there is no vector to load: a thread an element of the output, whose sum
 // then has fewer than eight terms (of an expanded dy: as many as there are rows).
-template <typename T, int EPI, int PL, int QL, bool DZ>
+template <typename T, int EPI, int PL, int QL, int SRC>
 __global__ __launch_bounds__(256) void product_few(const ProductArgs<T> a, int splits) {
+    constexpr bool DZ = SRC == SRC_DZ;
     const long long n = a.ni * a.nj * splits;
     for (long long at = (long long)blockIdx.x * 256 + threadIdx.x; at < n; at += (long long)gridDim.x * 256) {
         const long long i = at % a.ni, j = at / a.ni % a.nj;
@@ -621,17 +654,26 @@ __device__ inline unsigned xcd_run(unsigned b, unsigned n) {
     return x * q + (x < r ? x : r) + b / 8;
 }
 
-template <typename T, int EPI, int PL, int QL, bool DZ, int BI, int BJ, int WI, int WJ>
-__global__ __launch_bounds__(256, BI * BJ > 8192 ? (Piece<T>::N == 1 && EPI == EPI_PARTIAL ? 3 : 2) : BI * BJ > 4096 ? 3 : 4) void product(const ProductArgs<T> a) {
+// Workgroups that a CU's registers are shared among.  Two 16-bit pieces have two sums: one workgroup fewer, where registers would
+// be kept in memory otherwise.
+constexpr int groups_a_cu(int pieces, int epi, int src, int tile) {
+    const bool two = pieces == 1 && src != SRC_PLAIN;
+    if (tile > 8192) return pieces == 1 && epi == EPI_PARTIAL ? 3 : 2;
+    return tile > 4096 ? (two ? 2 : 3) : two ? 3 : 4;
+}
+
+template <typename T, int EPI, int PL, int QL, int SRC, int BI, int BJ, int WI, int WJ>
+__global__ __launch_bounds__(256, groups_a_cu(Piece<T>::N, EPI, SRC, BI * BJ)) void product(const ProductArgs<T> a) {
     typedef Piece<T> P;
     typedef typename P::type PT;
     typedef PT pt8 __attribute__((ext_vector_type(8)));
-    typedef Loader<T, BI, PL, false> LP;
-    typedef Loader<T, BJ, QL, DZ> LQ;
-    constexpr int NP = P::N, BK = P::BK, FI = BI / WI / 16, FJ = BJ / WJ / 16;
+    typedef Loader<T, BI, PL, SRC_PLAIN> LP;
+    typedef Loader<T, BJ, QL, SRC> LQ;
+    constexpr bool DZ = SRC == SRC_DZ;
+    constexpr int NP = P::N, NQ = LQ::PIECES, BK = P::BK, FI = BI / WI / 16, FJ = BJ / WJ / 16;
     // the results pass through LDS too, ROWS rows at a time, so that they leave as whole rows from a loop of little code
     constexpr int HALVES = BI * BJ > 8192 ? 2 : 1, ROWS = BJ / HALVES, PITCH = BI + 4;
-    constexpr int NQ = LQ::PIECES, TILES = NP * LP::PLANE + NQ * LQ::PLANE, RESULTS = ROWS * PITCH * 4;
+    constexpr int TILES = NP * LP::PLANE + NQ * LQ::PLANE, RESULTS = ROWS * PITCH * 4;
     __shared__ __attribute__((aligned(16))) char lds[TILES > RESULTS ? TILES : RESULTS];
     char* const lp = lds;
     char* const lq = lds + NP * LP::PLANE;
@@ -642,11 +684,14 @@ __global__ __launch_bounds__(256, BI * BJ > 8192 ? (Piece<T>::N == 1 && EPI == E
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const int wi = (wave % WI) * (BI / WI), wj = (wave / WI) * (BJ / WJ);
 
-    f32x4 acc[FI][FJ];
+    f32x4 acc[FI][FJ], rests[NQ == 2 ? FI : 1][NQ == 2 ? FJ : 1];
 #pragma unroll
     for (int x = 0; x < FI; ++x)
 #pragma unroll
-        for (int y = 0; y < FJ; ++y) acc[x][y] = 0.0f;
+        for (int y = 0; y < FJ; ++y) {
+            acc[x][y] = 0.0f;
+            if constexpr (NQ == 2) rests[x][y] = 0.0f;
+        }
     float sums[LQ::U];
 #pragma unroll
     for (int u = 0; u < LQ::U; ++u) sums[u] = 0.0f;
@@ -687,19 +732,34 @@ __global__ __launch_bounds__(256, BI * BJ > 8192 ? (Piece<T>::N == 1 && EPI == E
                 for (int b = 0; b < YB; ++b)
 #pragma unroll
                     for (int c = 0; c < NQ; ++c) fq[b][c] = *(const pt8*)(lq + c * LQ::PLANE + LQ::place(wj + (y + b) * 16 + (lane & 15), kk * 4 + (lane >> 4)));
-                // the partial products, smallest first
-                constexpr int PAIRS = NP == 3 ? 6 : NQ;
-                constexpr int PC[6] = {NP == 3 ? 2 : 0, 0, NP / 2, NP / 2, 0, 0}, QC[6] = {NP == 3 ? 0 : NQ - 1, NP - 1, NP / 2, 0, NP / 2, 0};
+                // float32's partial products, smallest first
+                constexpr int PAIRS = NP == 3 ? 6 : 1;
+                constexpr int PC[6] = {NP == 3 ? 2 : 0, 0, NP / 2, NP / 2, 0, 0}, QC[6] = {0, NP - 1, NP / 2, 0, NP / 2, 0};
 #pragma unroll
                 for (int c = 0; c < PAIRS; ++c)
 #pragma unroll
                     for (int b = 0; b < YB; ++b)
 #pragma unroll
                         for (int x = 0; x < FI; ++x) acc[x][y + b] = mfma(fp[x][PC[c]], fq[b][QC[c]], acc[x][y + b]);
+                if constexpr (NQ == 2) {
+#pragma unroll
+                    for (int b = 0; b < YB; ++b)
+#pragma unroll
+                        for (int x = 0; x < FI; ++x) rests[x][y + b] = mfma(fp[x][0], fq[b][1], rests[x][y + b]);
+                }
             }
         }
         if (NP == 3) __builtin_amdgcn_s_setprio(0);
         __syncthreads();
+    }
+
+    if constexpr (NQ == 2) {
+#pragma unroll
+        for (int x = 0; x < FI; ++x)
+#pragma unroll
+            for (int y = 0; y < FJ; ++y)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) acc[x][y][e] = join2(acc[x][y][e], rests[x][y][e]);
     }
 
     // column sums: the threads that hold the same columns add up through LDS, in the order of their rows
@@ -741,7 +801,7 @@ __global__ __launch_bounds__(256, BI * BJ > 8192 ? (Piece<T>::N == 1 && EPI == E
         if (have > 0)
             finish_rows<T, EPI, 4, 1024 / BI>(a, split, i, j0 + half * ROWS, threadIdx.x / (BI / 4), rows, mask, bias, [&](int jt, float* f) {
                 *(f32x4*)f = *(const f32x4*)&res[jt * PITCH + it];
-                if (NP == 3 || NQ == 2) {       // an infinity times a piece of zero
+                if (NP == 3) {          // an infinity times a piece of zero
 #pragma unroll
                     for (int e = 0; e < 4; ++e)
                         if (!(fabsf(f[e]) < INFINITY) && e < have) f[e] = plain_sum<T, PL, QL, DZ>(a.p, a.q, i + e, j0 + half * ROWS + jt, r0, r1);

@@ -12,8 +12,12 @@ inline long long tiles_of(long long n, int b) { return (n + b - 1) / b; }
 // workgroups of 256 threads that a grid dimension holds: their threads are counted in 32 bits
 constexpr int MAX_GROUPS = 0xffffff;
 
-// ---- dz = dy f'(pre) as an array of its own ----
-// dense dy: eight elements a thread, whatever the rows' length
+// ---- dz = dy f'(pre) as an array of its own: in float32 [m][n], in 16-bit types two pieces (split2), [m][2][n], and eight elements
+// behind the last ----
+template <typename T>
+inline long long dz_elements(long long m, long long n) { return sizeof(T) == 2 ? m * n * 2 + 8 : m * n; }
+
+// float32, dense dy: eight elements a thread, whatever the rows' length
 template <typename T>
 __global__ __launch_bounds__(256) void slope_flat(long long total, const T* __restrict__ dy, const void* __restrict__ pre, int act, T* __restrict__ dz) {
     typedef T vec8 __attribute__((ext_vector_type(8)));
@@ -43,7 +47,7 @@ __global__ __launch_bounds__(256) void slope_flat(long long total, const T* __re
     }
 }
 
-// any dy
+// float32, any dy
 template <typename T>
 __global__ __launch_bounds__(256) void slope_pass(long long m, long long n, const T* __restrict__ dy, long long lddy, const void* __restrict__ pre,
                                                   int act, T* __restrict__ dz) {
@@ -54,9 +58,9 @@ __global__ __launch_bounds__(256) void slope_pass(long long m, long long n, cons
     }
 }
 
-// The same for 16-bit types with the column sums of dz before it is rounded (the bias's gradient would see every rounding where
-// its terms cancel): a workgroup takes 8 WIDE columns (WIDE up to 32, by n) of `rows` rows and leaves sums[blockIdx.y][n].  Without
-// pre (no activation) dz is dy and only the sums are made.  65 536 x 1024 bf16: 402 MB in 93 us, 4.3 TB/s.
+// The same for 16-bit types, with the column sums of dz before it is rounded (the bias's gradient would see every rounding where
+// its terms cancel): a workgroup takes 8 WIDE columns (WIDE up to 32, by n) of `rows` rows and leaves sums[blockIdx.y][n], where
+// sums are wanted.  Without pre (no activation) dz is dy and only the sums are made.
 template <typename T, int WIDE>
 __global__ __launch_bounds__(256) void slope_sums(long long m, long long n, const T* __restrict__ dy, long long lddy, const void* __restrict__ pre,
                                                   int act, T* __restrict__ dz, int rows, float* __restrict__ sums) {
@@ -75,6 +79,7 @@ __global__ __launch_bounds__(256) void slope_sums(long long m, long long n, cons
             for (int e = 0; e < E; ++e) f[e] = (float)d[e];
             if (pre) {
                 float z[E];
+                T rest[E];
                 if (small_pre(act)) {
                     T t[E];
                     __builtin_memcpy(t, (const T*)pre + j * n + i, sizeof(t));
@@ -86,9 +91,10 @@ __global__ __launch_bounds__(256) void slope_sums(long long m, long long n, cons
 #pragma unroll
                 for (int e = 0; e < E; ++e) {
                     f[e] *= act_slope(act, z[e]);
-                    d[e] = (T)f[e];
+                    split2(f[e], d[e], rest[e]);
                 }
-                __builtin_memcpy(dz + j * n + i, d, sizeof(d));
+                __builtin_memcpy(dz + j * n * 2 + i, d, sizeof(d));
+                __builtin_memcpy(dz + j * n * 2 + n + i, rest, sizeof(rest));
             }
 #pragma unroll
             for (int e = 0; e < E; ++e) s[e] += f[e];
@@ -102,11 +108,12 @@ __global__ __launch_bounds__(256) void slope_sums(long long m, long long n, cons
                     if (pre) {
                         const long long at = j * n + i + e;
                         f *= act_slope(act, small_pre(act) ? kept_small<T>(act, ((const T*)pre)[at]) : ((const float*)pre)[at]);
-                        dz[at] = (T)f;
+                        split2(f, dz[j * n * 2 + i + e], dz[j * n * 2 + n + i + e]);
                     }
                     s[e] += f;
                 }
     }
+    if (!sums) return;
 #pragma unroll
     for (int e = 0; e < E; ++e) part[g][c][e] = s[e];
     __syncthreads();
@@ -176,35 +183,41 @@ inline hipError_t launch_add_splits(const float* partial, int splits, long long 
 }
 
 
-template <typename T, int EPI, int PL, int QL, bool DZ, int BI, int BJ, int WI, int WJ>
+template <typename T, int EPI, int PL, int QL, int SRC, int BI, int BJ, int WI, int WJ>
 inline hipError_t launch_product(ProductArgs<T> a, int splits, hipStream_t st) {
     const long long ti = tiles_of(a.ni, BI), tiles = ti * tiles_of(a.nj, BJ);
     if (tiles * splits > MAX_GROUPS) return hipErrorInvalidValue;       // the callers' limits on sizes keep it from happening
-    if (a.p.extent < 8 || a.q.extent < 8 || (a.q.pre && a.q.extent_pre < 8)) {
-        const long long want = (a.ni * a.nj * splits + 255) / 256;
-        hipLaunchKernelGGL((product_few<T, EPI, PL, QL, DZ>), dim3((unsigned)(want < 8192 ? want : 8192)), dim3(256), 0, st, a, splits);
-        return hipGetLastError();
+    if constexpr (SRC != SRC_SPLIT) {       // own_dz: the other operand has more than 64 elements
+        if (a.p.extent < 8 || a.q.extent < 8 || (a.q.pre && a.q.extent_pre < 8)) {
+            const long long want = (a.ni * a.nj * splits + 255) / 256;
+            hipLaunchKernelGGL((product_few<T, EPI, PL, QL, SRC>), dim3((unsigned)(want < 8192 ? want : 8192)), dim3(256), 0, st, a, splits);
+            return hipGetLastError();
+        }
     }
     a.ti = (int)ti;
     a.tiles = (unsigned)tiles;
-    hipLaunchKernelGGL((product<T, EPI, PL, QL, DZ, BI, BJ, WI, WJ>), dim3((unsigned)(tiles * splits)), dim3(256), 0, st, a);
+    hipLaunchKernelGGL((product<T, EPI, PL, QL, SRC, BI, BJ, WI, WJ>), dim3((unsigned)(tiles * splits)), dim3(256), 0, st, a);
     return hipGetLastError();
 }
 
 // Tiles of the products that write rows of m.  16-bit types that fill every CU with a wide tile: product_wide (65 536 x 1024 ->
-// 1024 bf16 155 us against 199 forward and 145 against 208 for dx; with 128 wide tiles both take 21 us, with 64 it is 20 against
-// 13).  Others by the output's width.  Up to 64 columns: 64 x 64 (196 608 x 64 -> 64 f32 28.4 us
+// 1024 bf16 155 us against 199 forward; dz in two pieces and dx 350 against 467, 16 384 x 512 -> 256, 256 tiles, 44 against 46; with
+// 128 wide tiles a forward pass takes 21 us both ways, with 64 it is 20 against 13).  Others by the output's width.  Up to 64 columns: 64 x 64 (196 608 x 64 -> 64 f32 28.4 us
 // forward and 35.4 for dx, against 30.4 and 36.5 with 64 x 128).
-template <typename T, int EPI, int PL, int QL, bool DZ>
+template <typename T, int EPI, int PL, int QL, int SRC>
 inline hipError_t launch_rows(const ProductArgs<T>& a, hipStream_t st) {
-    if constexpr (sizeof(T) == 2 && !DZ) {
-        if (a.nr >= 64 && tiles_of(a.ni, Wide::BI) * tiles_of(a.nj, Wide::BJ) >= 256 && a.ni > 64 && wide_operand(a.p, PL, a.ni) && wide_operand(a.q, QL, a.nj))
-            return launch_product_wide<T, EPI, PL, QL>(a, 1, st);
+    if constexpr (sizeof(T) == 2 && SRC != SRC_DZ) {
+        constexpr bool SPLIT = SRC == SRC_SPLIT;
+        if (a.nr >= 64 && tiles_of(a.ni, Wide::BI) * tiles_of(a.nj, SPLIT ? Wide::BJ / 2 : Wide::BJ) >= 256 && a.ni > 64 && wide_operand(a.p, PL, a.ni) &&
+            wide_operand(a.q, QL, a.nj))
+            return launch_product_wide<T, EPI, PL, QL, SPLIT>(a, 1, st);
     }
-    if (a.ni <= 16) return launch_product<T, EPI, PL, QL, DZ, 16, 128, 1, 4>(a, 1, st);
-    if (a.ni <= 64 || tiles_of(a.ni, 128) * tiles_of(a.nj, 128) < 256) return launch_product<T, EPI, PL, QL, DZ, 64, 64, 2, 2>(a, 1, st);
-    if constexpr (!DZ) return launch_product<T, EPI, PL, QL, DZ, 128, 128, 2, 2>(a, 1, st);
-    return hipErrorInvalidValue;        // own_dz: with DZ there are at most 64 columns
+    if constexpr (SRC != SRC_SPLIT) {       // own_dz: with SRC_SPLIT there are more than 64 columns, with SRC_DZ at most
+        if (a.ni <= 16) return launch_product<T, EPI, PL, QL, SRC, 16, 128, 1, 4>(a, 1, st);
+    }
+    if (a.ni <= 64 || tiles_of(a.ni, 128) * tiles_of(a.nj, 128) < 256) return launch_product<T, EPI, PL, QL, SRC, 64, 64, 2, 2>(a, 1, st);
+    if constexpr (SRC != SRC_DZ) return launch_product<T, EPI, PL, QL, SRC, 128, SRC == SRC_SPLIT ? 64 : 128, 2, 2>(a, 1, st);
+    return hipErrorInvalidValue;
 }
 
 // Weight gradients: the sum over m is long and the output small, so it is split over workgroups that leave float32 partial
@@ -214,11 +227,11 @@ struct WeightPlan {
     int bi, bj, splits;
     long long r_split;
 };
-inline WeightPlan weight_plan(int bk, bool wide, long long m, long long n, long long k) {
+inline WeightPlan weight_plan(int bk, bool wide, bool split, long long m, long long n, long long k) {
     WeightPlan p;
     p.wide = wide;
     if (wide) {
-        const long long tiles = tiles_of(k, Wide::BI) * tiles_of(n, Wide::BJ);
+        const long long tiles = tiles_of(k, Wide::BI) * tiles_of(n, split ? Wide::BJ / 2 : Wide::BJ);
         long long s = 512 / tiles;        // two workgroups a CU
         if (s > tiles_of(m, 512)) s = tiles_of(m, 512);
         if (s < 1) s = 1;
@@ -227,7 +240,7 @@ inline WeightPlan weight_plan(int bk, bool wide, long long m, long long n, long 
         return p;
     }
     p.bi = k <= 16 ? 16 : n <= 16 || k <= 64 || n <= 64 ? 64 : 128;
-    p.bj = p.bi == 128 ? 128 : p.bi == 64 && n <= 16 ? 16 : 64;
+    p.bj = p.bi == 128 ? (split ? 64 : 128) : p.bi == 64 && n <= 16 ? 16 : 64;
     const long long tiles = tiles_of(k, p.bi) * tiles_of(n, p.bj);
     // four workgroups a CU (64/64 f32 over 196 608 rows, product and sum of the splits: 38.6 us at 1024 workgroups, 41.2 at
     // 768, 46.0 at 512)
@@ -241,7 +254,8 @@ inline WeightPlan weight_plan(int bk, bool wide, long long m, long long n, long 
 }
 
 // Large weight gradients of 16-bit types, if the operands' addresses allow it too (wide_operand): 65 536 x 1024 -> 1024 bf16
-// with the bias's 145 us against 233; below, the tiles that split more finely are as fast or faster (4096 x 256 -> 256).
+// with the bias's 145 us against 233, dz in two pieces and dw 335 against 488; 4096 x 256 -> 256 takes 39 both ways, below the tiles
+// that split more finely are as fast or faster.
 inline bool wide_weights(int size, long long m, long long n, long long k) {
     return size == 2 && k >= 256 && n >= 128 && k % 8 == 0 && n % 8 == 0 && m >= 4096;
 }
@@ -257,22 +271,22 @@ inline long long round_up(long long n) { return (n + 255) / 256 * 256; }
 
 template <typename T>
 struct LinearRun {
-    // dz as an array of its own is rounded: its column sums are taken while it is made
-    static bool own_sums(int act, long long k) { return sizeof(T) == 2 && own_dz(act, k); }
+    // dz as an array of its own in 16-bit types: its column sums are taken while it is made
+    static bool split_dz(int act, long long k) { return sizeof(T) == 2 && own_dz(act, k); }
 
     static long long backward_workspace(int act, long long m, long long n, long long k) {
         if (m == 0) return 0;
-        const WeightPlan p = weight_plan(Piece<T>::BK, false, m, n, k);
+        const WeightPlan p = weight_plan(Piece<T>::BK, false, split_dz(act, k), m, n, k);
         const long long strips = tiles_of(m, strip_rows(m)) * n;
-        long long sums = p.splits * n * k + (own_sums(act, k) ? strips : p.splits * n);
-        if (wide_weights(sizeof(T), m, n, k)) sums = std::max(sums, weight_plan(Piece<T>::BK, true, m, n, k).splits * n * k + strips);
-        return (own_dz(act, k) ? round_up(m * n * (long long)sizeof(T)) : 0) + sums * 4;
+        long long sums = p.splits * n * k + (split_dz(act, k) ? strips : p.splits * n);
+        if (wide_weights(sizeof(T), m, n, k)) sums = std::max(sums, weight_plan(Piece<T>::BK, true, split_dz(act, k), m, n, k).splits * n * k + strips);
+        return (own_dz(act, k) ? round_up(dz_elements<T>(m, n) * (long long)sizeof(T)) : 0) + sums * 4;
     }
 
     static hipError_t forward(const LinearArgs& a, hipStream_t st) {
         ProductArgs<T> g = {};
-        g.p = {(const T*)a.w, a.ldw, (a.n - 1) * a.ldw + a.k, nullptr, 0, 0, 0};
-        g.q = {(const T*)a.x, a.ldx, (a.m - 1) * a.ldx + a.k, nullptr, 0, 0, 0};
+        g.p = {(const T*)a.w, a.ldw, (a.n - 1) * a.ldw + a.k, nullptr, 0, 0, 0, 0};
+        g.q = {(const T*)a.x, a.ldx, (a.m - 1) * a.ldx + a.k, nullptr, 0, 0, 0, 0};
         g.ni = a.n; g.nj = a.m; g.nr = a.k;
         g.out = (T*)a.y; g.ldo = a.ldy;
         g.bias = (const T*)a.bias; g.residual = (const T*)a.residual; g.ldr = a.ldr; g.pre = a.act != MPE_ACT_NONE ? a.pre : nullptr; g.act = a.act;
@@ -280,17 +294,19 @@ struct LinearRun {
         // -> 4096 bf16: 3.9 us against 14.1 in tiles; 2048 x 64 -> 64 f32 3.7 against 7.0; with 512 workgroups 1024 x 258 ->
         // 512 f32 10.4 against 13.6, 512 x 1024 -> 1024 bf16 12.6 against 11.4; with 1024 of them 10.9 against 7.6).
         if ((a.m <= 16 || tiles_of(a.m, 64) * tiles_of(a.n, 16) <= 512) && g.p.extent >= 8 && g.q.extent >= 8) return launch_forward_skinny<T>(g, st);
-        return launch_rows<T, EPI_FORWARD, R_INNER, R_INNER, false>(g, st);
+        return launch_rows<T, EPI_FORWARD, R_INNER, R_INNER, SRC_PLAIN>(g, st);
     }
 
-    template <bool DZ>
+    template <int SRC>
     static hipError_t weights(const ProductArgs<T>& g, const WeightPlan& p, hipStream_t st) {
-        if constexpr (!DZ) {        // own_dz: with DZ k is at most 64
-            if (p.bi == 128) return launch_product<T, EPI_PARTIAL, O_INNER, O_INNER, DZ, 128, 128, 2, 2>(g, p.splits, st);
+        if constexpr (SRC != SRC_DZ) {      // own_dz: with SRC_DZ k is at most 64
+            if (p.bi == 128) return launch_product<T, EPI_PARTIAL, O_INNER, O_INNER, SRC, 128, SRC == SRC_SPLIT ? 64 : 128, 2, 2>(g, p.splits, st);
         }
-        if (p.bi == 16) return launch_product<T, EPI_PARTIAL, O_INNER, O_INNER, DZ, 16, 64, 1, 4>(g, p.splits, st);
-        if (p.bj == 16) return launch_product<T, EPI_PARTIAL, O_INNER, O_INNER, DZ, 64, 16, 4, 1>(g, p.splits, st);
-        return launch_product<T, EPI_PARTIAL, O_INNER, O_INNER, DZ, 64, 64, 2, 2>(g, p.splits, st);
+        if constexpr (SRC != SRC_SPLIT) {   // and with SRC_SPLIT above
+            if (p.bi == 16) return launch_product<T, EPI_PARTIAL, O_INNER, O_INNER, SRC, 16, 64, 1, 4>(g, p.splits, st);
+        }
+        if (p.bj == 16) return launch_product<T, EPI_PARTIAL, O_INNER, O_INNER, SRC, 64, 16, 4, 1>(g, p.splits, st);
+        return launch_product<T, EPI_PARTIAL, O_INNER, O_INNER, SRC, 64, 64, 2, 2>(g, p.splits, st);
     }
 
     static hipError_t backward(const LinearArgs& a, hipStream_t st) {
@@ -299,16 +315,16 @@ struct LinearRun {
             return launch_add_splits<T>(nullptr, 0, a.n * a.k + a.n, a.n * a.k, (T*)a.dw, (T*)a.db, st);
         }
         const int act = kept_act<T>(a.act);
-        Operand<T> dz = {(const T*)a.dy, a.lddy, (a.m - 1) * a.lddy + a.n, a.act != MPE_ACT_NONE ? a.pre : nullptr, a.n, a.m * a.n, act};
-        const Operand<T> x = {(const T*)a.x, a.ldx, (a.m - 1) * a.ldx + a.k, nullptr, 0, 0, 0};
-        const bool own = own_dz(a.act, a.k);
+        Operand<T> dz = {(const T*)a.dy, a.lddy, (a.m - 1) * a.lddy + a.n, a.act != MPE_ACT_NONE ? a.pre : nullptr, a.n, a.m * a.n, act, 0};
+        const Operand<T> x = {(const T*)a.x, a.ldx, (a.m - 1) * a.ldx + a.k, nullptr, 0, 0, 0, 0};
+        const bool own = own_dz(a.act, a.k), split = split_dz(a.act, a.k);
         const bool wide = a.dw && wide_weights(sizeof(T), a.m, a.n, a.k) && wide_operand(x, O_INNER, a.k) && (own || wide_operand(dz, O_INNER, a.n));
         char* const ws = (char*)a.ws;
-        float* const partial = (float*)(ws + (own ? round_up(a.m * a.n * (long long)sizeof(T)) : 0));
-        const WeightPlan p = weight_plan(Piece<T>::BK, wide, a.m, a.n, a.k);
+        float* const partial = (float*)(ws + (own ? round_up(dz_elements<T>(a.m, a.n) * (long long)sizeof(T)) : 0));
+        const WeightPlan p = weight_plan(Piece<T>::BK, wide, split, a.m, a.n, a.k);
         const int strip = strip_rows(a.m), strips = (int)tiles_of(a.m, strip);
-        float* const sums = a.db && (wide || own_sums(a.act, a.k)) ? partial + p.splits * a.n * a.k : nullptr;
-        if (sums) {
+        float* const sums = a.db && (wide || split) ? partial + p.splits * a.n * a.k : nullptr;
+        if (sums || split) {
             if constexpr (sizeof(T) == 2)
                 e = launch_slope_sums<T>(a.m, a.n, (const T*)a.dy, a.lddy, own ? (const void*)a.pre : nullptr, act, (T*)ws, strip, sums, st);
         } else if (own && a.lddy == a.n) {
@@ -321,14 +337,18 @@ struct LinearRun {
             e = hipGetLastError();
         }
         if (e != hipSuccess) return e;
-        if (own) dz = {(const T*)ws, a.n, a.m * a.n, nullptr, 0, 0, MPE_ACT_NONE};
+        if (split) dz = {(const T*)ws, a.n * 2, a.m * a.n * 2 - a.n + 8, nullptr, 0, 0, MPE_ACT_NONE, a.n};
+        else if (own) dz = {(const T*)ws, a.n, a.m * a.n, nullptr, 0, 0, MPE_ACT_NONE, 0};
         if (a.dx) {
             ProductArgs<T> g = {};
-            g.p = {(const T*)a.w, a.ldw, (a.n - 1) * a.ldw + a.k, nullptr, 0, 0, 0};
+            g.p = {(const T*)a.w, a.ldw, (a.n - 1) * a.ldw + a.k, nullptr, 0, 0, 0, 0};
             g.q = dz;
             g.ni = a.k; g.nj = a.m; g.nr = a.n;
             g.out = (T*)a.dx; g.ldo = a.lddx;
-            e = dz.pre ? launch_rows<T, EPI_STORE, O_INNER, R_INNER, true>(g, st) : launch_rows<T, EPI_STORE, O_INNER, R_INNER, false>(g, st);
+            if constexpr (sizeof(T) == 2) {
+                if (split) e = launch_rows<T, EPI_STORE, O_INNER, R_INNER, SRC_SPLIT>(g, st);
+            }
+            if (!split) e = dz.pre ? launch_rows<T, EPI_STORE, O_INNER, R_INNER, SRC_DZ>(g, st) : launch_rows<T, EPI_STORE, O_INNER, R_INNER, SRC_PLAIN>(g, st);
             if (e != hipSuccess) return e;
         }
         if (a.dw || (a.db && !sums)) {
@@ -340,9 +360,11 @@ struct LinearRun {
             g.partial_ld = a.n * a.k + (sums ? 0 : a.n);
             g.with_sums = a.db && !sums;
             if constexpr (sizeof(T) == 2) {
-                if (wide) e = launch_product_wide<T, EPI_PARTIAL, O_INNER, O_INNER>(g, p.splits, st);
+                if (wide) e = split ? launch_product_wide<T, EPI_PARTIAL, O_INNER, O_INNER, true>(g, p.splits, st)
+                                    : launch_product_wide<T, EPI_PARTIAL, O_INNER, O_INNER, false>(g, p.splits, st);
+                else if (split) e = weights<SRC_SPLIT>(g, p, st);
             }
-            if (!wide) e = dz.pre ? weights<true>(g, p, st) : weights<false>(g, p, st);
+            if (!wide && !split) e = dz.pre ? weights<SRC_DZ>(g, p, st) : weights<SRC_PLAIN>(g, p, st);
             if (e == hipSuccess) e = launch_add_splits<T>(partial, p.splits, g.partial_ld, a.n * a.k, (T*)a.dw, sums ? nullptr : (T*)a.db, st);
         }
         if (e == hipSuccess && sums) e = launch_add_splits<T>(sums, strips, a.n, 0, nullptr, (T*)a.db, st);

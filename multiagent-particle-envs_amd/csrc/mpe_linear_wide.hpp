@@ -38,7 +38,9 @@ __device__ inline void copy_to_lds(const char* base, unsigned off, unsigned to) 
 // One operand's tile of BO x 32.  R_INNER: rows of 64 bytes, their four 16-byte chunks xored with the row, as Loader::place.
 // O_INNER: 32 rows of BO elements, chunks xored with twice the row's last two bits, so that the four rows a transposed read
 // touches lie on different banks.
-template <typename T, int BO, int LAYOUT>
+// SPLIT: every 64 outputs stand twice, 64 rows (columns) of their values and 64 of their rests, so that a wave's 128 are both
+// pieces of its 64 outputs and nothing else in the kernel has to know.
+template <typename T, int BO, int LAYOUT, bool SPLIT = false>
 struct WideTile {
     typedef T vec8 __attribute__((ext_vector_type(8)));
     typedef short v4i16 __attribute__((ext_vector_type(4)));
@@ -46,6 +48,10 @@ struct WideTile {
     static constexpr int COPIES = BO / 64;      // instructions a wave and stage: 1 KB each
     static constexpr int BYTES = BO * 64;
     static constexpr int RUN = LAYOUT == R_INNER ? 4 : BO / 8;     // chunks a row of the tile
+    static constexpr int OUTPUTS = SPLIT ? BO / 2 : BO;
+    // the output that a row (column) of the tile belongs to, and whether it is its rest
+    static __device__ inline int output_of(int at) { return SPLIT ? (at >> 7) * 64 + (at & 63) : at; }
+    static __device__ inline unsigned piece_of(const Operand<T>& op, int at) { return SPLIT && at & 64 ? (unsigned)op.rest : 0u; }
 
     unsigned off[COPIES];       // bytes from the tile's first element
     const char* next;
@@ -54,13 +60,14 @@ struct WideTile {
     static __device__ inline int swizzle(int row, int chunk) { return LAYOUT == R_INNER ? chunk ^ ((row >> 1) & 3) : chunk ^ ((row & 3) << 1); }
 
     __device__ inline void init(const Operand<T>& op, long long o0, long long no, long long r0) {
-        const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, left = (int)min(no - o0, (long long)BO);
+        const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, left = (int)min(no - o0, (long long)OUTPUTS);
         const unsigned ld = (unsigned)op.ld;
 #pragma unroll
         for (int u = 0; u < COPIES; ++u) {
             const int slot = (wave * COPIES + u) * 64 + lane, row = slot / RUN, chunk = swizzle(row, slot % RUN);
             // outputs that are not there read the last ones again and are never stored
-            off[u] = (LAYOUT == R_INNER ? (unsigned)min(row, left - 1) * ld + chunk * 8 : (unsigned)row * ld + min(chunk * 8, left - 8)) * 2u;
+            off[u] = (LAYOUT == R_INNER ? (unsigned)min(output_of(row), left - 1) * ld + chunk * 8 + piece_of(op, row)
+                                        : (unsigned)row * ld + min(output_of(chunk * 8), left - 8) + piece_of(op, chunk * 8)) * 2u;
         }
         next = (const char*)(op.data + (LAYOUT == R_INNER ? o0 * op.ld + r0 : r0 * op.ld + o0));
         step = LAYOUT == R_INNER ? 64 : 64 * op.ld;
@@ -77,10 +84,11 @@ struct WideTile {
     // earlier, an even number, because addresses are multiples of four bytes.  mend_end() then puts the elements into their
     // places, with the one that an odd number leaves out, and zeros behind the end; a lane mends the chunks it has copied.
     static __device__ inline int back(int left) { return (8 - left % 8) % 8 + (left & 1); }
-    static __device__ inline bool nothing_behind(const Operand<T>& op, long long row, long long no) { return row == no - 1 || op.ld == 0; }
+    // behind two pieces there are eight elements more
+    static __device__ inline bool nothing_behind(const Operand<T>& op, long long row, long long no) { return !SPLIT && (row == no - 1 || op.ld == 0); }
 
     __device__ inline void copy_end(unsigned lds, int wave, const Operand<T>& op, long long o0, long long no, int left) {
-        const int lane = threadIdx.x & 63, left_o = (int)min(no - o0, (long long)BO), before = LAYOUT == R_INNER ? 8 : 0;
+        const int lane = threadIdx.x & 63, left_o = (int)min(no - o0, (long long)OUTPUTS), before = LAYOUT == R_INNER ? 8 : 0;
         const unsigned ld = (unsigned)op.ld;
         const char* const base = uniform(next - before * 2);
 #pragma unroll
@@ -88,17 +96,17 @@ struct WideTile {
             const int slot = (wave * COPIES + u) * 64 + lane, row = slot / RUN, chunk = swizzle(row, slot % RUN);
             unsigned at;
             if (LAYOUT == R_INNER) {
-                const int r = min(row, left_o - 1), c = chunk * 8 < left ? chunk * 8 : 0;
-                at = (unsigned)r * ld + (unsigned)(c + before - (nothing_behind(op, o0 + r, no) && c + 8 > left ? back(left) : 0));
+                const int r = min(output_of(row), left_o - 1), c = chunk * 8 < left ? chunk * 8 : 0;
+                at = (unsigned)r * ld + piece_of(op, row) + (unsigned)(c + before - (nothing_behind(op, o0 + r, no) && c + 8 > left ? back(left) : 0));
             } else {
-                at = (unsigned)min(row, left - 1) * ld + (unsigned)min(chunk * 8, left_o - 8);
+                at = (unsigned)min(row, left - 1) * ld + (unsigned)min(output_of(chunk * 8), left_o - 8) + piece_of(op, chunk * 8);
             }
             copy_to_lds(base, at * 2u, lds + (wave * COPIES + u) * 1024);
         }
     }
 
     static __device__ inline void mend_end(char* lds, int wave, const Operand<T>& op, long long o0, long long no, long long nr, int left) {
-        const int lane = threadIdx.x & 63, left_o = (int)min(no - o0, (long long)BO);
+        const int lane = threadIdx.x & 63, left_o = (int)min(no - o0, (long long)OUTPUTS);
 #pragma unroll
         for (int u = 0; u < COPIES; ++u) {
             const int slot = (wave * COPIES + u) * 64 + lane, row = slot / RUN, chunk = swizzle(row, slot % RUN);
@@ -106,7 +114,7 @@ struct WideTile {
             vec8 v = (T)0.0f;
             if (LAYOUT == R_INNER && chunk * 8 < left) {
                 v = *(const vec8*)(lds + slot * 16);
-                if (nothing_behind(op, o0 + min(row, left_o - 1), no)) {
+                if (nothing_behind(op, o0 + min(output_of(row), left_o - 1), no)) {
                     if (back(left) < 8) shift_down<8>(v, back(left));
                     if (left & 1) {
                         const T last = op.data[(no - 1) * op.ld + nr - 1];
@@ -138,15 +146,15 @@ struct WideTile {
 
 typedef unsigned u32x2 __attribute__((ext_vector_type(2)));
 
-// A wave's 64 x 128 sums, four consecutive columns from i0 + x 16 + 4 (lane / 16) on of row j0 + y 16 + lane % 16 in acc[x][y],
+// A wave's 64 x 16 FJ sums, four consecutive columns from i0 + x 16 + 4 (lane / 16) on of row j0 + y 16 + lane % 16 in acc[x][y],
 // become results in LDS, rows of `pitch` bytes from to on, and in kept[x][y] what is kept, if that has the results' size (if it
 // is float32 it is stored at once).  The activation is a template parameter, since a switch would stand 32 times in the
 // unrolled code.
-template <typename T, int ACT, bool KEPT>
-__device__ __forceinline__ void seal(const ProductArgs<T>& a, const f32x4 (&acc)[4][8], u32x2 (&kept)[4][8], long long i0, long long j0, char* to, int pitch) {
+template <typename T, int ACT, bool KEPT, int FJ>
+__device__ __forceinline__ void seal(const ProductArgs<T>& a, const f32x4 (&acc)[4][8], u32x2 (&kept)[4][FJ], long long i0, long long j0, char* to, int pitch) {
     typedef typename Run<T, 4>::type vec4;
     typedef f16 half4 __attribute__((ext_vector_type(4)));
-    const int lane = threadIdx.x & 63, jl = lane & 15, left_j = (int)min(a.nj - j0, 128LL);
+    const int lane = threadIdx.x & 63, jl = lane & 15, left_j = (int)min(a.nj - j0, 16LL * FJ);
     // what is read is kept inside its row and the matrix; results that are not there get whatever it holds
     const auto four = [&](const T* row, long long i) __attribute__((always_inline)) {
         vec4 v;
@@ -157,10 +165,10 @@ __device__ __forceinline__ void seal(const ProductArgs<T>& a, const f32x4 (&acc)
     };
     const long long i0l = i0 + (lane >> 4) * 4;
     // everything is asked for at once; the four blocks of a row after one another, since they share lines
-    vec4 res[4][8];
+    vec4 res[4][FJ];
     if (a.residual) {
 #pragma unroll
-        for (int y = 0; y < 8; ++y)
+        for (int y = 0; y < FJ; ++y)
 #pragma unroll
             for (int x = 0; x < 4; ++x) res[x][y] = four(a.residual + min(j0 + y * 16 + jl, a.nj - 1) * a.ldr, i0l + x * 16);
     }
@@ -174,7 +182,7 @@ __device__ __forceinline__ void seal(const ProductArgs<T>& a, const f32x4 (&acc)
         }
     }
 #pragma unroll
-    for (int y = 0; y < 8; ++y) {
+    for (int y = 0; y < FJ; ++y) {
 #pragma unroll
         for (int x = 0; x < 4; ++x) {
             const long long i = i0l + x * 16;
@@ -213,13 +221,14 @@ __device__ __forceinline__ void seal(const ProductArgs<T>& a, const f32x4 (&acc)
     }
 }
 
-template <typename T, int EPI, int PL, int QL>
+// SPLIT: Q is dz in two pieces.  The tile is 128 x 128 then, and the second half of a wave's sums are those of the rests.
+template <typename T, int EPI, int PL, int QL, bool SPLIT>
 __global__ __launch_bounds__(256, 2) void product_wide(const ProductArgs<T> a) {
     typedef WideTile<T, Wide::BI, PL> TP;
-    typedef WideTile<T, Wide::BJ, QL> TQ;
+    typedef WideTile<T, Wide::BJ, QL, SPLIT> TQ;
     typedef T vec8 __attribute__((ext_vector_type(8)));
-    constexpr int BI = Wide::BI, BJ = Wide::BJ, BK = Wide::BK, FI = 4, FJ = 8, STAGE = TP::BYTES + TQ::BYTES;
-    constexpr int HALVES = 2, ROWS = BJ / HALVES, PITCH = BI + 4;
+    constexpr int BI = Wide::BI, BJ = TQ::OUTPUTS, BK = Wide::BK, FI = 4, FJ = 8, STAGE = TP::BYTES + TQ::BYTES;
+    constexpr int ROWS = 128, HALVES = BJ / ROWS, PITCH = BI + 4;
     static_assert(ROWS * PITCH * 4 <= Wide::STAGES * STAGE, "the results pass through the stages' memory");
     __shared__ __attribute__((aligned(16))) char lds[Wide::STAGES * STAGE];
 
@@ -228,7 +237,7 @@ __global__ __launch_bounds__(256, 2) void product_wide(const ProductArgs<T> a) {
     const long long r0 = (long long)split * a.r_split, r1 = EPI == EPI_PARTIAL ? min(r0 + a.r_split, a.nr) : a.nr;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const unsigned base = (unsigned)(uintptr_t)(lds_void*)lds;
-    const int wi = (wave & 1) * 64, wj = (wave >> 1) * 128;
+    const int wi = (wave & 1) * 64, half = wave >> 1;
 
     f32x4 acc[FI][FJ];
 #pragma unroll
@@ -241,7 +250,7 @@ __global__ __launch_bounds__(256, 2) void product_wide(const ProductArgs<T> a) {
         for (int x = 0; x < FI; ++x) fp[x] = TP::read(stage, wi + x * 16);
 #pragma unroll
         for (int y = 0; y < FJ; ++y) {
-            const vec8 fq = TQ::read(stage + TP::BYTES, wj + y * 16);
+            const vec8 fq = TQ::read(stage + TP::BYTES, half * 128 + y * 16);
 #pragma unroll
             for (int x = 0; x < FI; ++x) acc[x][y] = mfma(fp[x], fq, acc[x][y]);
         }
@@ -293,6 +302,17 @@ __global__ __launch_bounds__(256, 2) void product_wide(const ProductArgs<T> a) {
         stage = stage == 2 ? 0 : stage + 1;
     }
 
+    constexpr int OJ = SPLIT ? FJ / 2 : FJ;
+    const int wj = half * (16 * OJ);
+    if constexpr (SPLIT) {
+#pragma unroll
+        for (int x = 0; x < FI; ++x)
+#pragma unroll
+            for (int y = 0; y < OJ; ++y)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) acc[x][y][e] = join2(acc[x][y][e], acc[x][y + OJ][e]);
+    }
+
     if constexpr (EPI != EPI_PARTIAL) {
         // Results become what is stored while they are in registers, pass through LDS and leave as whole rows.
         constexpr int PITCH = BI * 2 + 16;
@@ -310,15 +330,15 @@ __global__ __launch_bounds__(256, 2) void product_wide(const ProductArgs<T> a) {
         // one path an activation, to the end: where paths meet again the compiler holds the tile twice
         const auto finish_as = [&](auto act, auto keep) __attribute__((always_inline)) {
             constexpr bool SMALL = decltype(keep)::value && (Kept<T>::SLOPE || decltype(act)::value == MPE_ACT_RELU);
-            u32x2 kept[FI][FJ];
+            u32x2 kept[FI][OJ];
             char* const mine = lds + wj * PITCH + wi * 2;
             __syncthreads();
-            seal<T, decltype(act)::value, decltype(keep)::value>(a, acc, kept, i0 + wi, j0 + wj, mine, PITCH);
+            seal<T, decltype(act)::value, decltype(keep)::value, OJ>(a, acc, kept, i0 + wi, j0 + wj, mine, PITCH);
             leave(a.out, a.ldo);
             if constexpr (SMALL) {
                 __syncthreads();
 #pragma unroll
-                for (int y = 0; y < FJ; ++y)
+                for (int y = 0; y < OJ; ++y)
 #pragma unroll
                     for (int x = 0; x < FI; ++x) *(u32x2*)(mine + (y * 16 + (lane & 15)) * PITCH + (x * 16 + (lane >> 4) * 4) * 2) = kept[x][y];
                 leave((T*)a.pre, a.ni);
@@ -337,7 +357,7 @@ __global__ __launch_bounds__(256, 2) void product_wide(const ProductArgs<T> a) {
             default: return with(std::integral_constant<int, MPE_ACT_SILU>());
         }
     }
-    // partial sums are float32 and pass in two halves
+    // partial sums are float32 and pass 128 rows at a time
     constexpr int N = 4;                                // a thread's columns
     const int it = threadIdx.x % (BI / N) * N;          // a thread's columns, the same in every row it takes
     const long long i = i0 + it;
@@ -346,18 +366,18 @@ __global__ __launch_bounds__(256, 2) void product_wide(const ProductArgs<T> a) {
     const float bias[N] = {};
     float* const res = (float*)lds;
 #pragma unroll
-    for (int half = 0; half < HALVES; ++half) {
+    for (int turn = 0; turn < HALVES; ++turn) {
         __syncthreads();
-        if (wj / ROWS == half) {
+        if (wj / ROWS == turn) {
 #pragma unroll
-            for (int y = 0; y < FJ; ++y)
+            for (int y = 0; y < OJ; ++y)
 #pragma unroll
-                for (int x = 0; x < FI; ++x) *(f32x4*)&res[(y * 16 + (lane & 15)) * PITCH + wi + x * 16 + (lane >> 4) * 4] = acc[x][y];
+                for (int x = 0; x < FI; ++x) *(f32x4*)&res[(wj % ROWS + y * 16 + (lane & 15)) * PITCH + wi + x * 16 + (lane >> 4) * 4] = acc[x][y];
         }
         __syncthreads();
-        const int rows = (int)max(0LL, min((long long)ROWS, a.nj - j0 - half * ROWS));
+        const int rows = (int)max(0LL, min((long long)ROWS, a.nj - j0 - turn * ROWS));
         if (have > 0)
-            finish_rows<T, EPI, N, 256 * N / BI>(a, split, i, j0 + half * ROWS, threadIdx.x / (BI / N), rows, mask, bias, [&](int jt, float* f) {
+            finish_rows<T, EPI, N, 256 * N / BI>(a, split, i, j0 + turn * ROWS, threadIdx.x / (BI / N), rows, mask, bias, [&](int jt, float* f) {
 #pragma unroll
                 for (int e = 0; e < N; e += 4) *(f32x4*)&f[e] = *(const f32x4*)&res[jt * PITCH + it + e];
             });
@@ -371,12 +391,12 @@ inline bool wide_operand(const Operand<T>& o, int layout, long long outputs) {
     return !o.pre && o.ld % 2 == 0 && (uintptr_t)o.data % 4 == 0 && (layout == R_INNER || outputs % 8 == 0);
 }
 
-template <typename T, int EPI, int PL, int QL>
+template <typename T, int EPI, int PL, int QL, bool SPLIT>
 inline hipError_t launch_product_wide(ProductArgs<T> a, int splits, hipStream_t st) {
-    const long long ti = (a.ni + Wide::BI - 1) / Wide::BI, tiles = ti * ((a.nj + Wide::BJ - 1) / Wide::BJ);
+    const long long bj = SPLIT ? Wide::BJ / 2 : Wide::BJ, ti = (a.ni + Wide::BI - 1) / Wide::BI, tiles = ti * ((a.nj + bj - 1) / bj);
     a.ti = (int)ti;
     a.tiles = (unsigned)tiles;
-    hipLaunchKernelGGL((product_wide<T, EPI, PL, QL>), dim3((unsigned)(tiles * splits)), dim3(256), 0, st, a);
+    hipLaunchKernelGGL((product_wide<T, EPI, PL, QL, SPLIT>), dim3((unsigned)(tiles * splits)), dim3(256), 0, st, a);
     return hipGetLastError();
 }
 

@@ -48,7 +48,8 @@ def linear(x, weight, bias=None, activation=None, residual=None):
     float16) on one GPU.  ``activation``: None / "none", "tanh", "relu", "gelu" (by erf) or "silu".  Sums are in float32 or
     better, with one rounding to the type at the end; float32 products are as exact as float32 multiplications.  For the
     backward pass float32 and float16 keep float32 pre-activations, bfloat16 keeps the slopes in float16 (nothing is kept for
-    none, and for relu and float32 tanh without residual)."""
+    none, and for relu and float32 tanh without residual); 16-bit gradients are sums of dz with twice the type's bits, rounded
+    once."""
     try:
         act = ACTIVATIONS[activation]
     except (KeyError, TypeError):

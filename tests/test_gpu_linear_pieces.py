@@ -1,0 +1,143 @@
+"""The gradients of mpe_hip.linear in 16-bit types: dz enters the products with twice the type's bits and a gradient is rounded
+once.
+
+Bounds, written down before any run, with u half a step of the type (bf16 2^-8, fp16 2^-11) and v = 2^-24: a sum of K terms is off
+by (K + 8) v of their sizes, a pre-activation by (k + 8) v of its, a slope by at most 0.9 of that, 16 v (1 + |z|) of its own and, in
+bfloat16, which keeps slopes in float16, by 2^-11 of itself; dz in two pieces is off by u^2 |dz| and half a step of the smallest
+float16 number; then one rounding, u of the result."""
+import math
+
+import pytest
+
+torch = pytest.importorskip("torch")
+pytestmark = pytest.mark.gpu
+
+DEV = "cuda:0"
+V = 2.0 ** -24
+U = {torch.bfloat16: 2.0 ** -8, torch.float16: 2.0 ** -11}
+TINY = {torch.bfloat16: 2.0 ** -126, torch.float16: 2.0 ** -24}
+HALVES = [torch.bfloat16, torch.float16]
+
+
+def act64(z, act):
+    return {"none": lambda: z, "tanh": lambda: torch.tanh(z), "gelu": lambda: z * 0.5 * torch.erfc(-z / math.sqrt(2)), "silu": lambda: z * torch.sigmoid(z)}[act]()
+
+
+def slope64(z, act):
+    z = z.detach().requires_grad_(True)
+    with torch.enable_grad():
+        return torch.autograd.grad(act64(z, act).sum(), z)[0]
+
+
+def gradients(x, w, b, dy, act):
+    """The kernels' dx, dw, db, and float64's with the sizes of what they sum and of what dz may be off by."""
+    import mpe_hip
+    leaves = [t.detach().requires_grad_(True) for t in (x, w, b)]
+    got = torch.autograd.grad(mpe_hip.linear(*leaves, act), leaves, dy)
+    xd, wd, dt, k = x.double(), w.double(), x.dtype, x.shape[1]
+    z = xd @ wd.T + b.double()
+    size = xd.abs() @ wd.abs().T + b.double().abs()
+    d = dy.double()
+    dz = d * slope64(z, act)
+    e = U[dt] ** 2 * dz.abs() + TINY[dt]
+    if act != "none":
+        e = e + d.abs() * (0.9 * (k + 8) * V * size + 16 * V * (1 + z.abs())) + (2.0 ** -11 if dt == torch.bfloat16 else 0.0) * dz.abs()
+    return got, dz, e
+
+
+def check(x, w, b, dy, act):
+    (dx, dw, db), dz, e = gradients(x, w, b, dy, act)
+    dt, (m, n) = x.dtype, dz.shape
+    xd, wd = x.double(), w.double()
+    for name, got, want, mag, off in (("dx", dx, dz @ wd, dz.abs() @ wd.abs(), (n + 8, e @ wd.abs())), ("dw", dw, dz.T @ xd, dz.abs().T @ xd.abs(), (m + 8, e.T @ xd.abs())),
+                                      ("db", db, dz.sum(0), dz.abs().sum(0), (m + 8, e.sum(0)))):
+        bound = off[0] * V * (mag + off[1]) + off[1]
+        bound = bound * (1 + U[dt]) + U[dt] * want.abs() + TINY[dt]
+        bad = ~((got.double() - want).abs() <= bound)
+        assert not bad.any(), "%s: %d of %d outside, worst %g" % (name, int(bad.sum()), bad.numel(), float(((got.double() - want).abs() / bound).max()))
+
+
+def make(m, k, n, dt, ld=None, seed=0):
+    g = torch.Generator(DEV).manual_seed(seed + 7919 * m + 131 * k + n)
+    rnd = lambda *s: torch.randn(*s, device=DEV, generator=g)
+    ld = ld or k
+    return rnd(m, ld).to(dt)[:, ld - k:], (rnd(n, k) / math.sqrt(k)).to(dt), rnd(n).to(dt), rnd(m, n).to(dt)
+
+
+# copies to LDS, whole and ragged; an odd row stride and odd widths that keep them out, in large and small tiles; narrow inputs
+SHAPES = [(8192, 256, 1024, 256), (8200, 320, 1032, 320), (16421, 264, 520, 264), (5000, 1000, 1304, 1001), (5000, 1001, 300, 1001), (3001, 258, 255, 258), (700, 70, 90, 70),
+          (3000, 64, 64, 64), (2000, 14, 64, 42), (900, 40, 17, 40), (300, 9, 130, 9)]
+
+
+@pytest.mark.parametrize("dt", HALVES)
+@pytest.mark.parametrize("m,k,n,ld", SHAPES)
+def test_the_error_is_one_rounding(m, k, n, ld, dt):
+    """Root mean square against that of float64's gradients rounded once.  What bfloat16's slopes add is an eighth of a rounding,
+    1 + 1/128; the sums' float32 far less."""
+    x, w, b, dy = make(m, k, n, dt, ld)
+    (dx, dw, _), dz, _ = gradients(x, w, b, dy, "gelu")
+    for got, want in ((dx, dz @ w.double()), (dw, dz.T @ x.double())):
+        least = float((want.to(dt).double() - want).norm())
+        assert float((got.double() - want).norm()) <= 1.02 * least + 1e-12
+
+
+@pytest.mark.parametrize("dt", HALVES)
+@pytest.mark.parametrize("act", ["gelu", "tanh", "silu", "none"])
+@pytest.mark.parametrize("m,k,n,ld", SHAPES)
+def test_sums_of_one_term_and_sums_that_cancel(m, k, n, ld, act, dt):
+    """Weights with one or two (opposite) entries a column and inputs with one or two a column: a rounding of dz has nothing to hide
+    behind."""
+    x, w, b, dy = make(m, k, n, dt, ld, seed=1)
+    col = torch.arange(k, device=DEV)
+    few = torch.zeros_like(w)
+    few[col % n, col] = w[col % n, col] + 0.75
+    check(x, few, b, dy, act)
+    few[(col + 1) % n, col] = -few[col % n, col]
+    near = dy.clone()
+    near[:, 1:] = dy[:, :1]
+    check(x, few, torch.zeros_like(b) if n > 1 else b, near, act)
+    rows = torch.zeros_like(x)
+    at = (col * 37) % m
+    rows[at, col] = x[at, col] + 0.75
+    check(rows, w, b, dy, act)
+    rows[(at + 1) % m, col] = -rows[at, col]
+    check(rows, w, b, dy[:1].expand(m, n) if act == "none" else dy[:1].expand(m, n).contiguous(), act)
+
+
+@pytest.mark.parametrize("dt", HALVES)
+@pytest.mark.parametrize("m,k,n,ld", SHAPES)
+def test_dense_sums(m, k, n, ld, dt):
+    check(*make(m, k, n, dt, ld, seed=2), "gelu")
+
+
+@pytest.mark.parametrize("dt", HALVES)
+@pytest.mark.parametrize("m,k,n,ld", SHAPES)
+def test_infinities_and_nan_reach_what_they_would(m, k, n, ld, dt):
+    """Where float32's sums are infinite or NaN the gradients are, and nowhere else; dz stays clear of zero."""
+    import mpe_hip
+    x, w, b, dy = make(m, k, n, dt, ld, seed=3)
+    b = b.abs() + 1
+    x, w = x * 0.25, w * 0.25
+    dy = (dy.abs() + 0.5) * torch.where(dy < 0, -1, 1)
+    z = torch.nn.functional.linear(x.float(), w.float(), b.float())
+    dz = dy.float() * slope64(z, "silu").float()
+    leaves = [t.detach().clone().requires_grad_(True) for t in (x, w, b)]
+    y = mpe_hip.linear(*leaves, "silu")
+    bad = dy.clone()
+    bad[3, 0], bad[5, n // 2], bad[m - 1, n - 1] = math.inf, math.nan, -math.inf
+    dz = torch.where(torch.isfinite(bad.float()), dz, bad.float())
+    got = torch.autograd.grad(y, leaves, bad)
+    for a, want in zip(got, (dz @ w.float(), dz.T @ x.float(), dz.sum(0))):
+        assert torch.equal(a.isnan(), want.isnan())
+        assert torch.equal(a.isinf(), want.isinf()) and torch.equal(a[a.isinf()].float(), want[want.isinf()])
+    # the same in the other operand of each product: the forward pass has to be finite, so the leaves change under it
+    dz = dy.float() * slope64(z, "silu").float()
+    for name in ("w", "x"):
+        leaves = [t.detach().clone().requires_grad_(True) for t in (x, w, b)]
+        y = mpe_hip.linear(*leaves, "silu")
+        t = leaves[1 if name == "w" else 0].data
+        t[2, 1], t[t.shape[0] - 1, k - 1] = math.inf, math.nan
+        got = torch.autograd.grad(y, leaves, dy)
+        a, want = (got[0], dz @ t.float()) if name == "w" else (got[1], dz.T @ t.float())
+        assert torch.equal(a.isnan(), want.isnan()), name
+        assert torch.equal(a.isinf(), want.isinf()) and torch.equal(a[a.isinf()].float(), want[want.isinf()]), name
