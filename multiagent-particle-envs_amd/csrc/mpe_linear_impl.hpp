@@ -209,16 +209,26 @@ __device__ inline void split3(const F& f, bf16x8& h, bf16x8& m, bf16x8& l) {
 // 16-bit dz enters a product as two pieces, value and rest: rounded to one it would add as much to the gradients' error again
 // as their own rounding does.  The rests are summed apart, so that an infinity of the other operand, which times a rest of zero
 // is NaN, spoils only what is then left out: the values alone tell what such a sum is.
+// float16 reaches neither far enough up (a slope of 1.13 takes dy beyond 65504) nor down (a rest below 2^-24 would be lost, and with
+// it the bits of every dz below 2^-13): the value is half of dz and the rest is kept 2^11 times as large.  Half of dz is no zero
+// unless dz is one, so that it times an infinity is one.
+template <typename T> struct Two { static constexpr float SCALE = 1.0f, REST = 1.0f; };
+template <> struct Two<f16> { static constexpr float SCALE = 0.5f, REST = 2048.0f; };
 template <typename T>
 __device__ inline void split2(float f, T& h, T& rest) {
     // f as it is: the compiler folds the product that made it into its rounding to float16 (one rounding instead of two), but not
     // where it becomes a float again, and next to a tie the rest would belong to another h
+    f *= Two<T>::SCALE;
     asm("" : "+v"(f));
     h = (T)f;
+    if (Two<T>::SCALE != 1.0f && h == (T)0.0f && f != 0.0f) h = (T)copysignf(0x1p-24f, f);
     const float d = f - (float)h;
-    rest = (T)(fabsf(d) < INFINITY ? d : 0.0f);         // of an infinity or a NaN nothing is left
+    rest = (T)(fabsf(d) < INFINITY ? d * Two<T>::REST : 0.0f);      // of an infinity or a NaN nothing is left
 }
-__device__ inline float join2(float sum, float rests) { return fabsf(rests) < INFINITY ? sum + rests : sum; }
+template <typename T>
+__device__ inline float join2(float sum, float rests) {
+    return (fabsf(rests) < INFINITY ? fmaf(rests, 1.0f / Two<T>::REST, sum) : sum) * (1.0f / Two<T>::SCALE);
+}
 
 // ---- operands ----
 enum { R_INNER, O_INNER };      // which index is contiguous in memory: the summed one, or the output's
@@ -759,7 +769,7 @@ __global__ __launch_bounds__(256, groups_a_cu(Piece<T>::N, EPI, SRC, BI * BJ)) v
 #pragma unroll
             for (int y = 0; y < FJ; ++y)
 #pragma unroll
-                for (int e = 0; e < 4; ++e) acc[x][y][e] = join2(acc[x][y][e], rests[x][y][e]);
+                for (int e = 0; e < 4; ++e) acc[x][y][e] = join2<T>(acc[x][y][e], rests[x][y][e]);
     }
 
     // column sums: the threads that hold the same columns add up through LDS, in the order of their rows

@@ -310,7 +310,7 @@ __global__ __launch_bounds__(256, 2) void product_wide(const ProductArgs<T> a) {
 #pragma unroll
             for (int y = 0; y < OJ; ++y)
 #pragma unroll
-                for (int e = 0; e < 4; ++e) acc[x][y][e] = join2(acc[x][y][e], acc[x][y + OJ][e]);
+                for (int e = 0; e < 4; ++e) acc[x][y][e] = join2<T>(acc[x][y][e], acc[x][y + OJ][e]);
     }
 
     if constexpr (EPI != EPI_PARTIAL) {

@@ -3,8 +3,8 @@ once.
 
 Bounds, written down before any run, with u half a step of the type (bf16 2^-8, fp16 2^-11) and v = 2^-24: a sum of K terms is off
 by (K + 8) v of their sizes, a pre-activation by (k + 8) v of its, a slope by at most 0.9 of that, 16 v (1 + |z|) of its own and, in
-bfloat16, which keeps slopes in float16, by 2^-11 of itself; dz in two pieces is off by u^2 |dz| and half a step of the smallest
-float16 number; then one rounding, u of the result."""
+bfloat16, which keeps slopes in float16, by 2^-11 of itself; dz in two pieces is off by u^2 |dz| and, in float16, by half a step of
+its smallest number over 2^10 (the rests are kept 2^11 times as large, of half of dz); then one rounding, u of the result."""
 import math
 
 import pytest
@@ -39,7 +39,7 @@ def gradients(x, w, b, dy, act):
     size = xd.abs() @ wd.abs().T + b.double().abs()
     d = dy.double()
     dz = d * slope64(z, act)
-    e = U[dt] ** 2 * dz.abs() + TINY[dt]
+    e = U[dt] ** 2 * dz.abs() + TINY[dt] * 2.0 ** -10
     if act != "none":
         e = e + d.abs() * (0.9 * (k + 8) * V * size + 16 * V * (1 + z.abs())) + (2.0 ** -11 if dt == torch.bfloat16 else 0.0) * dz.abs()
     return got, dz, e
@@ -54,6 +54,8 @@ def check(x, w, b, dy, act):
         bound = off[0] * V * (mag + off[1]) + off[1]
         bound = bound * (1 + U[dt]) + U[dt] * want.abs() + TINY[dt]
         bad = ~((got.double() - want).abs() <= bound)
+        if dt == torch.float16:         # 65520 is where rounding to float16 becomes infinite: an infinity is right from there on
+            bad &= ~((got.double() == torch.copysign(torch.full_like(want, math.inf), want)) & (want.abs() + bound >= 65520.0))
         assert not bad.any(), "%s: %d of %d outside, worst %g" % (name, int(bad.sum()), bad.numel(), float(((got.double() - want).abs() / bound).max()))
 
 
@@ -141,3 +143,26 @@ def test_infinities_and_nan_reach_what_they_would(m, k, n, ld, dt):
         a, want = (got[0], dz @ t.float()) if name == "w" else (got[1], dz.T @ t.float())
         assert torch.equal(a.isnan(), want.isnan()), name
         assert torch.equal(a.isinf(), want.isinf()) and torch.equal(a[a.isinf()].float(), want[want.isinf()]), name
+
+
+@pytest.mark.parametrize("m,k,n,ld", SHAPES)
+@pytest.mark.parametrize("power", [-20, -16, -12, -8])
+def test_float16_gradients_keep_their_bits_where_dz_is_small(m, k, n, ld, power):
+    """dy far down in float16's range: its own few bits are all that is lost.  The other operands are as much larger, so that the
+    results lie where float16 has all its bits; x and w in turn, so that pre-activations stay where slopes are between 0 and 1."""
+    x, w, b, dy = make(m, k, n, torch.float16, ld, seed=4)
+    dy = dy * 2.0 ** power
+    up = 2.0 ** min(-power - 6, 9)
+    check(x * up, w / up, b, dy, "silu")
+    check(x / up, w * up, b, dy, "silu")
+
+
+@pytest.mark.parametrize("m,k,n,ld", SHAPES)
+def test_float16_gradients_are_finite_where_dz_is_beyond_its_range(m, k, n, ld):
+    """gelu's slope is 1.13 at 1.41: dy of 60000 gives dz of 67000."""
+    x, w, b, dy = make(m, k, n, torch.float16, ld, seed=5)
+    x, w, b = x * 2.0 ** -8, w * 2.0 ** -6, torch.full_like(b, 1.41)
+    dy = torch.where(dy < 0, -60000.0, 60000.0).half()
+    got, dz, _ = gradients(x, w, b, dy, "gelu")
+    assert float(dz.abs().max()) > 65504 * 1.02
+    check(x, w, b, dy, "gelu")
