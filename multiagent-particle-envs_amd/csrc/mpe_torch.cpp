@@ -2,6 +2,7 @@
 // the autograd nodes, in C++ so that neither the calls nor the backward pass, which torch runs on a thread of its own, wait
 // for the interpreter.  The work itself is behind the C ABI: bind() hands over the addresses of the library that
 // mpe_hip/_lib.py has loaded, so there is one library in the process whichever build it is.
+#include <c10/core/AutogradState.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/autograd/custom_function.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
@@ -58,6 +59,12 @@ int type_of(const Tensor& t, const char* who) {
 }
 
 bool has(const MaybeTensor& t) { return t.has_value() && t->defined(); }
+
+// A forward-mode tangent would be lost without a word: a result without one counts as constant.
+void no_tangent(const MaybeTensor& t, const char* who) {
+    TORCH_CHECK_NOT_IMPLEMENTED(!has(t) || !c10::AutogradState::get_tls_state().get_fw_grad_mode() || !t->_fw_grad(0).defined(), who,
+                                ": forward-mode derivatives are not available");
+}
 void* ptr(const Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; }
 mpe_stream_t stream_of(const Tensor& t) { return (mpe_stream_t)c10::hip::getCurrentHIPStream(t.device().index()).stream(); }
 Tensor bytes_like(int64_t n, const Tensor& t) { return n > 0 ? at::empty({n}, t.options().dtype(at::kByte)) : Tensor(); }
@@ -141,6 +148,7 @@ struct Linear : torch::autograd::Function<Linear> {
         const auto saved = ctx->get_saved_variables();
         const Tensor &x = saved[0], &w = saved[1], &pre = saved[2], &dy = grads[0];
         if (!dy.defined()) return variable_list(6);
+        no_tangent(dy, "linear");
         const bool need_x = ctx->needs_input_grad(0), need_w = ctx->needs_input_grad(1);
         const bool need_b = with_b && ctx->needs_input_grad(2), need_r = with_r && ctx->needs_input_grad(with_b ? 3 : 2);
         Tensor dx, dw, db;
@@ -161,6 +169,7 @@ struct Linear : torch::autograd::Function<Linear> {
 };
 
 Tensor linear(const Tensor& x, const Tensor& w, const MaybeTensor& b, const MaybeTensor& r, int64_t act) {
+    for (const MaybeTensor& t : {MaybeTensor(x), MaybeTensor(w), b, r}) no_tangent(t, "linear");
     const int code = type_of(x, "linear");
     TORCH_CHECK_VALUE(x.dim() >= 1 && w.dim() == 2 && x.size(-1) == w.size(1) && w.size(0) >= 1 && w.size(1) >= 1,
                       "linear: x [..., k] and weight [n, k], n and k at least 1; got ", x.sizes(), " and ", w.sizes());
@@ -216,6 +225,7 @@ struct PpoLoss : torch::autograd::Function<PpoLoss> {
 
     static variable_list backward(AutogradContext* ctx, variable_list grads) {
         if (!grads[0].defined()) return variable_list(5);
+        no_tangent(grads[0], "ppo_loss");
         const int64_t a = ctx->saved_data["a"].toInt();
         const auto q = ctx->saved_data["q"].toDoubleVector();
         const auto s = ctx->get_saved_variables();      // throws where an input was written since
@@ -241,6 +251,7 @@ struct PpoLoss : torch::autograd::Function<PpoLoss> {
 py::tuple ppo_loss(const Tensor& logits, const Tensor& actions, const Tensor& old_logp, const Tensor& adv, const MaybeTensor& values, const MaybeTensor& old_values,
                    const MaybeTensor& returns, const MaybeTensor& mask, const MaybeTensor& weights, double clip, double value_clip, double value_coef,
                    double entropy_coef) {
+    for (const MaybeTensor& t : {MaybeTensor(logits), MaybeTensor(old_logp), MaybeTensor(adv), values, old_values, returns, weights}) no_tangent(t, "ppo_loss");
     const int code = type_of(logits, "ppo_loss");
     TORCH_CHECK_VALUE(logits.dim() >= 1 && logits.size(-1) >= 1, "ppo_loss: logits must be [..., v] with v at least 1, got ", logits.sizes());
     TORCH_CHECK_VALUE(has(values) == has(old_values) && has(values) == has(returns), "ppo_loss: values, old_values and returns go together");
@@ -276,6 +287,9 @@ bool dense(const Tensor& t) { return t.layout() == at::kStrided && (t.is_contigu
 
 Tensor clip(const std::vector<Tensor>& ts, double max_norm, const std::optional<std::vector<Tensor>>& outs) {
     const size_t n = ts.size();
+    for (const Tensor& t : ts) no_tangent(t, "clip_grad_norm");
+    if (outs)
+        for (const Tensor& t : *outs) no_tangent(t, "clip_grad_norm");
     TORCH_CHECK_VALUE(n > 0, "clip_grad_norm: no tensors");
     TORCH_CHECK_VALUE(n <= 0x7fffffff, "clip_grad_norm: too many tensors");
     TORCH_CHECK_VALUE(max_norm >= 0, "clip_grad_norm: max_norm must not be negative, got ", max_norm);

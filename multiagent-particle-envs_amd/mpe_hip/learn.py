@@ -6,7 +6,8 @@
 
 All take GPU tensors (float32, bfloat16 or float16; there is no CPU path), enqueue on the current stream of the tensors'
 device and return without synchronising.  All may be captured into a graph; a backward pass that is captured follows
-autograd's own rule that no eager graph of the same leaves is alive.  Second derivatives are not available.
+autograd's own rule that no eager graph of the same leaves is alive.  Second derivatives and forward-mode derivatives are not
+available: both are refused.
 
 The calls and their autograd nodes are C++ (csrc/mpe_torch.cpp, built into ``_native.so`` next to the library): an operator
 of a few microseconds would otherwise wait for the interpreter.
