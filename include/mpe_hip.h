@@ -482,6 +482,7 @@ int mpe_linear_backward(int device, int dtype, int activation, int64_t m, int64_
  *   stats = [sum w (-s), sum w u, sum w H, sum w (lp - old_logp)^2 / 2, sum w [|q - 1| > clip]] / sum w, sum w   (6 floats)
  * A row is left out, its gradients 0, if its weight is 0 or its action is not in [0, v), is forbidden, or has the logit
  * -infinity (so also where no word is left); what else the row holds is then not used.  With no row left, loss and stats are 0.  rows may be 0.
+ * A NaN in a row that counts shows in the loss and in the row's gradients; a q beyond float32's range times an adv of 0 is 0.
  * The backward pass reads the same inputs, the forward's stats and one device float grad_loss = d(objective)/d(loss) and
  * writes dlogits T[rows][v] (row stride ldd) and, with values, dvalues float[rows] (NULL: not wanted).
  */

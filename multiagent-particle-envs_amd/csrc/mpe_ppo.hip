@@ -56,10 +56,10 @@ __device__ inline void value_terms(const PpoArgs& p, const Row& x, double& loss,
     slope = d;
     if (p.value_clip >= 0.0f) {
         const double c = p.value_clip, step = v - v0;
-        const double held = (step < -c ? v0 - c : step > c ? v0 + c : v) - ret;
-        if (held * held > d * d) {
+        const double held = (step < -c ? v0 - c : step > c ? v0 + c : step == step ? v : step) - ret;     // NaN stays NaN
+        if (d == d && !(held * held <= d * d)) {
             loss = 0.5 * held * held;
-            slope = 0.0;        // beyond the border the held value does not move with v; inside it the two are equal
+            slope = held == held ? 0.0 : held;      // beyond the border the held value does not move with v; inside it the two are equal
         }
     }
 }
@@ -99,20 +99,21 @@ __device__ inline Terms row_terms(const PpoArgs& p, const Row& x, const Soft& q,
     y.logs = fast_log(q.s);
     y.ent = y.logs - q.t / q.s;
     const float diff = at - q.m - y.logs - x.old_lp, ratio = fast_exp(diff);
-    const float held = fminf(fmaxf(ratio, 1.0f - p.clip), 1.0f + p.clip);
-    const float free_term = ratio * x.adv, held_term = held * x.adv;
+    const float held = fminf(fmaxf(ratio, 1.0f - p.clip), 1.0f + p.clip);      // of a NaN a number: free_term shows it
+    // a ratio beyond float32 is a number all the same, and nothing times zero
+    const float free_term = x.adv == 0.0f && fabsf(diff) < INFINITY ? 0.0f : ratio * x.adv, held_term = held * x.adv;
     double vloss = 0.0, vslope = 0.0;
     if (p.values) value_terms(p, x, vloss, vslope);
     if (BACK) {
         const float share = share_all * x.w;
         y.g = free_term <= held_term ? -free_term * share : 0.0f;
-        if (free_term != free_term) y.g = free_term;      // NaN has to show
+        if (free_term != free_term) y.g = free_term;      // and here
         y.ce = p.entropy_coef * share;
         y.vslope = vslope;
         y.share = (double)(p.value_coef * share);
     } else {
         const double w = x.w;
-        sum[0] -= w * (double)(free_term <= held_term ? free_term : held_term);
+        sum[0] -= w * (double)(free_term > held_term ? held_term : free_term);      // NaN has to show
         sum[1] += w * vloss;
         sum[2] += w * y.ent;
         sum[3] += w * 0.5 * (double)diff * (double)diff;
