@@ -249,14 +249,14 @@ struct PpoLoss : torch::autograd::Function<PpoLoss> {
 };
 
 py::tuple ppo_loss(const Tensor& logits, const Tensor& actions, const Tensor& old_logp, const Tensor& adv, const MaybeTensor& values, const MaybeTensor& old_values,
-                   const MaybeTensor& returns, const MaybeTensor& mask, const MaybeTensor& weights, double clip, double value_clip, double value_coef,
+                   const MaybeTensor& returns, const MaybeTensor& mask, const MaybeTensor& weights, double clip, std::optional<double> value_clip, double value_coef,
                    double entropy_coef) {
     for (const MaybeTensor& t : {MaybeTensor(logits), MaybeTensor(old_logp), MaybeTensor(adv), values, old_values, returns, weights}) no_tangent(t, "ppo_loss");
     const int code = type_of(logits, "ppo_loss");
     TORCH_CHECK_VALUE(logits.dim() >= 1 && logits.size(-1) >= 1, "ppo_loss: logits must be [..., v] with v at least 1, got ", logits.sizes());
     TORCH_CHECK_VALUE(has(values) == has(old_values) && has(values) == has(returns), "ppo_loss: values, old_values and returns go together");
     TORCH_CHECK_VALUE(actions.scalar_type() == at::kInt || actions.scalar_type() == at::kLong, "ppo_loss: actions must be int32 or int64, not ", actions.scalar_type());
-    TORCH_CHECK_VALUE(clip >= 0 && (value_clip >= 0 || value_clip == -1.0), "ppo_loss: clip and value_clip must not be negative");
+    TORCH_CHECK_VALUE(clip >= 0 && (!value_clip || *value_clip >= 0), "ppo_loss: clip and value_clip must not be negative");
     const auto lead = logits.sizes().slice(0, logits.dim() - 1);
     const auto side = [&](const char* name, const MaybeTensor& t, at::ScalarType type, at::IntArrayRef shape) {
         if (!has(t)) return Tensor();
@@ -275,7 +275,7 @@ py::tuple ppo_loss(const Tensor& logits, const Tensor& actions, const Tensor& ol
     const std::vector<Tensor> s = {flat(side("actions", actions, actions.scalar_type(), lead)), flat(side("old_logp", old_logp, at::kFloat, lead)),
                                    flat(side("advantages", adv, at::kFloat, lead)), flat(side("old_values", old_values, at::kFloat, lead)),
                                    flat(side("returns", returns, at::kFloat, lead)), m, flat(w)};
-    const PpoCoefs q = {clip, value_clip, value_coef, entropy_coef};
+    const PpoCoefs q = {clip, value_clip.value_or(-1.0), value_coef, entropy_coef};
     const auto out = PpoLoss::apply(logits, values, &s, &q, (int64_t)code);
     return py::make_tuple(out[0], out[1].slice(0, 0, 5));
 }

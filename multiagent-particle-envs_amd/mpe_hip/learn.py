@@ -74,7 +74,7 @@ def ppo_loss(logits, actions, old_logp, advantages, values=None, old_values=None
     has the logit -infinity (so also where no move is left).  Returns ``(loss, stats)``: a float32 scalar and the float32 means
     ``[-s, u, H, (logp - old_logp)^2 / 2, share of clipped decisions]``."""
     return (_module or _native()).ppo_loss(logits, actions, old_logp, advantages, values, old_values, returns, action_mask, weights, clip,
-                                           -1.0 if value_clip is None else value_clip, value_coef, entropy_coef)
+                                           value_clip, value_coef, entropy_coef)
 
 
 def _list(tensors):

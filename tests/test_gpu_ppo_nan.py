@@ -87,3 +87,13 @@ def test_infinite_values_follow_the_formula():
         want = torch.maximum((a - c) ** 2, (b + (a - b).clamp(-torch.tensor(0.2).double(), torch.tensor(0.2).double()) - c) ** 2) / 2
         got = float(stats[1])
         assert math.isnan(got) if math.isnan(float(want)) else got == float(want) or abs(got - float(want)) <= 2.0 ** -22 * abs(float(want)), (V, V0, R, got, float(want))
+
+
+def test_every_negative_value_clip_is_refused():
+    """Also the number that stands for "not clipped" behind the C boundary."""
+    import mpe_hip
+    d = make(5)
+    for bad in (-1.0, -1, -0.5, -1e-60, math.nan):
+        with pytest.raises(ValueError, match="value_clip"):
+            mpe_hip.ppo_loss(**d, value_clip=bad)
+    assert torch.equal(mpe_hip.ppo_loss(**d, value_clip=math.inf)[0], mpe_hip.ppo_loss(**d)[0])
