@@ -9,8 +9,8 @@
 // Instead every float32 is written as the sum of three bfloat16 numbers h + m + l, each the rounded rest of what is
 // before it (3 x 8 bits: the sum is exact), and a product is summed from the six of the nine partial products that
 // float32 can tell: hh + (hm + mh) + (hl + mm + lh).  What is left out is below 2^-25 of |x||w|, half of a float32
-// rounding, and the partial sums are float32 as ever: this is float32 arithmetic at 6/16 of the cost.  Where a result
-// is not finite (infinities split into inf - inf) the element is summed again in plain float32.
+// rounding, and the partial sums are float32 as ever: this is float32 arithmetic at 6/16 of the cost.  Infinities split into
+// inf - inf: where a tile's result is not finite its sums are made again in plain float32 (plain_tile).
 //
 // A workgroup of four waves computes a BI x BJ tile.  Global loads of the next step fly while the matrix instructions of
 // this one run; the operands lie in LDS as rows of BK 16-bit pieces, in 16-byte chunks whose place is xored with the row,
@@ -493,7 +493,7 @@ struct Loader {
     }
 };
 
-// one element's sum in plain float32, for results that are not finite
+// one element's sum in plain float32
 template <typename T, int PL, int QL, bool DZ>
 __device__ inline float plain_sum(const Operand<T>& p, const Operand<T>& q, long long i, long long j, long long r0, long long r1) {
     float s = 0.0f;
@@ -664,6 +664,65 @@ __device__ inline unsigned xcd_run(unsigned b, unsigned n) {
     return x * q + (x < r ? x : r) + b / 8;
 }
 
+// A tile's sums in plain float32, in the place of those that are not finite.  A whole tile at a time, since a NaN or an infinity
+// in a row of one operand reaches a row of results: 16 384 x 1024 -> 1024 takes 1.0 ms if all of x is NaN and 0.75 with one NaN row
+// of weights, where finite numbers take 0.19 (one thread an element: 30 and 2.1).
+template <typename T, int PL, int QL, bool DZ, int BI, int BJ, int FI, int FJ>
+__device__ inline void plain_tile(const ProductArgs<T>& a, long long i0, long long j0, long long r0, long long r1, int wi, int wj, char* lds, f32x4 (&acc)[FI][FJ]) {
+    constexpr int KS = 16, PP = BI + 4, PQ = BJ + 4;
+    float* const tp = (float*)lds;
+    float* const tq = tp + KS * PP;
+    const int lane = threadIdx.x & 63;
+    f32x4 sum[FI][FJ];
+#pragma unroll
+    for (int x = 0; x < FI; ++x)
+#pragma unroll
+        for (int y = 0; y < FJ; ++y) sum[x][y] = 0.0f;
+#pragma unroll 1
+    for (long long r = r0; r < r1; r += KS) {
+        __syncthreads();
+#pragma unroll 1
+        for (int u = threadIdx.x; u < BI * KS; u += 256) {
+            const int o = PL == R_INNER ? u / KS : u % BI, k = PL == R_INNER ? u % KS : u / BI;
+            const long long i = min(i0 + o, a.ni - 1);
+            tp[k * PP + o] = r + k < r1 ? (float)a.p.data[PL == R_INNER ? i * a.p.ld + r + k : (r + k) * a.p.ld + i] : 0.0f;
+        }
+#pragma unroll 1
+        for (int u = threadIdx.x; u < BJ * KS; u += 256) {
+            const int o = QL == R_INNER ? u / KS : u % BJ, k = QL == R_INNER ? u % KS : u / BJ;
+            const long long j = min(j0 + o, a.nj - 1);
+            float f = 0.0f;
+            if (r + k < r1) {
+                f = (float)a.q.data[QL == R_INNER ? j * a.q.ld + r + k : (r + k) * a.q.ld + j];
+                if (DZ && a.q.pre) f *= act_slope(a.q.act, pre_at(a.q, QL == R_INNER ? j * a.q.ld_pre + r + k : (r + k) * a.q.ld_pre + j));
+            }
+            tq[k * PQ + o] = f;
+        }
+        __syncthreads();
+#pragma unroll 1
+        for (int k = 0; k < KS; ++k) {
+            f32x4 p[FI];
+#pragma unroll
+            for (int x = 0; x < FI; ++x) p[x] = *(const f32x4*)&tp[k * PP + wi + x * 16 + (lane >> 4) * 4];
+#pragma unroll
+            for (int y = 0; y < FJ; ++y) {
+                const float q = tq[k * PQ + wj + y * 16 + (lane & 15)];
+#pragma unroll
+                for (int x = 0; x < FI; ++x)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) sum[x][y][e] = fmaf(p[x][e], q, sum[x][y][e]);
+            }
+        }
+    }
+#pragma unroll
+    for (int x = 0; x < FI; ++x)
+#pragma unroll
+        for (int y = 0; y < FJ; ++y)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) acc[x][y][e] = fabsf(acc[x][y][e]) < INFINITY ? acc[x][y][e] : sum[x][y][e];
+    __syncthreads();
+}
+
 // Workgroups that a CU's registers are shared among.  Two 16-bit pieces have two sums: one workgroup fewer, where registers would
 // be kept in memory otherwise.
 constexpr int groups_a_cu(int pieces, int epi, int src, int tile) {
@@ -763,6 +822,17 @@ __global__ __launch_bounds__(256, groups_a_cu(Piece<T>::N, EPI, SRC, BI * BJ)) v
         __syncthreads();
     }
 
+    if constexpr (NP == 3) {        // an infinity times a piece of zero
+        bool bad = false;
+#pragma unroll
+        for (int x = 0; x < FI; ++x)
+#pragma unroll
+            for (int y = 0; y < FJ; ++y)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) bad |= !(fabsf(acc[x][y][e]) < INFINITY);
+        static_assert(16 * (BI + BJ + 8) * 4 <= sizeof(lds), "plain_tile's operands");
+        if (__syncthreads_or(bad)) plain_tile<T, PL, QL, DZ, BI, BJ>(a, i0, j0, r0, r1, wi, wj, lds, acc);
+    }
     if constexpr (NQ == 2) {
 #pragma unroll
         for (int x = 0; x < FI; ++x)
@@ -811,11 +881,6 @@ __global__ __launch_bounds__(256, groups_a_cu(Piece<T>::N, EPI, SRC, BI * BJ)) v
         if (have > 0)
             finish_rows<T, EPI, 4, 1024 / BI>(a, split, i, j0 + half * ROWS, threadIdx.x / (BI / 4), rows, mask, bias, [&](int jt, float* f) {
                 *(f32x4*)f = *(const f32x4*)&res[jt * PITCH + it];
-                if (NP == 3) {          // an infinity times a piece of zero
-#pragma unroll
-                    for (int e = 0; e < 4; ++e)
-                        if (!(fabsf(f[e]) < INFINITY) && e < have) f[e] = plain_sum<T, PL, QL, DZ>(a.p, a.q, i + e, j0 + half * ROWS + jt, r0, r1);
-                }
             });
     }
 }

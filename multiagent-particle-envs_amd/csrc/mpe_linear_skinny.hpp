@@ -2,6 +2,8 @@
 // a single memory access if enough of them are in flight (4 x 1024 -> 4096 bf16: 8.4 MB in 3.9 us, 3 x 14 -> 64 f32 2.4 us, of
 // which an empty launch takes 1.8).
 #pragma once
+#include <type_traits>
+
 #include "mpe_linear_impl.hpp"
 
 namespace mpe {
@@ -55,65 +57,105 @@ __global__ __launch_bounds__(512) void forward_skinny(const ProductArgs<T> a) {
     for (int y = 0; y < FJ; ++y) row_q[y] = (unsigned)min((long long)(y * 16 + l), a.nj - 1 - j0);
 
     f32x4 acc[FJ];
+    // a wave's share of the sums: on the matrix cores, or in plain float32, for which the lanes pass the elements around
+    const auto share = [&](auto plain) __attribute__((always_inline)) {
 #pragma unroll
-    for (int y = 0; y < FJ; ++y) acc[y] = 0.0f;
-    for (int t = wave * each; t < t1; t += AHEAD) {
-        vec8 vp[AHEAD], vq[AHEAD][FJ];
+        for (int y = 0; y < FJ; ++y) acc[y] = 0.0f;
+        for (int t = wave * each; t < t1; t += AHEAD) {
+            vec8 vp[AHEAD], vq[AHEAD][FJ];
 #pragma unroll
-        for (int u = 0; u < AHEAD; ++u)
-            if (t + u < t1) {
-                const long long r = (long long)(t + u) * 32;
-                const Window wp(a.p.extent, i0 * a.p.ld + r, 8), wq(a.q.extent, j0 * a.q.ld + r, 8);
-                __builtin_memcpy(&vp[u], (const char*)(a.p.data + wp.base) + wp.at(row_p * (unsigned)a.p.ld + g * 8) * (unsigned)sizeof(T), sizeof(vec8));
-#pragma unroll
-                for (int y = 0; y < FJ; ++y)
-                    __builtin_memcpy(&vq[u][y], (const char*)(a.q.data + wq.base) + wq.at(row_q[y] * (unsigned)a.q.ld + g * 8) * (unsigned)sizeof(T), sizeof(vec8));
-            }
-#pragma unroll
-        for (int u = 0; u < AHEAD; ++u)
-            if (t + u < t1) {
-                const long long r = (long long)(t + u) * 32;
-                if (r + 32 > a.nr) {        // the sum ends here: elements into their places, zeros behind them
+            for (int u = 0; u < AHEAD; ++u)
+                if (t + u < t1) {
+                    const long long r = (long long)(t + u) * 32;
                     const Window wp(a.p.extent, i0 * a.p.ld + r, 8), wq(a.q.extent, j0 * a.q.ld + r, 8);
-                    const int left = (int)(a.nr - r) - g * 8;
-                    const int by = wp.moved(row_p * (unsigned)a.p.ld + g * 8);
-                    if (by > 0 && by < 8) shift_down<8>(vp[u], by);
+                    __builtin_memcpy(&vp[u], (const char*)(a.p.data + wp.base) + wp.at(row_p * (unsigned)a.p.ld + g * 8) * (unsigned)sizeof(T), sizeof(vec8));
 #pragma unroll
-                    for (int e = 0; e < 8; ++e) vp[u][e] = e < left ? vp[u][e] : (T)0.0f;
+                    for (int y = 0; y < FJ; ++y)
+                        __builtin_memcpy(&vq[u][y], (const char*)(a.q.data + wq.base) + wq.at(row_q[y] * (unsigned)a.q.ld + g * 8) * (unsigned)sizeof(T), sizeof(vec8));
+                }
 #pragma unroll
-                    for (int y = 0; y < FJ; ++y) {
-                        const int byq = wq.moved(row_q[y] * (unsigned)a.q.ld + g * 8);
-                        if (byq > 0 && byq < 8) shift_down<8>(vq[u][y], byq);
+            for (int u = 0; u < AHEAD; ++u)
+                if (t + u < t1) {
+                    const long long r = (long long)(t + u) * 32;
+                    if (r + 32 > a.nr) {        // the sum ends here: elements into their places, zeros behind them
+                        const Window wp(a.p.extent, i0 * a.p.ld + r, 8), wq(a.q.extent, j0 * a.q.ld + r, 8);
+                        const int left = (int)(a.nr - r) - g * 8;
+                        const int by = wp.moved(row_p * (unsigned)a.p.ld + g * 8);
+                        if (by > 0 && by < 8) shift_down<8>(vp[u], by);
 #pragma unroll
-                        for (int e = 0; e < 8; ++e) vq[u][y][e] = e < left ? vq[u][y][e] : (T)0.0f;
+                        for (int e = 0; e < 8; ++e) vp[u][e] = e < left ? vp[u][e] : (T)0.0f;
+#pragma unroll
+                        for (int y = 0; y < FJ; ++y) {
+                            const int byq = wq.moved(row_q[y] * (unsigned)a.q.ld + g * 8);
+                            if (byq > 0 && byq < 8) shift_down<8>(vq[u][y], byq);
+#pragma unroll
+                            for (int e = 0; e < 8; ++e) vq[u][y][e] = e < left ? vq[u][y][e] : (T)0.0f;
+                        }
+                    }
+                    if constexpr (decltype(plain)::value) {
+#pragma unroll 1
+                        for (int from = 0; from < 64; from += 16)
+#pragma unroll
+                            for (int k = 0; k < 8; ++k) {
+                                float p[4];
+#pragma unroll
+                                for (int e = 0; e < 4; ++e) p[e] = __shfl((float)vp[u][k], from + g * 4 + e);
+#pragma unroll
+                                for (int y = 0; y < FJ; ++y) {
+                                    const float q = __shfl((float)vq[u][y][k], from + l);
+#pragma unroll
+                                    for (int e = 0; e < 4; ++e) acc[y][e] = fmaf(p[e], q, acc[y][e]);
+                                }
+                            }
+                    } else {
+                        Frag<T> p;
+                        p.set(vp[u]);
+#pragma unroll
+                        for (int y = 0; y < FJ; ++y) {
+                            Frag<T> q;
+                            q.set(vq[u][y]);
+                            acc[y] = multiply<T>(acc[y], p, q);
+                        }
                     }
                 }
-                Frag<T> p;
-                p.set(vp[u]);
+        }
 #pragma unroll
-                for (int y = 0; y < FJ; ++y) {
-                    Frag<T> q;
-                    q.set(vq[u][y]);
-                    acc[y] = multiply<T>(acc[y], p, q);
-                }
-            }
+        for (int y = 0; y < FJ; ++y) *(f32x4*)&part[wave][y * 16 + l][g * 4] = acc[y];
+        __syncthreads();
+    };
+    const auto total = [&](int jt) {
+        float f = 0.0f;
+#pragma unroll
+        for (int w = 0; w < WAVES; ++w) f += part[w][jt][threadIdx.x & 15];
+        return f;
+    };
+    share(std::false_type());
+    constexpr int MINE = (FJ + 1) / 2;      // a thread's results, 32 rows apart
+    float f[MINE];
+    bool bad = false;
+#pragma unroll
+    for (int c = 0; c < MINE; ++c) {
+        f[c] = (int)(threadIdx.x >> 4) + c * 32 < 16 * FJ ? total((threadIdx.x >> 4) + c * 32) : 0.0f;
+        bad |= !(fabsf(f[c]) < INFINITY);
     }
+    if (Frag<T>::N == 3 && __syncthreads_or(bad)) {      // an infinity times a piece of zero
+        share(std::true_type());
 #pragma unroll
-    for (int y = 0; y < FJ; ++y) *(f32x4*)&part[wave][y * 16 + l][g * 4] = acc[y];
-    __syncthreads();
+        for (int c = 0; c < MINE; ++c)
+            if (!(fabsf(f[c]) < INFINITY)) f[c] = total((threadIdx.x >> 4) + c * 32);
+    }
     const long long i = i0 + (threadIdx.x & 15);
     if (i >= a.ni) return;
     const float bias[1] = {a.bias ? (float)a.bias[i] : 0.0f};
-#pragma unroll 1
-    for (int jt = threadIdx.x >> 4; jt < 16 * FJ && j0 + jt < a.nj; jt += 32) {
-        const long long j = j0 + jt;
-        float f[1] = {0.0f};
 #pragma unroll
-        for (int w = 0; w < WAVES; ++w) f[0] += part[w][jt][threadIdx.x & 15];
-        if (Frag<T>::N == 3 && !(fabsf(f[0]) < INFINITY)) f[0] = plain_sum<T, R_INNER, R_INNER, false>(a.p, a.q, i, j, 0, a.nr);
+    for (int c = 0; c < MINE; ++c) {
+        const int jt = (threadIdx.x >> 4) + c * 32;
+        const long long j = j0 + jt;
+        if (jt >= 16 * FJ || j >= a.nj) break;
         T res = (T)0.0f;
         if (a.residual) load_residual<T, 1>(a, i, j, 1u, res);
-        finish<T, EPI_FORWARD, 1>(a, 0, i, j, 1u, bias, res, f);
+        const float one[1] = {f[c]};
+        finish<T, EPI_FORWARD, 1>(a, 0, i, j, 1u, bias, res, one);
     }
 }
 
