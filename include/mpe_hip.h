@@ -484,7 +484,8 @@ int mpe_linear_backward(int device, int dtype, int activation, int64_t m, int64_
  * -infinity (so also where no word is left); what else the row holds is then not used.  With no row left, loss and stats are 0.  rows may be 0.
  * A NaN in a row that counts shows in the loss and in the row's gradients; a q beyond float32's range times an adv of 0 is 0.
  * The backward pass reads the same inputs, the forward's stats and one device float grad_loss = d(objective)/d(loss) and
- * writes dlogits T[rows][v] (row stride ldd) and, with values, dvalues float[rows] (NULL: not wanted).
+ * writes dlogits T[rows][v] (row stride ldd; NULL with ldd 0: only dvalues is wanted) and, with values, dvalues float[rows] (NULL:
+ * not wanted).
  */
 #define MPE_PPO_WORKSPACE_BYTES 61440
 int mpe_ppo_loss_forward(int device, int dtype, int64_t rows, int64_t v, const void* logits, int64_t ld, const void* actions, int action_bytes,

@@ -808,10 +808,12 @@ int mpe_ppo_loss_backward(int device, int dtype, int64_t rows, int64_t v, const 
     const int rc = check_ppo("mpe_ppo_loss_backward", a);
     if (rc != MPE_OK) return rc;
     if (rows == 0) return MPE_OK;
-    if (!stats || !grad_loss || !dlogits) return fail(nullptr, MPE_ERR_INVALID, "mpe_ppo_loss_backward: stats, grad_loss and dlogits must not be NULL");
+    const bool values_alone = !dlogits && ldd == 0 && dvalues;
+    if (!stats || !grad_loss || (!dlogits && !values_alone))
+        return fail(nullptr, MPE_ERR_INVALID, "mpe_ppo_loss_backward: stats, grad_loss and dlogits must not be NULL (dlogits may, with ldd 0 and dvalues)");
     if (dvalues && !values) return fail(nullptr, MPE_ERR_INVALID, "mpe_ppo_loss_backward: dvalues without values");
     const int64_t s = dtype_bytes(dtype), nd = extent(rows, v, ldd, s);
-    if (bad_stride(rows, ldd, v, false)) return fail(nullptr, MPE_ERR_INVALID, "mpe_ppo_loss_backward: a row stride is smaller than its row");
+    if (dlogits && bad_stride(rows, ldd, v, false)) return fail(nullptr, MPE_ERR_INVALID, "mpe_ppo_loss_backward: a row stride is smaller than its row");
     if (misaligned(dlogits, s) || misaligned(dvalues, 4) || misaligned(stats, 4) || misaligned(grad_loss, 4))
         return fail(nullptr, MPE_ERR_INVALID, "mpe_ppo_loss_backward: a buffer is not aligned to its element");
     const void* in[10] = {logits, actions, old_logp, adv, mask, weights, values, old_values, returns, stats};

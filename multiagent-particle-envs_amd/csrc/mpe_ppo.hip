@@ -404,6 +404,19 @@ __global__ __launch_bounds__(256) void ppo_many(const PpoArgs p) {
     if (!BACK) leave_sums<4>(p, sum, scratch);
 }
 
+// The values' gradient alone: which rows count, and nothing of the softmax.
+template <typename T>
+__global__ __launch_bounds__(256) void ppo_values(const PpoArgs p) {
+    const float share_all = share_of(p);
+    for (long long r = (long long)blockIdx.x * 256 + threadIdx.x; r < p.rows; r += (long long)gridDim.x * 256) {
+        const Row x = read_row(p, r);
+        double vloss, vslope;
+        value_terms(p, x, vloss, vslope);
+        const bool live = x.live && (!p.mask || p.mask[r * p.ldm + x.a]) && (float)((const T*)p.logits)[r * p.ld + x.a] != -INFINITY;
+        p.dvalues[r] = live ? (float)(vslope * (double)(p.value_coef * (share_all * x.w))) : 0.0f;
+    }
+}
+
 __global__ __launch_bounds__(1024) void ppo_finish(const double* __restrict__ partial, int n, float value_coef, float entropy_coef,
                                                    float* __restrict__ loss, float* __restrict__ stats) {
     __shared__ double scratch[16][NSTAT];
@@ -455,6 +468,13 @@ hipError_t launch_ppo_forward(const PpoArgs& a, hipStream_t st) {
 
 hipError_t launch_ppo_backward(const PpoArgs& a, hipStream_t st) {
     if (a.rows == 0) return hipSuccess;
+    if (!a.dlogits) {
+        const long long want = (a.rows + 255) / 256;
+        return with_dtype(a.dtype, [&](auto z) {
+            hipLaunchKernelGGL((ppo_values<decltype(z)>), dim3((unsigned)(want < BACKWARD_GRID ? want : BACKWARD_GRID)), dim3(256), 0, st, a);
+            return hipGetLastError();
+        });
+    }
     return with_dtype(a.dtype, [&](auto z) { return launch_rows<decltype(z), true>(a, nullptr, st); });
 }
 

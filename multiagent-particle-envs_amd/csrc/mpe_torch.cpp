@@ -236,13 +236,12 @@ struct PpoLoss : torch::autograd::Function<PpoLoss> {
             const int64_t v = logits.size(-1);
             const Rows l2 = rows_of(logits, v), m2 = s[8].defined() ? rows_of(s[8], v) : Rows{Tensor(), 0};
             const Tensor val = flat(values), grad = grads[0].scalar_type() == at::kFloat ? grads[0] : grads[0].to(at::kFloat);
-            dl = at::empty(logits.sizes(), logits.options());
+            if (need_l) dl = at::empty(logits.sizes(), logits.options());
             if (need_v) dv = at::empty(values.sizes(), values.options());
             check(api.ppo_backward(logits.device().index(), (int)(a & 15), logits.numel() / v, v, ptr(l2.t), l2.ld, ptr(s[3]), (int)s[3].element_size(),
                                    (const float*)ptr(s[4]), (const float*)ptr(s[5]), (const uint8_t*)ptr(m2.t), m2.ld, (const float*)ptr(s[9]),
                                    (const float*)ptr(val), (const float*)ptr(s[6]), (const float*)ptr(s[7]), q[0], q[1], q[2], q[3], (const float*)ptr(s[2]),
-                                   (const float*)ptr(grad), ptr(dl), v, (float*)ptr(dv), stream_of(logits)));
-            if (!need_l) dl = Tensor();
+                                   (const float*)ptr(grad), ptr(dl), need_l ? v : 0, (float*)ptr(dv), stream_of(logits)));
         }
         return once({dl, dv, Tensor(), Tensor(), Tensor()}, "ppo_loss");
     }

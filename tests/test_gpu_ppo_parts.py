@@ -1,0 +1,42 @@
+"""mpe_hip.ppo_loss where only values learn."""
+import pytest
+
+torch = pytest.importorskip("torch")
+pytestmark = pytest.mark.gpu
+
+DEV = "cuda:0"
+
+
+def make(rows, v, dt=torch.float32):
+    g = torch.Generator(DEV).manual_seed(rows + v)
+    rnd = lambda *s: torch.randn(*s, device=DEV, generator=g)
+    d = dict(logits=rnd(rows, v).to(dt), actions=torch.randint(-1, v + 1, (rows,), device=DEV, generator=g), old_logp=rnd(rows) - 1, advantages=rnd(rows), values=rnd(rows),
+             old_values=rnd(rows), returns=rnd(rows), action_mask=rnd(rows, v) < 1, weights=(rnd(rows) + 0.5).clamp(min=0))
+    d["logits"][::5, 0] = -float("inf")
+    return d
+
+
+@pytest.mark.parametrize("dt", [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("rows,v", [(1, 1), (75, 5), (3000, 20), (100, 300), (9, 9000)])
+@pytest.mark.parametrize("value_clip", [None, 0.2])
+def test_the_values_gradient_alone_has_the_same_bits(rows, v, dt, value_clip):
+    import mpe_hip
+    d = make(rows, v, dt)
+    for mask, weights in ((True, True), (False, False)):
+        q = dict(d, action_mask=d["action_mask"] if mask else None, weights=d["weights"] if weights else None)
+        leaves = [q["logits"].clone().requires_grad_(True), q["values"].clone().requires_grad_(True)]
+        both = torch.autograd.grad(mpe_hip.ppo_loss(**dict(q, logits=leaves[0], values=leaves[1]), value_clip=value_clip)[0], leaves)
+        alone, = torch.autograd.grad(mpe_hip.ppo_loss(**dict(q, values=leaves[1]), value_clip=value_clip)[0], leaves[1:])
+        assert torch.equal(alone, both[1])
+
+
+def test_the_values_gradient_alone_needs_no_place_for_the_logits():
+    import mpe_hip
+    d = make(2000, 8192)
+    values = d["values"].requires_grad_(True)
+    loss, _ = mpe_hip.ppo_loss(**d)
+    torch.cuda.synchronize()
+    before = torch.cuda.memory_allocated()
+    torch.cuda.reset_peak_memory_stats()
+    torch.autograd.grad(loss, values)
+    assert torch.cuda.max_memory_allocated() - before < d["logits"].numel()        # a quarter of their bytes
