@@ -93,6 +93,9 @@ Rows rows_or_one(const Tensor& t, int64_t cols) {
     return rows_of(t, cols);
 }
 
+// t itself, or its copy if rows_of had to make one
+Tensor as_taken(const Tensor& t, const Rows& rows) { return rows.t.is_alias_of(t) ? t : rows.t.view(t.sizes()); }
+
 Tensor flat(const Tensor& t) { return t.defined() && !t.is_contiguous() ? t.contiguous() : t; }
 
 // Gradients that cannot be differentiated again say so if it is tried.
@@ -204,7 +207,7 @@ struct PpoCoefs {
 struct PpoLoss : torch::autograd::Function<PpoLoss> {
     static variable_list forward(AutogradContext* ctx, const Tensor& logits, const MaybeTensor& values, const std::vector<Tensor>* side, const PpoCoefs* q,
                                  int64_t code) {
-        // side: actions, old_logp, adv, old_values, returns, mask, weights, the first five and the last contiguous
+        // side: actions, old_logp, adv, old_values, returns, mask, weights; the mask as rows, the others contiguous
         const int64_t v = logits.size(-1);
         const Rows l2 = rows_of(logits, v), m2 = (*side)[5].defined() ? rows_of((*side)[5], v) : Rows{Tensor(), 0};
         const Tensor val = has(values) ? flat(*values) : Tensor();
@@ -218,7 +221,8 @@ struct PpoLoss : torch::autograd::Function<PpoLoss> {
                               (float*)ptr(stats), ptr(ws), MPE_PPO_WORKSPACE_BYTES, stream_of(logits)));
         ctx->saved_data["a"] = code | (has(values) ? 16 : 0);
         ctx->saved_data["q"] = std::vector<double>{q->clip, q->value_clip, q->value_coef, q->entropy_coef};
-        ctx->save_for_backward({logits, has(values) ? *values : Tensor(), stats, s[0], s[1], s[2], s[3], s[4], s[5], s[6]});
+        // what had to be copied is saved as it was copied
+        ctx->save_for_backward({as_taken(logits, l2), val, stats, s[0], s[1], s[2], s[3], s[4], s[5], s[6]});
         ctx->mark_non_differentiable({stats});
         return {loss, stats};
     }
@@ -235,12 +239,12 @@ struct PpoLoss : torch::autograd::Function<PpoLoss> {
         if (need_l || need_v) {
             const int64_t v = logits.size(-1);
             const Rows l2 = rows_of(logits, v), m2 = s[8].defined() ? rows_of(s[8], v) : Rows{Tensor(), 0};
-            const Tensor val = flat(values), grad = grads[0].scalar_type() == at::kFloat ? grads[0] : grads[0].to(at::kFloat);
+            const Tensor grad = grads[0].scalar_type() == at::kFloat ? grads[0] : grads[0].to(at::kFloat);
             if (need_l) dl = at::empty(logits.sizes(), logits.options());
             if (need_v) dv = at::empty(values.sizes(), values.options());
             check(api.ppo_backward(logits.device().index(), (int)(a & 15), logits.numel() / v, v, ptr(l2.t), l2.ld, ptr(s[3]), (int)s[3].element_size(),
                                    (const float*)ptr(s[4]), (const float*)ptr(s[5]), (const uint8_t*)ptr(m2.t), m2.ld, (const float*)ptr(s[9]),
-                                   (const float*)ptr(val), (const float*)ptr(s[6]), (const float*)ptr(s[7]), q[0], q[1], q[2], q[3], (const float*)ptr(s[2]),
+                                   (const float*)ptr(values), (const float*)ptr(s[6]), (const float*)ptr(s[7]), q[0], q[1], q[2], q[3], (const float*)ptr(s[2]),
                                    (const float*)ptr(grad), ptr(dl), need_l ? v : 0, (float*)ptr(dv), stream_of(logits)));
         }
         return once({dl, dv, Tensor(), Tensor(), Tensor()}, "ppo_loss");
@@ -268,6 +272,7 @@ py::tuple ppo_loss(const Tensor& logits, const Tensor& actions, const Tensor& ol
     if (has(mask)) {
         TORCH_CHECK_VALUE(mask->scalar_type() == at::kBool || mask->scalar_type() == at::kByte, "ppo_loss: action_mask must be bool or uint8, not ", mask->scalar_type());
         m = side("action_mask", mask, mask->scalar_type(), logits.sizes());
+        m = as_taken(m, rows_of(m, logits.size(-1)));
     }
     if (has(weights)) w = side("weights", weights->scalar_type() == at::kBool ? MaybeTensor(weights->to(at::kFloat)) : weights, at::kFloat, lead);
     side("values", values, at::kFloat, lead);

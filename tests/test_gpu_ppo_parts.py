@@ -1,4 +1,4 @@
-"""mpe_hip.ppo_loss where only values learn."""
+"""mpe_hip.ppo_loss where only values learn, and where its inputs do not lie as rows."""
 import pytest
 
 torch = pytest.importorskip("torch")
@@ -40,3 +40,25 @@ def test_the_values_gradient_alone_needs_no_place_for_the_logits():
     torch.cuda.reset_peak_memory_stats()
     torch.autograd.grad(loss, values)
     assert torch.cuda.max_memory_allocated() - before < d["logits"].numel()        # a quarter of their bytes
+
+
+@pytest.mark.parametrize("rows,v", [(400, 5), (300, 700)])
+def test_inputs_that_are_copied_are_copied_once(rows, v):
+    """Columns of a transposed tensor, a mask of one row for all: the backward pass finds the forward's copies."""
+    import mpe_hip
+    d = make(rows, v)
+    turned = d["logits"].T.contiguous().T.requires_grad_(True)
+    q = dict(d, logits=turned, action_mask=d["action_mask"][:1].expand(rows, v), values=torch.stack([d["values"]] * 2, 1)[:, 0].requires_grad_(True))
+    plain = {k: t.detach().contiguous().requires_grad_(k in ("logits", "values")) for k, t in q.items()}
+    loss, _ = mpe_hip.ppo_loss(**q, value_clip=0.2)
+    want = torch.autograd.grad(mpe_hip.ppo_loss(**plain, value_clip=0.2)[0], [plain["logits"], plain["values"]])
+    before = torch.cuda.memory_allocated()
+    torch.cuda.reset_peak_memory_stats()
+    got = torch.autograd.grad(loss, [turned, q["values"]], retain_graph=True)
+    size = sum(t.numel() * t.element_size() for t in got)
+    assert torch.cuda.max_memory_allocated() - before <= size + 2048
+    assert all(torch.equal(a, b) for a, b in zip(got, want)) and got[0].shape == (rows, v)
+    cube = {k: t.detach().reshape((rows // 4, 4) + t.shape[1:]) for k, t in q.items()}
+    cube["logits"] = turned.detach().view(rows, v).unflatten(0, (rows // 4, 4)).requires_grad_(True)
+    got3, = torch.autograd.grad(mpe_hip.ppo_loss(**cube, value_clip=0.2)[0], cube["logits"])
+    assert torch.equal(got3.reshape(rows, v), want[0])
