@@ -76,6 +76,7 @@ struct Rows {
 };
 
 Rows rows_of(const Tensor& t, int64_t cols) {
+    if (t.is_neg()) return rows_of(t.resolve_neg(), cols);      // memory that holds the negative of its numbers
     if (t.is_contiguous()) return {t, cols};
     Tensor m = t.dim() == 2 ? t : t.reshape({-1, cols});
     const int64_t rows = m.size(0), ld = m.stride(0);
@@ -85,7 +86,7 @@ Rows rows_of(const Tensor& t, int64_t cols) {
 
 // One row of a vector's length or more that expand() repeats stays one row: stride 0.
 Rows rows_or_one(const Tensor& t, int64_t cols) {
-    if (cols >= 8 && !t.is_contiguous() && t.dim() >= 2 && t.numel() > 0 && t.stride(-1) == 1) {
+    if (cols >= 8 && !t.is_neg() && !t.is_contiguous() && t.dim() >= 2 && t.numel() > 0 && t.stride(-1) == 1) {
         bool one = true;
         for (int64_t d = 0; d + 1 < t.dim(); ++d) one = one && (t.stride(d) == 0 || t.size(d) == 1);
         if (one) return {t, 0};
@@ -96,7 +97,7 @@ Rows rows_or_one(const Tensor& t, int64_t cols) {
 // t itself, or its copy if rows_of had to make one
 Tensor as_taken(const Tensor& t, const Rows& rows) { return rows.t.is_alias_of(t) ? t : rows.t.view(t.sizes()); }
 
-Tensor flat(const Tensor& t) { return t.defined() && !t.is_contiguous() ? t.contiguous() : t; }
+Tensor flat(const Tensor& t) { return t.defined() && (!t.is_contiguous() || t.is_neg()) ? t.resolve_neg().contiguous() : t; }
 
 // Gradients that cannot be differentiated again say so if it is tried.
 variable_list once(variable_list grads, const char* who) {
@@ -239,7 +240,7 @@ struct PpoLoss : torch::autograd::Function<PpoLoss> {
         if (need_l || need_v) {
             const int64_t v = logits.size(-1);
             const Rows l2 = rows_of(logits, v), m2 = s[8].defined() ? rows_of(s[8], v) : Rows{Tensor(), 0};
-            const Tensor grad = grads[0].scalar_type() == at::kFloat ? grads[0] : grads[0].to(at::kFloat);
+            const Tensor grad = (grads[0].scalar_type() == at::kFloat ? grads[0] : grads[0].to(at::kFloat)).resolve_neg();
             if (need_l) dl = at::empty(logits.sizes(), logits.options());
             if (need_v) dv = at::empty(values.sizes(), values.options());
             check(api.ppo_backward(logits.device().index(), (int)(a & 15), logits.numel() / v, v, ptr(l2.t), l2.ld, ptr(s[3]), (int)s[3].element_size(),
@@ -287,7 +288,7 @@ py::tuple ppo_loss(const Tensor& logits, const Tensor& actions, const Tensor& ol
 // ---- global norm ----
 
 // t's elements fill one run of memory, in whatever order of dimensions
-bool dense(const Tensor& t) { return t.layout() == at::kStrided && (t.is_contiguous() || t.is_non_overlapping_and_dense()); }
+bool dense(const Tensor& t) { return !t.is_neg() && t.layout() == at::kStrided && (t.is_contiguous() || t.is_non_overlapping_and_dense()); }
 
 Tensor clip(const std::vector<Tensor>& ts, double max_norm, const std::optional<std::vector<Tensor>>& outs) {
     const size_t n = ts.size();
@@ -309,14 +310,14 @@ Tensor clip(const std::vector<Tensor>& ts, double max_norm, const std::optional<
         type[i] = type_code(t.scalar_type());
         TORCH_CHECK_VALUE(t.is_cuda() && t.device() == dev && type[i] >= 0, "clip_grad_norm: tensor ", i,
                           " must be float32, bfloat16 or float16 on the GPU of tensor 0 (", dev, "), got ", t.scalar_type(), " on ", t.device());
-        TORCH_CHECK_VALUE(dense(t), "clip_grad_norm: tensor ", i, " is sparse or has gaps or repeated elements");
+        TORCH_CHECK_VALUE(dense(t), "clip_grad_norm: tensor ", i, " is sparse, a negative view or has gaps or repeated elements");
         src[i] = t.data_ptr();
         count[i] = t.numel();
         if (!outs) continue;
         const Tensor& o = (*outs)[i];
         TORCH_CHECK_VALUE(!at::GradMode::is_enabled() || !o.requires_grad(), "clip_grad_norm: out ", i, " requires gradients, which clipping does not have");
         if (!o.is_same(t))
-            TORCH_CHECK_VALUE(o.layout() == at::kStrided && o.scalar_type() == t.scalar_type() && o.device() == dev && o.sizes() == t.sizes() &&
+            TORCH_CHECK_VALUE(!o.is_neg() && o.layout() == at::kStrided && o.scalar_type() == t.scalar_type() && o.device() == dev && o.sizes() == t.sizes() &&
                                   ((o.is_contiguous() && t.is_contiguous()) || o.strides() == t.strides()),
                               "clip_grad_norm: out ", i, " must have the shape, strides, type and device of its tensor");
         dst[i] = o.data_ptr();

@@ -40,3 +40,29 @@ def test_function_transforms_are_refused(transform):
             torch.func.grad(f)(x)
         else:
             torch.func.vmap(f)(x[:, None])
+
+
+def test_views_of_the_negative_of_their_memory():
+    """The imaginary part of a conjugate: torch keeps the sign as a mark on the tensor."""
+    import mpe_hip
+    neg = lambda *s: torch.randn(*s, dtype=torch.complex64, device=DEV).conj().imag
+    plain = lambda t: torch.empty_like(t).copy_(t)
+    x, w, b, dy = neg(40, 1), neg(3, 1), neg(3), neg(40, 3)
+    assert x.is_neg() and w.is_neg() and not plain(x).is_neg()
+    for first in ((x, w, b, dy), (torch._neg_view(plain(x)), torch._neg_view(plain(w)), torch._neg_view(plain(b)), torch._neg_view(plain(dy))),
+                  (neg(1, 40), neg(30, 40), neg(30), neg(1, 30))):
+        got, want = [], []
+        for out, q in ((got, first), (want, [plain(t) for t in first])):
+            leaves = [t.requires_grad_(True) for t in q[:3]]
+            y = mpe_hip.linear(*leaves, "tanh")
+            out += [y.detach()] + list(torch.autograd.grad(y, leaves, q[3]))
+        assert all(torch.equal(p, q) for p, q in zip(got, want))
+    logits, act = torch._neg_view(torch.randn(6, 5, device=DEV)), torch.zeros(6, dtype=torch.int32, device=DEV)
+    rest = [torch._neg_view(torch.randn(6, device=DEV)) for _ in range(5)]
+    one, two = (mpe_hip.ppo_loss(f(logits), act, *[f(t) for t in rest], weights=f(rest[0])) for f in (lambda t: t, plain))
+    assert torch.equal(one[0], two[0]) and torch.equal(one[1], two[1])
+    for bad in (torch._neg_view(torch.randn(4, device=DEV)), neg(1)):
+        with pytest.raises(ValueError, match="negative view"):
+            mpe_hip.grad_norm([bad])
+        with pytest.raises(ValueError, match="out 0"):
+            mpe_hip.clip_grad_norm([plain(bad)], 1.0, out=[bad])
