@@ -66,13 +66,20 @@ __device__ inline Normal normal_of(float z) {
     return n;
 }
 
-// tanh as exact as a 16-bit type can tell (2e-6 of it): the series' first two terms below 1/16
-__device__ inline float tanh_16(float z) {
-    const float big = fmaf(-2.0f, __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(z * (2.0f * 1.44269504088896341f))), 1.0f);
-    return fabsf(z) < 0.0625f ? fmaf(z * z * z, -1.0f / 3.0f, z) : big;
+// tanh as exact as a 16-bit type can tell (2e-6 of it): the series' first two terms below 1/16, elsewhere 2 r - 1 with
+// e = e^(-2|z|) and r = 1 / (1 + e).  Its slope is 4 e r^2, which keeps its relative precision where 1 - tanh^2 has none left.
+__device__ inline float tanh_16(float z, float& slope) {
+    const float e = __builtin_amdgcn_exp2f(fabsf(z) * (-2.0f * 1.44269504088896341f)), r = __builtin_amdgcn_rcpf(1.0f + e);
+    slope = 4.0f * e * (r * r);
+    return fabsf(z) < 0.0625f ? fmaf(z * z * z, -1.0f / 3.0f, z) : copysignf(fmaf(2.0f, r, -1.0f), z);
 }
 template <typename T>
-__device__ inline float tanh_for(float z) { return sizeof(T) == 2 ? tanh_16(z) : tanh_of(z); }
+__device__ inline float tanh_for(float z, float& slope) {
+    if (sizeof(T) == 2) return tanh_16(z, slope);
+    const float t = tanh_of(z);
+    slope = fmaf(-t, t, 1.0f);
+    return t;
+}
 
 __device__ inline float relu(float z) { return z > 0.0f || z != z ? z : 0.0f; }
 
@@ -97,8 +104,7 @@ __device__ inline void act_both(int act, float* z, float* slope) {
         case MPE_ACT_TANH:
 #pragma unroll
             for (int e = 0; e < N; ++e) {
-                z[e] = tanh_for<T>(z[e]);
-                slope[e] = fmaf(-z[e], z[e], 1.0f);
+                z[e] = tanh_for<T>(z[e], slope[e]);
             }
             break;
         case MPE_ACT_GELU:
@@ -130,7 +136,10 @@ __device__ inline void act_values(int act, float* z) {
         case MPE_ACT_NONE: break;
         case MPE_ACT_TANH:
 #pragma unroll
-            for (int e = 0; e < N; ++e) z[e] = tanh_for<T>(z[e]);
+            for (int e = 0; e < N; ++e) {
+                float slope;
+                z[e] = tanh_for<T>(z[e], slope);
+            }
             break;
         case MPE_ACT_RELU:
 #pragma unroll

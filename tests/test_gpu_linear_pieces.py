@@ -166,3 +166,24 @@ def test_float16_gradients_are_finite_where_dz_is_beyond_its_range(m, k, n, ld):
     got, dz, _ = gradients(x, w, b, dy, "gelu")
     assert float(dz.abs().max()) > 65504 * 1.02
     check(x, w, b, dy, "gelu")
+
+
+@pytest.mark.parametrize("m,k,n", [(513, 1, 1), (513, 14, 20), (513, 70, 40), (8192, 64, 1024), (8193, 264, 520)])
+@pytest.mark.parametrize("act", ["tanh", "silu"])
+def test_bfloat16_keeps_small_slopes_to_their_own_precision(m, k, n, act):
+    """Saturated units: slopes down to 2^-28, where 2^14 times them leave float16's normal range.  One term in every sum.  Off by the
+    kept slope's rounding 2^-11, by the exponential's (2 |z| + 8) 2^-22 and, silu's only, by 2^-22 of the size of its two terms, and
+    rounded once."""
+    import mpe_hip
+    dt = torch.bfloat16
+    z = torch.linspace(-9.5, 9.5, m, device=DEV).to(dt)
+    x, w, dy = torch.zeros(m, k, device=DEV, dtype=dt), torch.zeros(n, k, device=DEV, dtype=dt), torch.zeros(m, n, device=DEV, dtype=dt)
+    x[:, 0], w[n - 1, 0], dy[:, n - 1] = z, 1.0, 3.0
+    x.requires_grad_(True)
+    got, = torch.autograd.grad(mpe_hip.linear(x, w, None, act), x, dy)
+    zd = z.double()
+    slope = 1 / torch.cosh(zd) ** 2 if act == "tanh" else torch.sigmoid(zd) * (1 + zd * torch.sigmoid(-zd))
+    parts = slope if act == "tanh" else torch.sigmoid(zd) * (1 + zd.abs())
+    off = 3 * (slope.abs() * 2.0 ** -11 + parts * (2 * zd.abs() + 8) * 2.0 ** -22 + 2.0 ** -39)
+    assert ((got[:, 0].double() - 3 * slope).abs() <= off + U[dt] * (3 * slope.abs() + off)).all()
+    assert float(got[:, 1:].abs().sum()) == 0
