@@ -16,14 +16,16 @@ namespace mpe {
 namespace {
 
 constexpr int NSTAT = 6;        // policy, value, entropy, kl, clipped, weight
-// Grids.  Forward: five workgroups a CU, which all find room at once (the rollout of 4.9 M rows: 67 us at 1024 workgroups,
-// 64 at 1280, 72 at 1792, when the last ones have to wait for a place).  Backward: enough that none is left over at the
+// Grids.  Forward: five workgroups a CU, which all find room at once (the rollout of 4.9 M rows of five words: 67 us at 1024
+// workgroups, 64 at 1280, 72 at 1792, when the last ones have to wait for a place), three where registers and LDS hold no more
+// (ppo_few from 9 words on; 50 M logits, 768 against 1280: 9 words 105 us against 112, 12 words 117 against 130, 24 words 87 against
+// 95; whole rows go on from 768 to 1280, 40 words 647 to 452).  Backward: enough that none is left over at the
 // end (86 us at 4096 workgroups of 256 rows, 84 at 8192, 88 at 16384; whole rows: 50 us from 2048 to 16384, 55 at 1280).
 //
 // What bounds it.  4.9 M rows of five words: memory, 236 MB in 62 us (3.8 TB/s) and 354 MB in 82 (4.3); 60 float64 and some 150
 // float32 operations a row hide behind it.  4096 rows of 8192 bf16 words with a mask: 101 MB in 23.8 us (4.2 TB/s), and 168 MB in
 // 48.8 backwards (3.4 TB/s; asking for the next row while one is worked on was slower: 58, there are waves enough).
-constexpr int FORWARD_GRID = 1280, BACKWARD_GRID = 8192;
+constexpr int FORWARD_GRID = 1280, FORWARD_GRID_FEW = 768, BACKWARD_GRID = 8192;
 static_assert(FORWARD_GRID * 8 * NSTAT <= MPE_PPO_WORKSPACE_BYTES, "a partial sum for every workgroup");
 
 struct Row {
@@ -432,8 +434,8 @@ __global__ __launch_bounds__(1024) void ppo_finish(const double* __restrict__ pa
 
 template <typename T, bool BACK>
 hipError_t launch_rows(const PpoArgs& a, int* grid_out, hipStream_t st) {
-    const auto grid_for = [&](long long per_block) {
-        const int most = BACK ? BACKWARD_GRID : FORWARD_GRID;
+    const auto grid_for = [&](long long per_block, int forward_grid = FORWARD_GRID) {
+        const int most = BACK ? BACKWARD_GRID : forward_grid;
         long long g = (a.rows + per_block - 1) / per_block;
         g = g < 1 ? 1 : g > most ? most : g;
         if (grid_out) *grid_out = (int)g;
@@ -443,7 +445,7 @@ hipError_t launch_rows(const PpoArgs& a, int* grid_out, hipStream_t st) {
     if (a.v <= FEW) {
         const size_t bytes = 256 * (size_t)(a.v | 1) * 4;
         if (a.v <= 8) hipLaunchKernelGGL((ppo_few<T, BACK, 8>), grid_for(256), dim3(256), bytes, st, a);
-        else hipLaunchKernelGGL((ppo_few<T, BACK, FEW>), grid_for(256), dim3(256), bytes, st, a);
+        else hipLaunchKernelGGL((ppo_few<T, BACK, FEW>), grid_for(256, FORWARD_GRID_FEW), dim3(256), bytes, st, a);
     } else if (a.v <= 64 * E) {
         hipLaunchKernelGGL((ppo_many<T, BACK, 1, 1>), grid_for(4), dim3(256), 0, st, a);
     } else if (a.v <= 4 * 64 * E) {
