@@ -9,6 +9,8 @@
 //
 // The backward pass takes no softmax statistics from the forward pass: it has to read the logits again anyway and
 // recomputes them while the row is at hand.
+#include <type_traits>
+
 #include "mpe_learn.hpp"
 
 namespace mpe {
@@ -17,15 +19,15 @@ namespace {
 
 constexpr int NSTAT = 6;        // policy, value, entropy, kl, clipped, weight
 // Grids.  Forward: five workgroups a CU, which all find room at once (the rollout of 4.9 M rows of five words: 67 us at 1024
-// workgroups, 64 at 1280, 72 at 1792, when the last ones have to wait for a place), three where registers and LDS hold no more
-// (ppo_few from 9 words on; 50 M logits, 768 against 1280: 9 words 105 us against 112, 12 words 117 against 130, 24 words 87 against
-// 95; whole rows go on from 768 to 1280, 40 words 647 to 452).  Backward: enough that none is left over at the
+// workgroups, 64 at 1280, 72 at 1792, when the last ones have to wait for a place), three and two where registers and LDS hold no
+// more (ppo_few from 9 and from 33 words on; 50 M logits, 9 words 105 us at 768 and 112 at 1280, 24 words 87 and 95, 48 words 107 at
+// 512 and 134 at 768).  Backward: enough that none is left over at the
 // end (86 us at 4096 workgroups of 256 rows, 84 at 8192, 88 at 16384; whole rows: 50 us from 2048 to 16384, 55 at 1280).
 //
 // What bounds it.  4.9 M rows of five words: memory, 236 MB in 62 us (3.8 TB/s) and 354 MB in 82 (4.3); 60 float64 and some 150
 // float32 operations a row hide behind it.  4096 rows of 8192 bf16 words with a mask: 101 MB in 23.8 us (4.2 TB/s), and 168 MB in
 // 48.8 backwards (3.4 TB/s; asking for the next row while one is worked on was slower: 58, there are waves enough).
-constexpr int FORWARD_GRID = 1280, FORWARD_GRID_FEW = 768, BACKWARD_GRID = 8192;
+constexpr int FORWARD_GRID = 1280, FORWARD_GRID_32 = 768, FORWARD_GRID_FEW = 512, BACKWARD_GRID = 8192;
 static_assert(FORWARD_GRID * 8 * NSTAT <= MPE_PPO_WORKSPACE_BYTES, "a partial sum for every workgroup");
 
 struct Row {
@@ -176,7 +178,7 @@ __device__ inline void leave_sums(const PpoArgs& p, const double* sum, double (*
 // Few words: a lane takes a row.  A workgroup's 256 rows are fetched into LDS (consecutive lanes read consecutive elements
 // whatever v is; rows there are an odd number of words apart, so that 64 lanes walking their rows meet 64 banks) and the
 // gradients leave the same way.
-constexpr int FEW = 32;
+constexpr int FEW = 62;         // 256 rows of 63 floats end with 64 KB of LDS
 
 template <typename T, bool BACK, int VR>        // VR: at least v
 __global__ __launch_bounds__(256) void ppo_few(const PpoArgs p) {
@@ -188,8 +190,9 @@ __global__ __launch_bounds__(256) void ppo_few(const PpoArgs p) {
     const float share_all = BACK ? share_of(p) : 0.0f;
 
     // the next tile's loads are in flight while this one is worked on
+    typedef std::conditional_t<(VR > 32), unsigned long long, unsigned> bits;
     T raw[VR];
-    unsigned ok = 0;
+    bits ok = 0;
     Row next;
     auto load = [&](long long r0) {
         const int rows = (int)min(256LL, p.rows - r0), n = rows * v;
@@ -203,7 +206,7 @@ __global__ __launch_bounds__(256) void ppo_few(const PpoArgs p) {
             if (u < v) {
                 if (tid + u * 256 < n) {
                     raw[u] = base[(long long)row * p.ld + col];
-                    ok |= (!mask || mask[(long long)row * p.ldm + col] ? 1u : 0u) << u;
+                    ok |= (!mask || mask[(long long)row * p.ldm + col] ? (bits)1 : (bits)0) << u;
                 }
                 row += dr;
                 col += dc;
@@ -432,6 +435,10 @@ __global__ __launch_bounds__(1024) void ppo_finish(const double* __restrict__ pa
     if (threadIdx.x == 0) write_totals(scratch[0], value_coef, entropy_coef, loss, stats);
 }
 
+// A variant goes as far as its registers and its LDS do.  On both sides of each border, 50 M logits forward and backward, us: 32
+// words 83 and 130 in ppo_few, 552 and 574 in ppo_many; 62 words 99 and 170, 63 in ppo_many 328 and 374; one vector a lane, 256
+// float32 words 79 and 110, with room for four 115 and 156; four vectors, 1024 words 38 and 90, four waves a row 106 and 157; four waves,
+// 4096 words 38 and 83, read twice 66 and 179 (bfloat16, 8192 words: 31 and 62, 37 and 88).
 template <typename T, bool BACK>
 hipError_t launch_rows(const PpoArgs& a, int* grid_out, hipStream_t st) {
     const auto grid_for = [&](long long per_block, int forward_grid = FORWARD_GRID) {
@@ -445,6 +452,7 @@ hipError_t launch_rows(const PpoArgs& a, int* grid_out, hipStream_t st) {
     if (a.v <= FEW) {
         const size_t bytes = 256 * (size_t)(a.v | 1) * 4;
         if (a.v <= 8) hipLaunchKernelGGL((ppo_few<T, BACK, 8>), grid_for(256), dim3(256), bytes, st, a);
+        else if (a.v <= 32) hipLaunchKernelGGL((ppo_few<T, BACK, 32>), grid_for(256, FORWARD_GRID_32), dim3(256), bytes, st, a);
         else hipLaunchKernelGGL((ppo_few<T, BACK, FEW>), grid_for(256, FORWARD_GRID_FEW), dim3(256), bytes, st, a);
     } else if (a.v <= 64 * E) {
         hipLaunchKernelGGL((ppo_many<T, BACK, 1, 1>), grid_for(4), dim3(256), 0, st, a);

@@ -62,3 +62,13 @@ def test_inputs_that_are_copied_are_copied_once(rows, v):
     cube["logits"] = turned.detach().view(rows, v).unflatten(0, (rows // 4, 4)).requires_grad_(True)
     got3, = torch.autograd.grad(mpe_hip.ppo_loss(**cube, value_clip=0.2)[0], cube["logits"])
     assert torch.equal(got3.reshape(rows, v), want[0])
+
+
+@pytest.mark.parametrize("dt", [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("rows,v", [(300, 31), (300, 32), (300, 33), (2000, 47), (300, 48), (259, 49), (300, 61), (1030, 62), (300, 63)])
+def test_about_as_many_words_as_lanes(rows, v, dt):
+    """Where a lane a row and a wave a row meet: the formula, with masks and weights."""
+    from test_gpu_ppo import check
+    from test_gpu_ppo import make as rollout
+    check(rollout(rows, v, dt, mask=True, weights=True), value_clip=0.2)
+    check(rollout(rows, v, dt, values=False))
