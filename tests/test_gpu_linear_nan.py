@@ -104,3 +104,17 @@ def test_the_time_stays_in_proportion(m, k, n, times):
     row, everything = best(x, w2), best(torch.full_like(x, math.nan), w)
     print("\n%d x %d -> %d: %.1f us, a NaN row of weights %.1f, all NaN %.1f" % (m, k, n, finite * 100, row * 100, everything * 100))
     assert row <= times * finite and everything <= times * finite
+
+
+@pytest.mark.parametrize("power", [-60, -100, -109, -112, -116, -120])
+def test_numbers_far_down_in_float32(power):
+    """The parts of a number end with bfloat16's smallest, 2^-133: below 2^-109 what lies under half of it, 2^-134, is lost of every
+    factor, and nothing else."""
+    import mpe_hip
+    for m, k, n in ((5, 40, 30), (300, 100, 72), (5000, 17, 200)):
+        x, w, b, dy = make(m, k, n, seed=2)
+        for xx, ww, other in ((x * 2.0 ** power, w, w.double().abs().sum(1)[None]), (x, w * 2.0 ** power, x.double().abs().sum(1)[:, None])):
+            lost = 2.0 ** -134 * other
+            got, want = mpe_hip.linear(xx, ww), xx.double() @ ww.double().T
+            mag = xx.double().abs() @ ww.double().abs().T
+            assert ((got.double() - want).abs() <= (k + 8) * V * mag + lost + 2.0 ** -149).all()

@@ -187,3 +187,58 @@ def test_bfloat16_keeps_small_slopes_to_their_own_precision(m, k, n, act):
     off = 3 * (slope.abs() * 2.0 ** -11 + parts * (2 * zd.abs() + 8) * 2.0 ** -22 + 2.0 ** -39)
     assert ((got[:, 0].double() - 3 * slope).abs() <= off + U[dt] * (3 * slope.abs() + off)).all()
     assert float(got[:, 1:].abs().sum()) == 0
+
+
+@pytest.mark.parametrize("m,k,n", [(4_200_001, 256, 520), (4_200_001, 259, 513)])
+def test_pieces_of_more_than_2_to_32_elements(m, k, n):
+    """Both pieces of dz together; first, middle and last rows, which an offset of 32 bits would miss."""
+    import mpe_hip
+    dt = torch.bfloat16
+    rnd = lambda *s, seed: torch.randn(*s, device=DEV, dtype=dt, generator=torch.Generator(DEV).manual_seed(seed))
+    x, w = rnd(m, k, seed=1).requires_grad_(True), (rnd(n, k, seed=2) / 16).requires_grad_(True)
+    y = mpe_hip.linear(x, w, None, "silu")
+    rows = torch.tensor([0, 1, 2 ** 31 // n - 1, 2 ** 31 // n, 2 ** 31 // n + 1, 2 ** 32 // (2 * n), 2 ** 32 // n // 2 + 1, m - 2, m - 1], device=DEV).unique()
+    dy = torch.zeros_like(y)
+    dy[rows] = rnd(len(rows), n, seed=3)            # the others add zeros: exact
+    dx, dw = torch.autograd.grad(y, (x, w), dy)
+    xd, wd, d = x.detach()[rows].double(), w.detach().double(), dy[rows].double()
+    z = xd @ wd.T
+    dz = d * slope64(z, "silu")
+    e = d.abs() * (0.9 * (k + 8) * V * (xd.abs() @ wd.abs().T) + 16 * V * (1 + z.abs())) + (2.0 ** -11 + U[dt] ** 2) * dz.abs()
+    for got, want, off, mag, terms in ((dx[rows], dz @ wd, e @ wd.abs(), dz.abs() @ wd.abs(), n), (dw, dz.T @ xd, e.T @ xd.abs(), dz.abs().T @ xd.abs(), len(rows))):
+        bound = off + (terms + 8) * V * (mag + off)
+        assert ((got.double() - want).abs() <= bound * (1 + U[dt]) + U[dt] * want.abs() + TINY[dt]).all()
+    other = torch.ones(m, dtype=torch.bool, device=DEV)
+    other[rows] = False
+    assert float(dx[other].abs().max()) == 0
+
+
+@pytest.mark.parametrize("dt", HALVES)
+@pytest.mark.parametrize("m,k,n", [(16384, 256, 512), (3001, 258, 255), (3000, 64, 64)])
+def test_captured_gradients_replay(m, k, n, dt):
+    """A captured forward and backward pass beside a second one of the same leaves, replayed between eager calls on new inputs."""
+    import mpe_hip
+    x, w, b, dy = make(m, k, n, dt)
+    leaves = [t.detach().clone().requires_grad_(True) for t in (x, w, b)]
+    call = lambda ls, up: torch.autograd.grad(mpe_hip.linear(*ls, "gelu"), ls, up)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        call(leaves, dy)
+    torch.cuda.current_stream().wait_stream(side)
+    graphs, outs = [torch.cuda.CUDAGraph() for _ in range(2)], []
+    for graph in graphs:
+        with torch.cuda.graph(graph):
+            outs.append(call(leaves, dy))
+    for i in range(3):
+        with torch.no_grad():
+            for t in leaves:
+                t.copy_(torch.randn_like(t) * 0.3)
+            dy.copy_(torch.randn_like(dy))
+        for graph in graphs:
+            graph.replay()
+        torch.cuda.synchronize()
+        want = call([t.detach().clone().requires_grad_(True) for t in leaves], dy)
+        for out in outs:
+            assert all(torch.equal(p, q) for p, q in zip(out, want)), i
+        torch.cuda.synchronize()
