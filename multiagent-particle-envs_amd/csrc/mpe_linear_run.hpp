@@ -12,10 +12,11 @@ inline long long tiles_of(long long n, int b) { return (n + b - 1) / b; }
 // workgroups of 256 threads that a grid dimension holds: their threads are counted in 32 bits
 constexpr int MAX_GROUPS = 0xffffff;
 
-// ---- dz = dy f'(pre) as an array of its own: in float32 [m][n], in 16-bit types two pieces (split2), [m][2][n], and eight elements
-// behind the last ----
+// ---- dz = dy f'(pre) as an array of its own: in float32 [m][n], in 16-bit types two pieces (split2), [m][2][piece_row(n)] ----
+// whole vectors, so that no row starts between two
+inline long long piece_row(long long n) { return (n + 7) / 8 * 8; }
 template <typename T>
-inline long long dz_elements(long long m, long long n) { return sizeof(T) == 2 ? m * n * 2 + 8 : m * n; }
+inline long long dz_elements(long long m, long long n) { return sizeof(T) == 2 ? m * piece_row(n) * 2 : m * n; }
 
 // float32, dense dy: eight elements a thread, whatever the rows' length
 template <typename T>
@@ -67,7 +68,7 @@ __global__ __launch_bounds__(256) void slope_sums(long long m, long long n, cons
     constexpr int E = 8, STEP = 256 / WIDE;
     __shared__ float part[STEP][WIDE][E + 1];
     const int c = threadIdx.x % WIDE, g = threadIdx.x / WIDE;
-    const long long i = ((long long)blockIdx.x * WIDE + c) * E, j1 = min((long long)(blockIdx.y + 1) * rows, m);
+    const long long i = ((long long)blockIdx.x * WIDE + c) * E, row = (n + E - 1) / E * E, j1 = min((long long)(blockIdx.y + 1) * rows, m);
     float s[E] = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
     if (i + E <= n) {
 #pragma unroll 4
@@ -94,14 +95,15 @@ __global__ __launch_bounds__(256) void slope_sums(long long m, long long n, cons
                     split2(f[e], d[e], rest[e]);
                 }
                 if (dz) {
-                    __builtin_memcpy(dz + j * n * 2 + i, d, sizeof(d));
-                    __builtin_memcpy(dz + j * n * 2 + n + i, rest, sizeof(rest));
+                    __builtin_memcpy(dz + j * row * 2 + i, d, sizeof(d));
+                    __builtin_memcpy(dz + j * row * 2 + row + i, rest, sizeof(rest));
                 }
             }
 #pragma unroll
             for (int e = 0; e < E; ++e) s[e] += f[e];
         }
     } else if (i < n) {         // the last columns
+#pragma unroll 4
         for (long long j = (long long)blockIdx.y * rows + g; j < j1; j += STEP)
 #pragma unroll
             for (int e = 0; e < E; ++e)
@@ -110,7 +112,7 @@ __global__ __launch_bounds__(256) void slope_sums(long long m, long long n, cons
                     if (pre) {
                         const long long at = j * n + i + e;
                         f *= act_slope(act, small_pre(act) ? kept_small<T>(act, ((const T*)pre)[at]) : ((const float*)pre)[at]);
-                        if (dz) split2(f, dz[j * n * 2 + i + e], dz[j * n * 2 + n + i + e]);
+                        if (dz) split2(f, dz[j * row * 2 + i + e], dz[j * row * 2 + row + i + e]);
                     }
                     s[e] += f;
                 }
@@ -270,7 +272,8 @@ struct WeightPlan {
     int bi, bj, splits;
     long long r_split;
 };
-inline WeightPlan weight_plan(int bk, bool wide, bool split, long long m, long long n, long long k) {
+// two: 16-bit dz in two pieces, split: from an array
+inline WeightPlan weight_plan(int bk, bool wide, bool two, bool split, long long m, long long n, long long k) {
     WeightPlan p;
     p.wide = wide;
     if (wide) {
@@ -286,8 +289,8 @@ inline WeightPlan weight_plan(int bk, bool wide, bool split, long long m, long l
     p.bj = p.bi == 128 ? (split ? 64 : 128) : p.bi == 64 && n <= 16 ? 16 : 64;
     const long long tiles = tiles_of(k, p.bi) * tiles_of(n, p.bj);
     // four workgroups a CU (64/64 f32 over 196 608 rows, product and sum of the splits: 38.6 us at 1024 workgroups, 41.2 at
-    // 768, 46.0 at 512)
-    long long s = 1024 / tiles;
+    // 768, 46.0 at 512); of two pieces as many as there is room for (64/64 bf16 over 524 288 rows 77 at 768, 100 at 1024)
+    long long s = (two ? 256 * groups_a_cu(1, EPI_PARTIAL, split ? SRC_SPLIT : SRC_DZ, p.bi * p.bj) : 1024) / tiles;
     const long long most = tiles_of(m, 4 * bk);      // at least four steps each
     if (s > most) s = most;
     if (s < 1) s = 1;
@@ -302,9 +305,13 @@ inline WeightPlan weight_plan(int bk, bool wide, bool split, long long m, long l
 inline bool wide_weights(int size, long long m, long long n, long long k) {
     return size == 2 && k >= 256 && n >= 128 && k % 8 == 0 && n % 8 == 0 && m >= 4096;
 }
-// Rows a workgroup of slope_sums takes: 128, more where there would be more than 32768 such strips (a grid's second dimension
-// ends at 65535).
-inline int strip_rows(long long m) { return (int)std::max(128LL, tiles_of(tiles_of(m, 32768), 8) * 8); }
+// Rows a workgroup of slope_sums takes: 128, or 32 where that would be less than two workgroups a CU (with whole vectors in the rows
+// of pieces, 10 007 x 258 -> 255 bf16, dz and dx: 36 us, 82 without both); more where there would be more than 32768 strips (a
+// grid's second dimension ends at 65535).
+inline int strip_rows(long long m, long long n) {
+    const long long rows = tiles_of(m, 128) * tiles_of(n, 256) < 512 ? 32 : 128;
+    return (int)std::max(rows, tiles_of(tiles_of(m, 32768), 8) * 8);
+}
 
 // Wide inputs: dz becomes an array of its own, where it would otherwise be worked out in every tile of k of both products
 // (131 072 x 128 -> 128 gelu, both gradients: bf16 68 us against 116, f32 148 against 177; x 64 -> 64 bf16 57 against 54).
@@ -314,15 +321,16 @@ inline long long round_up(long long n) { return (n + 255) / 256 * 256; }
 
 template <typename T>
 struct LinearRun {
+    static bool two_pieces(int act) { return sizeof(T) == 2 && act != MPE_ACT_NONE; }
     // dz as an array of its own in 16-bit types: its column sums are taken while it is made
     static bool split_dz(int act, long long k) { return sizeof(T) == 2 && own_dz(act, k); }
 
     static long long backward_workspace(int act, long long m, long long n, long long k) {
         if (m == 0) return 0;
-        const WeightPlan p = weight_plan(Piece<T>::BK, false, split_dz(act, k), m, n, k);
-        const long long strips = tiles_of(m, strip_rows(m)) * n;
+        const WeightPlan p = weight_plan(Piece<T>::BK, false, two_pieces(act), split_dz(act, k), m, n, k);
+        const long long strips = tiles_of(m, strip_rows(m, n)) * n;
         long long sums = p.splits * n * k + (split_dz(act, k) ? strips : p.splits * n);
-        if (wide_weights(sizeof(T), m, n, k)) sums = std::max(sums, weight_plan(Piece<T>::BK, true, split_dz(act, k), m, n, k).splits * n * k + strips);
+        if (wide_weights(sizeof(T), m, n, k)) sums = std::max(sums, weight_plan(Piece<T>::BK, true, two_pieces(act), split_dz(act, k), m, n, k).splits * n * k + strips);
         return (own_dz(act, k) ? round_up(dz_elements<T>(m, n) * (long long)sizeof(T)) : 0) + sums * 4;
     }
 
@@ -364,8 +372,8 @@ struct LinearRun {
         const bool wide = wide_weights(sizeof(T), a.m, a.n, a.k) && wide_operand(x, O_INNER, a.k) && (own || wide_operand(dz, O_INNER, a.n));
         char* const ws = (char*)a.ws;
         float* const partial = (float*)(ws + (own ? round_up(dz_elements<T>(a.m, a.n) * (long long)sizeof(T)) : 0));
-        const WeightPlan p = weight_plan(Piece<T>::BK, wide, split, a.m, a.n, a.k);
-        const int strip = strip_rows(a.m), strips = (int)tiles_of(a.m, strip);
+        const WeightPlan p = weight_plan(Piece<T>::BK, wide, two_pieces(a.act), split, a.m, a.n, a.k);
+        const int strip = strip_rows(a.m, a.n), strips = (int)tiles_of(a.m, strip);
         const bool products = a.dx || a.dw;
         float* const sums = a.db && (wide || split) ? partial + p.splits * a.n * a.k : nullptr;
         if (sums || (split && products)) {
@@ -381,7 +389,8 @@ struct LinearRun {
             e = hipGetLastError();
         }
         if (e != hipSuccess) return e;
-        if (split && products) dz = {(const T*)ws, a.n * 2, a.m * a.n * 2 - a.n + 8, nullptr, 0, 0, MPE_ACT_NONE, a.n};
+        const long long row = piece_row(a.n);
+        if (split && products) dz = {(const T*)ws, row * 2, a.m * row * 2 - row, nullptr, 0, 0, MPE_ACT_NONE, row};
         else if (own && products) dz = {(const T*)ws, a.n, a.m * a.n, nullptr, 0, 0, MPE_ACT_NONE, 0};
         if (a.dx) {
             ProductArgs<T> g = {};

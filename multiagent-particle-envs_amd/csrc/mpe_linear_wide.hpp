@@ -84,7 +84,7 @@ struct WideTile {
     // earlier, an even number, because addresses are multiples of four bytes.  mend_end() then puts the elements into their
     // places, with the one that an odd number leaves out, and zeros behind the end; a lane mends the chunks it has copied.
     static __device__ inline int back(int left) { return (8 - left % 8) % 8 + (left & 1); }
-    // behind two pieces there are eight elements more
+    // rows of pieces hold whole chunks
     static __device__ inline bool nothing_behind(const Operand<T>& op, long long row, long long no) { return !SPLIT && (row == no - 1 || op.ld == 0); }
 
     __device__ inline void copy_end(unsigned lds, int wave, const Operand<T>& op, long long o0, long long no, int left) {
