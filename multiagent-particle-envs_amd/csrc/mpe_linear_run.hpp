@@ -12,50 +12,38 @@ inline long long tiles_of(long long n, int b) { return (n + b - 1) / b; }
 // workgroups of 256 threads that a grid dimension holds: their threads are counted in 32 bits
 constexpr int MAX_GROUPS = 0xffffff;
 
-// ---- dz = dy f'(pre) as an array of its own: in float32 [m][n], in 16-bit types two pieces (split2), [m][2][piece_row(n)] ----
+// ---- dz = dy f'(pre) as an array of its own: in float32 [m][n], in 16-bit types two pieces (split2), [m][2][piece_row(n)], or
+// one where that is exact ----
 // whole vectors, so that no row starts between two
 inline long long piece_row(long long n) { return (n + 7) / 8 * 8; }
 template <typename T>
 inline long long dz_elements(long long m, long long n) { return sizeof(T) == 2 ? m * piece_row(n) * 2 : m * n; }
 
-// float32, dense dy: eight elements a thread, whatever the rows' length
+// float32 (the one T), dense dy: eight elements a thread, whatever the rows' length
 template <typename T>
-__global__ __launch_bounds__(256) void slope_flat(long long total, const T* __restrict__ dy, const void* __restrict__ pre, int act, T* __restrict__ dz) {
+__global__ __launch_bounds__(256) void slope_flat(long long total, const T* __restrict__ dy, const T* __restrict__ pre, int act, T* __restrict__ dz) {
     typedef T vec8 __attribute__((ext_vector_type(8)));
-    typedef float z8 __attribute__((ext_vector_type(8)));
     for (long long at = ((long long)blockIdx.x * 256 + threadIdx.x) * 8; at < total; at += (long long)gridDim.x * 2048) {
         if (at + 8 <= total) {
-            vec8 d;
-            z8 z;
+            vec8 d, z;
             __builtin_memcpy(&d, dy + at, sizeof(d));
-            if (small_pre(act)) {
-                vec8 t;
-                __builtin_memcpy(&t, (const T*)pre + at, sizeof(t));
+            __builtin_memcpy(&z, pre + at, sizeof(z));
 #pragma unroll
-                for (int e = 0; e < 8; ++e) z[e] = kept_small<T>(act, t[e]);
-            } else {
-                __builtin_memcpy(&z, (const float*)pre + at, sizeof(z));
-            }
-#pragma unroll
-            for (int e = 0; e < 8; ++e) d[e] = (T)((float)d[e] * act_slope(act, z[e]));
+            for (int e = 0; e < 8; ++e) d[e] *= act_slope(act, z[e]);
             __builtin_memcpy(dz + at, &d, sizeof(d));
         } else {
-            for (long long k = at; k < total; ++k) {
-                const float z = small_pre(act) ? kept_small<T>(act, ((const T*)pre)[k]) : ((const float*)pre)[k];
-                dz[k] = (T)((float)dy[k] * act_slope(act, z));
-            }
+            for (long long k = at; k < total; ++k) dz[k] = dy[k] * act_slope(act, pre[k]);
         }
     }
 }
 
-// float32, any dy
+// any dy
 template <typename T>
-__global__ __launch_bounds__(256) void slope_pass(long long m, long long n, const T* __restrict__ dy, long long lddy, const void* __restrict__ pre,
-                                                  int act, T* __restrict__ dz) {
+__global__ __launch_bounds__(256) void slope_pass(long long m, long long n, const T* __restrict__ dy, long long lddy, const T* __restrict__ pre, int act,
+                                                  T* __restrict__ dz) {
     for (long long at = (long long)blockIdx.x * 256 + threadIdx.x; at < m * n; at += (long long)gridDim.x * 256) {
         const long long j = at / n, i = at - j * n;
-        const float z = small_pre(act) ? kept_small<T>(act, ((const T*)pre)[at]) : ((const float*)pre)[at];
-        dz[at] = (T)((float)dy[j * lddy + i] * act_slope(act, z));
+        dz[at] = dy[j * lddy + i] * act_slope(act, pre[at]);
     }
 }
 
@@ -64,7 +52,7 @@ __global__ __launch_bounds__(256) void slope_pass(long long m, long long n, cons
 // sums are wanted.  Without pre (no activation) dz is dy and only the sums are made, and so without a place for dz.
 template <typename T, int WIDE>
 __global__ __launch_bounds__(256) void slope_sums(long long m, long long n, const T* __restrict__ dy, long long lddy, const void* __restrict__ pre,
-                                                  int act, T* __restrict__ dz, int rows, float* __restrict__ sums) {
+                                                  int act, T* __restrict__ dz, bool split, int rows, float* __restrict__ sums) {
     constexpr int E = 8, STEP = 256 / WIDE;
     __shared__ float part[STEP][WIDE][E + 1];
     const int c = threadIdx.x % WIDE, g = threadIdx.x / WIDE;
@@ -92,9 +80,12 @@ __global__ __launch_bounds__(256) void slope_sums(long long m, long long n, cons
 #pragma unroll
                 for (int e = 0; e < E; ++e) {
                     f[e] *= act_slope(act, z[e]);
-                    split2(f[e], d[e], rest[e]);
+                    if (split) split2(f[e], d[e], rest[e]);
+                    else d[e] = (T)f[e];
                 }
-                if (dz) {
+                if (dz && !split) {
+                    __builtin_memcpy(dz + j * n + i, d, sizeof(d));
+                } else if (dz) {
                     __builtin_memcpy(dz + j * row * 2 + i, d, sizeof(d));
                     __builtin_memcpy(dz + j * row * 2 + row + i, rest, sizeof(rest));
                 }
@@ -112,7 +103,8 @@ __global__ __launch_bounds__(256) void slope_sums(long long m, long long n, cons
                     if (pre) {
                         const long long at = j * n + i + e;
                         f *= act_slope(act, small_pre(act) ? kept_small<T>(act, ((const T*)pre)[at]) : ((const float*)pre)[at]);
-                        if (dz) split2(f, dz[j * row * 2 + i + e], dz[j * row * 2 + row + i + e]);
+                        if (dz && !split) dz[at] = (T)f;
+                        else if (dz) split2(f, dz[j * row * 2 + i + e], dz[j * row * 2 + row + i + e]);
                     }
                     s[e] += f;
                 }
@@ -131,11 +123,11 @@ __global__ __launch_bounds__(256) void slope_sums(long long m, long long n, cons
 
 // As many columns side by side as there are: 131 072 x 128 bf16 19.4 us (dw and db together 56; 67 with 32 wherever n is).
 template <typename T, int WIDE = 32>
-inline hipError_t launch_slope_sums(long long m, long long n, const T* dy, long long lddy, const void* pre, int act, T* dz, int rows, float* sums, hipStream_t st) {
+inline hipError_t launch_slope_sums(long long m, long long n, const T* dy, long long lddy, const void* pre, int act, T* dz, bool split, int rows, float* sums, hipStream_t st) {
     if constexpr (WIDE > 2) {
-        if (n <= WIDE * 4) return launch_slope_sums<T, WIDE / 2>(m, n, dy, lddy, pre, act, dz, rows, sums, st);
+        if (n <= WIDE * 4) return launch_slope_sums<T, WIDE / 2>(m, n, dy, lddy, pre, act, dz, split, rows, sums, st);
     }
-    hipLaunchKernelGGL((slope_sums<T, WIDE>), dim3((unsigned)tiles_of(n, WIDE * 8), (unsigned)tiles_of(m, rows)), dim3(256), 0, st, m, n, dy, lddy, pre, act, dz, rows, sums);
+    hipLaunchKernelGGL((slope_sums<T, WIDE>), dim3((unsigned)tiles_of(n, WIDE * 8), (unsigned)tiles_of(m, rows)), dim3(256), 0, st, m, n, dy, lddy, pre, act, dz, split, rows, sums);
     return hipGetLastError();
 }
 
@@ -227,7 +219,6 @@ inline hipError_t launch_add_splits(const float* partial, int splits, long long 
     return hipGetLastError();
 }
 
-
 template <typename T, int EPI, int PL, int QL, int SRC, int BI, int BJ, int WI, int WJ>
 inline hipError_t launch_product(ProductArgs<T> a, int splits, hipStream_t st) {
     const long long ti = tiles_of(a.ni, BI), tiles = ti * tiles_of(a.nj, BJ);
@@ -305,11 +296,11 @@ inline WeightPlan weight_plan(int bk, bool wide, bool two, bool split, long long
 inline bool wide_weights(int size, long long m, long long n, long long k) {
     return size == 2 && k >= 256 && n >= 128 && k % 8 == 0 && n % 8 == 0 && m >= 4096;
 }
-// Rows a workgroup of slope_sums takes: 128, or 32 where that would be less than two workgroups a CU (with whole vectors in the rows
-// of pieces, 10 007 x 258 -> 255 bf16, dz and dx: 36 us, 82 without both); more where there would be more than 32768 strips (a
+// Rows a workgroup of slope_sums takes: 128, or 32 where that would be less than four workgroups a CU (65 536 x 256 -> 256 bf16 relu,
+// all gradients: 66 us, 79 with 128; 65 536 x 512 -> 512 silu 213 and 206); more where there would be more than 32768 strips (a
 // grid's second dimension ends at 65535).
 inline int strip_rows(long long m, long long n) {
-    const long long rows = tiles_of(m, 128) * tiles_of(n, 256) < 512 ? 32 : 128;
+    const long long rows = tiles_of(m, 128) * tiles_of(n, 256) < 1024 ? 32 : 128;
     return (int)std::max(rows, tiles_of(tiles_of(m, 32768), 8) * 8);
 }
 
@@ -321,16 +312,18 @@ inline long long round_up(long long n) { return (n + 255) / 256 * 256; }
 
 template <typename T>
 struct LinearRun {
-    static bool two_pieces(int act) { return sizeof(T) == 2 && act != MPE_ACT_NONE; }
     // dz as an array of its own in 16-bit types: its column sums are taken while it is made
-    static bool split_dz(int act, long long k) { return sizeof(T) == 2 && own_dz(act, k); }
+    static bool own_sums(int act, long long k) { return sizeof(T) == 2 && own_dz(act, k); }
+    // relu's is dy or zero, which one number of the type holds
+    static bool split_dz(int act, long long k) { return own_sums(act, k) && act != MPE_ACT_RELU; }
+    static bool two_pieces(int act, long long k) { return split_dz(act, k) || (sizeof(T) == 2 && act != MPE_ACT_NONE && !own_dz(act, k)); }
 
     static long long backward_workspace(int act, long long m, long long n, long long k) {
         if (m == 0) return 0;
-        const WeightPlan p = weight_plan(Piece<T>::BK, false, two_pieces(act), split_dz(act, k), m, n, k);
+        const WeightPlan p = weight_plan(Piece<T>::BK, false, two_pieces(act, k), split_dz(act, k), m, n, k);
         const long long strips = tiles_of(m, strip_rows(m, n)) * n;
-        long long sums = p.splits * n * k + (split_dz(act, k) ? strips : p.splits * n);
-        if (wide_weights(sizeof(T), m, n, k)) sums = std::max(sums, weight_plan(Piece<T>::BK, true, two_pieces(act), split_dz(act, k), m, n, k).splits * n * k + strips);
+        long long sums = p.splits * n * k + (own_sums(act, k) ? strips : p.splits * n);
+        if (wide_weights(sizeof(T), m, n, k)) sums = std::max(sums, weight_plan(Piece<T>::BK, true, two_pieces(act, k), split_dz(act, k), m, n, k).splits * n * k + strips);
         return (own_dz(act, k) ? round_up(dz_elements<T>(m, n) * (long long)sizeof(T)) : 0) + sums * 4;
     }
 
@@ -372,21 +365,23 @@ struct LinearRun {
         const bool wide = wide_weights(sizeof(T), a.m, a.n, a.k) && wide_operand(x, O_INNER, a.k) && (own || wide_operand(dz, O_INNER, a.n));
         char* const ws = (char*)a.ws;
         float* const partial = (float*)(ws + (own ? round_up(dz_elements<T>(a.m, a.n) * (long long)sizeof(T)) : 0));
-        const WeightPlan p = weight_plan(Piece<T>::BK, wide, two_pieces(a.act), split, a.m, a.n, a.k);
+        const WeightPlan p = weight_plan(Piece<T>::BK, wide, two_pieces(a.act, a.k), split, a.m, a.n, a.k);
         const int strip = strip_rows(a.m, a.n), strips = (int)tiles_of(a.m, strip);
         const bool products = a.dx || a.dw;
-        float* const sums = a.db && (wide || split) ? partial + p.splits * a.n * a.k : nullptr;
-        if (sums || (split && products)) {
+        const bool own_16 = own_sums(a.act, a.k);
+        float* const sums = a.db && (wide || own_16) ? partial + p.splits * a.n * a.k : nullptr;
+        if (sums || (own_16 && products)) {
             if constexpr (sizeof(T) == 2)
-                e = launch_slope_sums<T>(a.m, a.n, (const T*)a.dy, a.lddy, own ? (const void*)a.pre : nullptr, act, products ? (T*)ws : nullptr, strip, sums, st);
-        } else if (own && products && a.lddy == a.n) {
-            const long long want = (a.m * a.n + 2047) / 2048;
-            hipLaunchKernelGGL((slope_flat<T>), dim3((unsigned)(want < 8192 ? want : 8192)), dim3(256), 0, st, a.m * a.n, (const T*)a.dy, (const void*)a.pre, act, (T*)ws);
-            e = hipGetLastError();
+                e = launch_slope_sums<T>(a.m, a.n, (const T*)a.dy, a.lddy, own ? (const void*)a.pre : nullptr, act, products ? (T*)ws : nullptr, split, strip, sums, st);
         } else if (own && products) {
-            const long long want = (a.m * a.n + 255) / 256;
-            hipLaunchKernelGGL((slope_pass<T>), dim3((unsigned)(want < 8192 ? want : 8192)), dim3(256), 0, st, a.m, a.n, (const T*)a.dy, a.lddy, (const void*)a.pre, act, (T*)ws);
-            e = hipGetLastError();
+            if constexpr (sizeof(T) == 4) {
+                const bool dense = a.lddy == a.n;
+                const long long want = dense ? (a.m * a.n + 2047) / 2048 : (a.m * a.n + 255) / 256;
+                const dim3 grid((unsigned)(want < 8192 ? want : 8192));
+                if (dense) hipLaunchKernelGGL((slope_flat<float>), grid, dim3(256), 0, st, a.m * a.n, (const float*)a.dy, (const float*)a.pre, act, (float*)ws);
+                else hipLaunchKernelGGL((slope_pass<float>), grid, dim3(256), 0, st, a.m, a.n, (const float*)a.dy, a.lddy, (const float*)a.pre, act, (float*)ws);
+                e = hipGetLastError();
+            }
         }
         if (e != hipSuccess) return e;
         const long long row = piece_row(a.n);

@@ -242,3 +242,19 @@ def test_captured_gradients_replay(m, k, n, dt):
         for out in outs:
             assert all(torch.equal(p, q) for p, q in zip(out, want)), i
         torch.cuda.synchronize()
+
+
+@pytest.mark.parametrize("dt", HALVES)
+@pytest.mark.parametrize("m,k,n,ld", SHAPES)
+def test_relus_dz_is_exact_in_one_piece(m, k, n, ld, dt):
+    """dy or zero: sums of one term are products rounded once, and dense ones are off by no more than their float32 order."""
+    import mpe_hip
+    x, w, b, dy = make(m, k, n, dt, ld, seed=6)
+    leaves = [t.detach().clone().requires_grad_(True) for t in (x, w, b)]
+    y = mpe_hip.linear(*leaves, "relu")
+    dx, dw, db = torch.autograd.grad(y, leaves, dy)
+    dz = torch.where(y.detach() > 0, dy, torch.zeros_like(dy)).double()
+    xd, wd = x.double(), w.double()
+    for got, want, mag, terms in ((dx, dz @ wd, dz.abs() @ wd.abs(), n), (dw, dz.T @ xd, dz.abs().T @ xd.abs(), m), (db, dz.sum(0), dz.abs().sum(0), m)):
+        off = (terms + 8) * V * mag
+        assert ((got.double() - want).abs() <= off + U[dt] * (want.abs() + off) + TINY[dt]).all()
