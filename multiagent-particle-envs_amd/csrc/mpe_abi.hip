@@ -777,7 +777,8 @@ static PpoArgs ppo_args(int dtype, int64_t rows, int64_t v, const void* logits, 
     PpoArgs a = {};
     a.dtype = dtype; a.rows = rows; a.v = v; a.logits = logits; a.ld = ld; a.actions = actions; a.action_bytes = action_bytes;
     a.old_logp = old_logp; a.adv = adv; a.mask = mask; a.ldm = ldm; a.weights = weights; a.values = values; a.old_values = old_values; a.returns = returns;
-    a.clip = (float)clip; a.value_clip = (float)value_clip; a.value_coef = (float)value_coef; a.entropy_coef = (float)entropy_coef;
+    a.clip = clip < 0.0 ? -1.0f : (float)clip; a.value_clip = value_clip < 0.0 ? -1.0f : (float)value_clip;     // a sign that float32 keeps
+    a.value_coef = (float)value_coef; a.entropy_coef = (float)entropy_coef;
     return a;
 }
 

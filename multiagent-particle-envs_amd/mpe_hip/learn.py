@@ -47,10 +47,10 @@ def linear(x, weight, bias=None, activation=None, residual=None):
     ``x`` ``[..., k]`` (rows may be strided: ``env.obs_n[i]`` is taken as it lies), ``weight`` ``[n, k]``, ``bias`` ``[n]``,
     ``residual`` of the result's shape ``[..., n]`` (an expanded tensor will do); all of one type (float32, bfloat16,
     float16) on one GPU.  ``activation``: None / "none", "tanh", "relu", "gelu" (by erf) or "silu".  Sums are in float32 or
-    better, with one rounding to the type at the end; float32 products are as exact as float32 multiplications
-    (of numbers above 2^-109 or so).  For the backward pass float32 and float16 keep float32 pre-activations, bfloat16 keeps the slopes in float16 (nothing is kept for
-    none, and for relu and float32 tanh without residual); 16-bit gradients are sums of dz with twice the type's bits, rounded
-    once."""
+    better, with one rounding to the type at the end; float32 products are as exact as float32 multiplications, of numbers
+    above 2^-109.  For the backward pass float32 and float16 keep float32 pre-activations, bfloat16 keeps the slopes in float16
+    (nothing is kept for none, and for relu and float32 tanh without residual); 16-bit gradients are sums of dz with twice the
+    type's bits, rounded once."""
     try:
         act = ACTIVATIONS[activation]
     except (KeyError, TypeError):

@@ -97,3 +97,18 @@ def test_every_negative_value_clip_is_refused():
         with pytest.raises(ValueError, match="value_clip"):
             mpe_hip.ppo_loss(**d, value_clip=bad)
     assert torch.equal(mpe_hip.ppo_loss(**d, value_clip=math.inf)[0], mpe_hip.ppo_loss(**d)[0])
+
+
+def test_a_value_clip_below_zero_by_less_than_float32_holds_does_not_clip():
+    """Behind the C boundary, where every negative value_clip means none."""
+    from mpe_hip import _lib
+    lib, d = _lib.load(), make(5)
+    def stats(value_clip):
+        loss, out, ws = torch.empty(1, device=DEV), torch.empty(6, device=DEV), torch.empty(_lib.PPO_WORKSPACE_BYTES, dtype=torch.uint8, device=DEV)
+        p = {k: t.contiguous().data_ptr() for k, t in d.items()}
+        assert lib.mpe_ppo_loss_forward(0, _lib.MPE_F32, ROWS, 5, p["logits"], 5, p["actions"], 4, p["old_logp"], p["advantages"], None, 0, None, p["values"], p["old_values"],
+                                        p["returns"], 0.2, value_clip, 0.5, 0.01, loss.data_ptr(), out.data_ptr(), ws.data_ptr(), ws.numel(),
+                                        torch.cuda.current_stream().cuda_stream) == 0
+        torch.cuda.synchronize()
+        return out
+    assert torch.equal(stats(-1e-60), stats(-1.0)) and not torch.equal(stats(0.0), stats(-1.0))

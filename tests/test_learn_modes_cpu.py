@@ -23,3 +23,10 @@ def test_tensors_with_a_forward_mode_tangent_are_refused():
                     call()
             with fw._set_fwd_grad_enabled(False), pytest.raises(ValueError, match="GPU"):
                 call()
+
+
+def test_a_clip_below_zero_by_less_than_float32_holds_is_refused():
+    from test_learn_cpu import _lib, _ppo
+    _, lib = _lib()
+    for bad in (-1e-60, -1e-46):
+        assert _ppo(lib, clip=bad) == -1 and "clip" in lib.mpe_last_error(None).decode()
