@@ -50,9 +50,9 @@ __global__ __launch_bounds__(256) void slope_pass(long long m, long long n, cons
 // The same for 16-bit types, with the column sums of dz before it is rounded (the bias's gradient would see every rounding where
 // its terms cancel): a workgroup takes 8 WIDE columns (WIDE up to 32, by n) of `rows` rows and leaves sums[blockIdx.y][n], where
 // sums are wanted.  Without pre (no activation) dz is dy and only the sums are made, and so without a place for dz.
-template <typename T, int WIDE>
+template <typename T, bool SPLIT, int WIDE>
 __global__ __launch_bounds__(256) void slope_sums(long long m, long long n, const T* __restrict__ dy, long long lddy, const void* __restrict__ pre,
-                                                  int act, T* __restrict__ dz, bool split, int rows, float* __restrict__ sums) {
+                                                  int act, T* __restrict__ dz, int rows, float* __restrict__ sums) {
     constexpr int E = 8, STEP = 256 / WIDE;
     __shared__ float part[STEP][WIDE][E + 1];
     const int c = threadIdx.x % WIDE, g = threadIdx.x / WIDE;
@@ -80,10 +80,10 @@ __global__ __launch_bounds__(256) void slope_sums(long long m, long long n, cons
 #pragma unroll
                 for (int e = 0; e < E; ++e) {
                     f[e] *= act_slope(act, z[e]);
-                    if (split) split2(f[e], d[e], rest[e]);
+                    if (SPLIT) split2(f[e], d[e], rest[e]);
                     else d[e] = (T)f[e];
                 }
-                if (dz && !split) {
+                if (dz && !SPLIT) {
                     __builtin_memcpy(dz + j * n + i, d, sizeof(d));
                 } else if (dz) {
                     __builtin_memcpy(dz + j * row * 2 + i, d, sizeof(d));
@@ -103,7 +103,7 @@ __global__ __launch_bounds__(256) void slope_sums(long long m, long long n, cons
                     if (pre) {
                         const long long at = j * n + i + e;
                         f *= act_slope(act, small_pre(act) ? kept_small<T>(act, ((const T*)pre)[at]) : ((const float*)pre)[at]);
-                        if (dz && !split) dz[at] = (T)f;
+                        if (dz && !SPLIT) dz[at] = (T)f;
                         else if (dz) split2(f, dz[j * row * 2 + i + e], dz[j * row * 2 + row + i + e]);
                     }
                     s[e] += f;
@@ -122,12 +122,12 @@ __global__ __launch_bounds__(256) void slope_sums(long long m, long long n, cons
 }
 
 // As many columns side by side as there are: 131 072 x 128 bf16 19.4 us (dw and db together 56; 67 with 32 wherever n is).
-template <typename T, int WIDE = 32>
-inline hipError_t launch_slope_sums(long long m, long long n, const T* dy, long long lddy, const void* pre, int act, T* dz, bool split, int rows, float* sums, hipStream_t st) {
+template <typename T, bool SPLIT, int WIDE = 32>
+inline hipError_t launch_slope_sums(long long m, long long n, const T* dy, long long lddy, const void* pre, int act, T* dz, int rows, float* sums, hipStream_t st) {
     if constexpr (WIDE > 2) {
-        if (n <= WIDE * 4) return launch_slope_sums<T, WIDE / 2>(m, n, dy, lddy, pre, act, dz, split, rows, sums, st);
+        if (n <= WIDE * 4) return launch_slope_sums<T, SPLIT, WIDE / 2>(m, n, dy, lddy, pre, act, dz, rows, sums, st);
     }
-    hipLaunchKernelGGL((slope_sums<T, WIDE>), dim3((unsigned)tiles_of(n, WIDE * 8), (unsigned)tiles_of(m, rows)), dim3(256), 0, st, m, n, dy, lddy, pre, act, dz, split, rows, sums);
+    hipLaunchKernelGGL((slope_sums<T, SPLIT, WIDE>), dim3((unsigned)tiles_of(n, WIDE * 8), (unsigned)tiles_of(m, rows)), dim3(256), 0, st, m, n, dy, lddy, pre, act, dz, rows, sums);
     return hipGetLastError();
 }
 
@@ -371,8 +371,11 @@ struct LinearRun {
         const bool own_16 = own_sums(a.act, a.k);
         float* const sums = a.db && (wide || own_16) ? partial + p.splits * a.n * a.k : nullptr;
         if (sums || (own_16 && products)) {
-            if constexpr (sizeof(T) == 2)
-                e = launch_slope_sums<T>(a.m, a.n, (const T*)a.dy, a.lddy, own ? (const void*)a.pre : nullptr, act, products ? (T*)ws : nullptr, split, strip, sums, st);
+            if constexpr (sizeof(T) == 2) {
+                T* const to = products ? (T*)ws : nullptr;
+                if (split) e = launch_slope_sums<T, true>(a.m, a.n, (const T*)a.dy, a.lddy, a.pre, act, to, strip, sums, st);
+                else e = launch_slope_sums<T, false>(a.m, a.n, (const T*)a.dy, a.lddy, own ? (const void*)a.pre : nullptr, act, to, strip, sums, st);
+            }
         } else if (own && products) {
             if constexpr (sizeof(T) == 4) {
                 const bool dense = a.lddy == a.n;
