@@ -21,9 +21,9 @@
 //
 // What bounds it.  float32, 65 536 x 1024 -> 1024: 699 us, 197 TFLOP/s of float32 where the library's own instruction reaches
 // 154: six matrix instructions a product, and 5.5 vector instructions an element of a tile to split it.  Narrow layers,
-// 196 608 x 64 -> 64 f32 tanh: memory, 100 MB in 28.4 us (3.5 TB/s), dx 150 MB in 35.4 (4.2), dw and db 150 MB in 31.5 and 7.5 for
-// the sum of the splits.  In between, 10 007 x 258 -> 255 f32: 24.4, 20 and 21 us, a chain of nine dependent steps on 2.5 workgroups
-// a CU.
+// 196 608 x 64 -> 64 f32 tanh: memory, 100 MB in 28.0 us (3.6 TB/s), dx 150 MB in 35.5 (4.2), dw and db 150 MB in 30.5 and 7.4 for
+// the sum of the splits; bf16 21, 30.5 and 31.5.  In between, 10 007 x 258 -> 255 f32: 25, 20 and 20 us, a chain of nine dependent steps
+// on 2.5 workgroups a CU.  Of the 16-bit tiles those of two pieces and the weights' 128 x 128 keep some registers in memory.
 #pragma once
 #include "mpe_learn.hpp"
 

@@ -49,7 +49,8 @@ __global__ __launch_bounds__(256) void slope_pass(long long m, long long n, cons
 
 // The same for 16-bit types, with the column sums of dz before it is rounded (the bias's gradient would see every rounding where
 // its terms cancel): a workgroup takes 8 WIDE columns (WIDE up to 32, by n) of `rows` rows and leaves sums[blockIdx.y][n], where
-// sums are wanted.  Without pre (no activation) dz is dy and only the sums are made, and so without a place for dz.
+// sums are wanted.  Without pre (no activation) dz is dy and only the sums are made, and so without a place for dz.  65 536 x 1024
+// bf16 gelu: 537 MB in 97 us, 5.5 TB/s (part of it stays in the Infinity Cache).
 template <typename T, bool SPLIT, int WIDE>
 __global__ __launch_bounds__(256) void slope_sums(long long m, long long n, const T* __restrict__ dy, long long lddy, const void* __restrict__ pre,
                                                   int act, T* __restrict__ dz, int rows, float* __restrict__ sums) {
@@ -238,8 +239,8 @@ inline hipError_t launch_product(ProductArgs<T> a, int splits, hipStream_t st) {
 
 // Tiles of the products that write rows of m.  16-bit types that fill every CU with a wide tile: product_wide (65 536 x 1024 ->
 // 1024 bf16 155 us against 199 forward; dz in two pieces and dx 350 against 467, 16 384 x 512 -> 256, 256 tiles, 44 against 46; with
-// 128 wide tiles a forward pass takes 21 us both ways, with 64 it is 20 against 13).  Others by the output's width.  Up to 64 columns: 64 x 64 (196 608 x 64 -> 64 f32 28.4 us
-// forward and 35.4 for dx, against 30.4 and 36.5 with 64 x 128).
+// 128 wide tiles a forward pass takes 21 us both ways, with 64 it is 20 against 13).  Others by the output's width.  Up to 64
+// columns: 64 x 64 (196 608 x 64 -> 64 f32 28 us forward and 35.5 for dx, against 30.4 and 36.5 with 64 x 128).
 template <typename T, int EPI, int PL, int QL, int SRC>
 inline hipError_t launch_rows(const ProductArgs<T>& a, hipStream_t st) {
     if constexpr (sizeof(T) == 2 && SRC != SRC_DZ) {
@@ -305,7 +306,8 @@ inline int strip_rows(long long m, long long n) {
 }
 
 // Wide inputs: dz becomes an array of its own, where it would otherwise be worked out in every tile of k of both products
-// (131 072 x 128 -> 128 gelu, both gradients: bf16 68 us against 116, f32 148 against 177; x 64 -> 64 bf16 57 against 54).
+// (131 072 x 128 -> 128 gelu, both gradients: bf16 75 us against 116, f32 140 against 177; at the border, x 64 -> 64, about even: bf16 57
+// with an array and 54 without, f32 61 and 63; over 524 288 rows 139 and 154, 196 and 209).
 inline bool own_dz(int act, long long k) { return act != MPE_ACT_NONE && k > 64; }
 
 inline long long round_up(long long n) { return (n + 255) / 256 * 256; }

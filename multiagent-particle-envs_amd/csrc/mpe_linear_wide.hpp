@@ -4,9 +4,10 @@
 // with 73 KB of LDS and half the registers two workgroups share a CU and one's results leave while the other multiplies.
 //
 // What bounds it (65 536 x 1024 -> 1024 bf16, 137 GFLOP): without activation 141 us, 0.97 PFLOP/s, where a large library product
-// reaches 1.31.  A step's matrix instructions take 512 cycles of every SIMD, its 72 KB of LDS traffic 562 cycles of the CU, so
-// LDS and the matrix cores are about equally busy; with gelu, its slope and a residual 231 us, where a quarter of the vector
-// unit's time goes into 28 instructions an element and the clock drops by a tenth in a longer run.
+// reaches 1.31.  Nothing is saturated: by the counters the matrix cores are busy for 26 % of the cycles of a forward pass with gelu,
+// its slope and a residual (232 us), for 48 % of dx's with dz in two pieces (272 us for 275 GFLOP) and for 56 % of the weight
+// gradient's (230 us, where LDS conflicts take a fifth of the cycles).  The rest are waits, and the ends of a tile, which only the
+// CU's other workgroup covers: two stages of copies before its first product, activations and stores behind its last.
 //
 // An operand whose contiguous index is the output's lies in LDS as it lies in memory, and ds_read_b64_tr_b16 turns it: 16
 // lanes read four rows of 16 elements and each gets one column.
