@@ -31,6 +31,25 @@ def test_every_subset_gives_the_same_bits(m, k, n, act, dt):
         assert all(q is None or torch.equal(q, f) for q, f in zip(got, full)), need
 
 
+@pytest.mark.parametrize("dt", DTYPES)
+@pytest.mark.parametrize("act", ["none", "silu"])
+@pytest.mark.parametrize("m,k,n", [(40, 6, 9), (1000, 14, 64), (3001, 258, 255), (8200, 320, 1032)])
+def test_subsets_with_upstream_gradients_that_are_not_rows(m, k, n, act, dt):
+    """One row for all, columns of a wider tensor, a transposed one: the same bits from every subset (their alignment may choose another
+    kernel than a contiguous tensor's)."""
+    import mpe_hip
+    g = torch.Generator(DEV).manual_seed(m + k + n)
+    x, w, b, wide = [torch.randn(*s, device=DEV, generator=g).to(dt) for s in ((m, k), (n, k), (n,), (m, n + 3))]
+    for dy in (wide[:1, :n].expand(m, n), wide[:, 1:n + 1], wide[:, :n].T.contiguous().T):
+        def grads(need, up):
+            leaves = [t.detach().clone().requires_grad_(q) for t, q in zip((x, w, b), need)]
+            got = iter(torch.autograd.grad(mpe_hip.linear(*leaves, act), [t for t in leaves if t.requires_grad], up))
+            return [next(got) if q else None for q in need]
+        want = grads((True, True, True), dy)
+        for need in ((False, False, True), (True, False, True), (False, True, False), (True, False, False)):
+            assert all(q is None or torch.equal(q, f) for q, f in zip(grads(need, dy), want)), need
+
+
 @pytest.mark.parametrize("m,k,n,act,dt", [(65536, 1024, 1024, "none", torch.float32), (65536, 1024, 1024, "none", torch.bfloat16), (65536, 512, 512, "gelu", torch.float32),
                                           (65536, 512, 500, "gelu", torch.float16)])
 def test_a_bias_alone_costs_no_product(m, k, n, act, dt):
