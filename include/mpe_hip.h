@@ -473,7 +473,7 @@ int mpe_linear_backward(int device, int dtype, int activation, int64_t m, int64_
  *   old_logp    float[rows]     log-probability of the action when the rollout was collected
  *   adv         float[rows]     advantages (mpe_gae)
  *   mask        uint8[rows][v], row stride ldm >= v, or NULL: 0 forbids the word
- *   weights     float[rows] or NULL (all 1)
+ *   weights     float[rows], none negative, or NULL (all 1)
  *   values, old_values, returns  float[rows], all three or none
  * Per row, over the allowed words: lp = log softmax(logits)[action], q = exp(lp - old_logp), H the entropy,
  *   s = min(q adv, clamp(q, 1 - clip, 1 + clip) adv),

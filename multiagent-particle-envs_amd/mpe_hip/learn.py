@@ -64,8 +64,8 @@ def ppo_loss(logits, actions, old_logp, advantages, values=None, old_values=None
 
     ``logits`` ``[..., v]`` (float32, bfloat16, float16; rows may be strided); everything else has its leading shape:
     ``actions`` int32 / int64, ``old_logp`` and ``advantages`` float32, optionally ``values``, ``old_values`` and
-    ``returns`` float32 (together), ``action_mask`` bool / uint8 ``[..., v]`` (0 forbids a move) and ``weights`` float32 /
-    bool.  Per decision, with the softmax over the allowed moves: ``q = exp(logp - old_logp)``,
+    ``returns`` float32 (together), ``action_mask`` bool / uint8 ``[..., v]`` (0 forbids a move) and ``weights`` float32
+    (none negative) / bool.  Per decision, with the softmax over the allowed moves: ``q = exp(logp - old_logp)``,
     ``s = min(q A, clamp(q, 1 - clip, 1 + clip) A)``, the entropy ``H`` and the value loss
     ``u = max((V - R)^2, (V0 + clamp(V - V0, -value_clip, value_clip) - R)^2) / 2`` (``value_clip`` None: ``(V - R)^2 / 2``);
     ``loss = sum w (-s + value_coef u - entropy_coef H) / sum w``.
